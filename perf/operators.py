@@ -284,7 +284,7 @@ def run(state):
         if case["kind"] == "append":
             q = ap.kv4_append(state["kv"], state["batch"], state["k"], state["v"], q=state["q"], q_norm=state["q_norm"],
                               k_norm=state["k_norm"], eps=1e-6, rotary=state["rotary"], interleaved=case["interleaved"])
-            return (q,) + ap.kv4_read(state["kv"], state["batch"])
+            return (q,) + ap.kv4_read(state["kv"], state["batch"], state["T"])
         return ap.kv4_attention(state["kv"], state["batch"], state["q"], causal=case["causal"], window=case["window"],
                                 lse=case["lse"], workspace=state["workspace"])
     if case["kind"] == "linear":
