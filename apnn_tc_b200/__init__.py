@@ -13,5 +13,8 @@ from .ops import (  # noqa: F401
     apconv, apmm, conv_check, conv_workspace_bytes, apmm_w1a2, apmm_w1a2_decompose, apmm_w1a3, apmm_w1a4, apmm_w2a2, apmm_w2a2_decompose, expand_planes, expand_planes_fp4, gemm_fp4, gemm_i8, gemm_w8,
     gemm_check, gemm_workspace_bytes, images_quantization, make_epilogue,
 )
+from .decoder import (  # noqa: F401
+    KVBatch, KVCache4, kv4_append, kv4_attention, kv4_attention_check, kv4_attention_workspace_bytes, kv4_read, linear_planes,
+)
 
 __all__ = [n for n in dir() if not n.startswith("_")]

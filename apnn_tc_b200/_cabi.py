@@ -18,6 +18,8 @@ ROWS_I8, ROWS_FP4 = 1, 2   # Epilogue.out_i8: one byte, or one e2m1 nibble, per 
 SIGN_NONE, SIGN_W, SIGN_X = 0, 1, 2
 POOL_NONE, POOL_AVG2, POOL_MAX2 = 0, 1, 2
 ALGO_AUTO, ALGO_BMMA, ALGO_IMMA, ALGO_TCGEN05, ALGO_TCGEN05_PAIR = 0, 1, 2, 3, 4
+TYPE_BF16, TYPE_FP16, TYPE_FP32 = 0, 1, 2
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 ALGOS = {"auto": ALGO_AUTO, "bmma": ALGO_BMMA, "imma": ALGO_IMMA, "tcgen05": ALGO_TCGEN05, "tcgen05_pair": ALGO_TCGEN05_PAIR}
 
 # every symbol the header declares; the CPU test-suite checks the library exports them all
@@ -27,6 +29,8 @@ EXPORTS = (
     "apnn_conv2d_workspace_bytes", "apnn_conv2d_check", "apnn_conv2d_i8", "apnn_bit_compress", "apnn_quantize_pack", "apnn_quantize_im2col", "apnn_create",
     "apnn_destroy", "apnn_gemm_host", "apnn_conv2d_host", "apnn_probe_peak", "apnn_quantize_im2col_i8", "apnn_quantize_window_rows_i8", "apnn_quantize_blocks_i8", "apnn_maxpool2x2_i8", "apnn_requantize_i32",
     "apnn_conv2d_fp4", "apnn_linear_fp4", "apnn_gemm_planes", "apnn_conv2d_i8_to_fp4", "apnn_maxpool2x2_rows",
+    "apnn_linear_planes", "apnn_kv4_append", "apnn_kv4_read", "apnn_kv4_attention", "apnn_kv4_attention_workspace_bytes",
+    "apnn_kv4_attention_check",
 )
 
 
@@ -54,6 +58,48 @@ class Epilogue(ctypes.Structure):
     def __init__(self, *args, **kw):
         super().__init__(*args, **kw)
         self.struct_size = ctypes.sizeof(Epilogue)
+
+
+class _Sized(ctypes.Structure):
+    """A descriptor whose first member records its size."""
+    def __init__(self, *args, **kw):
+        super().__init__(*args, **kw)
+        self.struct_size = ctypes.sizeof(self)
+
+
+class LinearDesc(_Sized):
+    """``apnn_linear_desc``"""
+    _fields_ = [("struct_size", ctypes.c_uint32), ("x_type", ctypes.c_int32), ("out_type", ctypes.c_int32), ("activation", ctypes.c_int32),
+                ("zero", ctypes.c_float), ("scale", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p),
+                ("ldx", ctypes.c_int64), ("ldo", ctypes.c_int64), ("ldr", ctypes.c_int64)]
+
+
+class Kv4Cache(_Sized):
+    """``apnn_kv4_cache``"""
+    _fields_ = [("struct_size", ctypes.c_uint32), ("type", ctypes.c_int32), ("data", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+                ("pages", ctypes.c_int32), ("heads", ctypes.c_int32), ("page_size", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+class Kv4Batch(_Sized):
+    """``apnn_kv4_batch``"""
+    _fields_ = [("struct_size", ctypes.c_uint32), ("sequences", ctypes.c_int32), ("cu_q", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
+                ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int32), ("max_q", ctypes.c_int32)]
+
+
+class Kv4AppendArgs(_Sized):
+    """``apnn_kv4_append_args``"""
+    _fields_ = [("struct_size", ctypes.c_uint32), ("rows", ctypes.c_int32), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64), ("q", ctypes.c_void_p), ("q_out", ctypes.c_void_p),
+                ("q_stride", ctypes.c_int64), ("q_out_stride", ctypes.c_int64), ("q_heads", ctypes.c_int32),
+                ("rotary_dim", ctypes.c_int32), ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_double),
+                ("interleaved", ctypes.c_int32), ("rotary", ctypes.c_void_p), ("rotary_rows", ctypes.c_int32)]
+
+
+class Kv4AttentionArgs(_Sized):
+    """``apnn_kv4_attention_args``"""
+    _fields_ = [("struct_size", ctypes.c_uint32), ("rows", ctypes.c_int32), ("q", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("lse", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64), ("q_heads", ctypes.c_int32),
+                ("causal", ctypes.c_int32), ("window", ctypes.c_int32), ("scale", ctypes.c_float)]
 
 
 class ApnnError(RuntimeError):
@@ -115,6 +161,13 @@ def lib() -> ctypes.CDLL:
     L.apnn_destroy.argtypes = [vp]
     L.apnn_gemm_host.argtypes = [vp, i, i, i, vp, vp, vp, i, i, i, ep]
     L.apnn_conv2d_host.argtypes = [vp, i, i, vp, vp, vp, i, i, i, i, i, i, i, ep]
+    L.apnn_linear_planes.argtypes = [vp, i, vp, vp, vp, i, i, i, vp, vp]
+    L.apnn_kv4_append.argtypes = [vp, vp, vp, vp]
+    L.apnn_kv4_read.argtypes = [vp, vp, vp, vp, vp, i]
+    L.apnn_kv4_attention_workspace_bytes.restype = sz
+    L.apnn_kv4_attention_workspace_bytes.argtypes = [vp, vp, i]
+    L.apnn_kv4_attention.argtypes = [vp, vp, vp, vp, vp, sz]
+    L.apnn_kv4_attention_check.argtypes = [vp, vp]
     _lib = L
     return L
 

@@ -381,6 +381,133 @@ apnn_status apnn_quantize_window_rows_i8(void *stream, const float *images, void
 apnn_status apnn_quantize_blocks_i8(void *stream, const float *images, void *out_i8, int B, int H, int W,
                                     int C, int stride, int bits, int halo, int cpad);
 
+/* ---- low-bit decoder layers ------------------------------------------------------
+ * No counterpart in the reference, which runs convolutional networks only: the operators that a language model's
+ * layer needs around weights of a few bits and a cache of 4-bit keys and values.  All on the caller's stream and the
+ * current device, capturable, no allocation; tensors are the caller's. */
+enum { APNN_TYPE_BF16 = 0, APNN_TYPE_FP16 = 1, APNN_TYPE_FP32 = 2 };
+enum {
+  APNN_ACT_NONE = 0,
+  APNN_ACT_RELU = 1,
+  APNN_ACT_SILU = 2,     /* v / (1 + exp(-v)) */
+  APNN_ACT_GELU = 3,     /* v/2 (1 + erf(v / sqrt 2)) */
+  APNN_ACT_GELU_TANH = 4 /* v/2 (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) */
+};
+
+/* Matrix product over weight planes with bias, activation and residual in its epilogue:
+ *   Out[m][n] = act( scale[n] * sum_k X[m][k] * (level[n][k] - zero) + bias[n] ) + residual[m][n]
+ * W[wbits][N][PAD128(K)/32] as apnn_bit_compress writes the levels [N][K] (wbits 1..4), X[M][K] of 16-bit floats with
+ * rows ldx elements apart, Out and residual with rows ldo and ldr apart.  Sums in 32 bits, one rounding at the store.
+ * zero: a multiple of 1/2 in 0..15, so that level - zero is exact in either type (1/2 with one plane: weights of
+ * -scale/2 and +scale/2; (2^wbits - 1)/2: symmetric levels).  bias and residual may be null; residual may be Out itself
+ * (same stride).  Values of X that are not finite make their row NaN or infinite and touch no other row.
+ * Rules: W, X 16-byte aligned, ldx a multiple of 8; Out and residual aligned to their element; M, N, K >= 1 (ragged edges handled).
+ * status_flag: null, or 4 bytes of device memory, written 0 at launch and non-zero if a bounded wait expires. */
+typedef struct apnn_linear_desc {
+  uint32_t struct_size;
+  int32_t x_type;       /* APNN_TYPE_BF16 or APNN_TYPE_FP16 */
+  int32_t out_type;     /* x_type or APNN_TYPE_FP32; of Out and residual */
+  int32_t activation;   /* APNN_ACT_* */
+  float zero;
+  const float *scale;   /* device, [N] */
+  const float *bias;    /* device, [N], or null */
+  const void *residual; /* device, [M][ldr], or null */
+  int64_t ldx, ldo, ldr;
+} apnn_linear_desc;
+#define APNN_LINEAR_DESC_INIT {(uint32_t)sizeof(apnn_linear_desc)}
+apnn_status apnn_linear_planes(void *stream, int wbits, const void *W, const void *X, void *Out, int M, int N, int K,
+                               const apnn_linear_desc *desc, int *status_flag);
+
+/* A cache of keys and values in 4 bits, in pages.  A page holds `page_size` positions of every head; for each head
+ *   key levels [page_size][D/2] (two per byte, the even element in the low half), value levels [page_size][D/2],
+ *   (step, lowest) of every key row [page_size][2], (step, lowest) of every value row [page_size][2], in `type`,
+ * page_size * (D + 8) bytes, heads one after the other, pages page_stride bytes apart (a multiple of 16).  An element
+ * stands for step * level + lowest.  D is 64, 128 or 256, page_size a power of two from 8 to 1024. */
+typedef struct apnn_kv4_cache {
+  uint32_t struct_size;
+  int32_t type;          /* APNN_TYPE_BF16 or APNN_TYPE_FP16: of the row parameters, and of q, k, v and out */
+  void *data;            /* device, 16-byte aligned */
+  int64_t page_stride;   /* bytes */
+  int32_t pages, heads, page_size, head_dim;
+} apnn_kv4_cache;
+#define APNN_KV4_CACHE_INIT {(uint32_t)sizeof(apnn_kv4_cache)}
+
+/* The sequences of one call.  Rows cu_q[b] .. cu_q[b+1] - 1 of q, k, v and out belong to sequence b, whose length
+ * kv_len[b] counts them: row i of its n rows stands at position kv_len[b] - n + i.  Position p lies in page
+ * table[b][p / page_size].  The arrays are read on the device when the kernels run, so a captured graph follows them.
+ * Rows behind cu_q[sequences] (a batch padded to a fixed size) are left as they were.  A position that is negative or
+ * beyond the table, or whose page number is not one of the cache's, is not written, reads as NaN, and is masked in attention. */
+typedef struct apnn_kv4_batch {
+  uint32_t struct_size;
+  int32_t sequences;
+  const int32_t *cu_q;    /* device, [sequences + 1], ascending from 0 */
+  const int32_t *kv_len;  /* device, [sequences] */
+  const int32_t *table;   /* device, [sequences][table_stride], table_width entries of a row used */
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t max_q;          /* no sequence has more rows in this call; further rows are not attended */
+} apnn_kv4_batch;
+#define APNN_KV4_BATCH_INIT {(uint32_t)sizeof(apnn_kv4_batch)}
+
+/* Keys and values of the batch's rows into the cache, in one pass with the norm of each head of the queries and keys and
+ * the rotation by their positions.  Per row and head, every operation rounded to fp32 on its own (the mean in fp64), so
+ * that the levels are reproducible bit for bit:
+ *   y = x * (1 / sqrt(mean(x^2) + eps)) * weight          (with a norm weight; else y = x)
+ *   (a, b) -> (a c - b s, b c + a s)                      over `rotary_dim` leading elements, pairs (i, i + rotary_dim/2) or
+ *                                                         adjacent ones; c and s from rotary[position]
+ *   lowest = min y, step = max y / 15 - min y / 15, both rounded to the cache's type (a step below 2^-126 counts as 0),
+ *   level = clamp(rint((y - lowest) * (1 / step)), 0, 15), 0 where step is 0
+ * Values are quantised as they are.  A row with a value, step or lowest that is not finite is held as NaN, as is a row
+ * whose position lies behind the rotary table.  q (may be null) is only normed and rotated, into q_out (may be q itself). */
+typedef struct apnn_kv4_append_args {
+  uint32_t struct_size;
+  int32_t rows;           /* rows of q, k, v: none beyond is touched */
+  const void *k, *v;      /* [rows][heads][D], rows k_stride / v_stride elements apart (multiples of 8), 16-byte aligned */
+  int64_t k_stride, v_stride;
+  const void *q;          /* [rows][q_heads][D] or null */
+  void *q_out;
+  int64_t q_stride, q_out_stride;
+  int32_t q_heads;
+  int32_t rotary_dim;     /* 0, or a multiple of 16 up to D */
+  const void *q_norm, *k_norm; /* [D] in the cache's type, or null */
+  double eps;
+  int32_t interleaved;    /* 1: pairs are adjacent elements */
+  const float *rotary;    /* [rotary_rows][rotary_dim]: rotary_dim/2 cosines, then as many sines */
+  int32_t rotary_rows;
+} apnn_kv4_append_args;
+#define APNN_KV4_APPEND_ARGS_INIT {(uint32_t)sizeof(apnn_kv4_append_args)}
+apnn_status apnn_kv4_append(void *stream, const apnn_kv4_cache *cache, const apnn_kv4_batch *batch,
+                            const apnn_kv4_append_args *args);
+
+/* The batch's rows back out of the cache, as values: k_out and v_out [rows][heads][D] in the cache's type, dense. */
+apnn_status apnn_kv4_read(void *stream, const apnn_kv4_cache *cache, const apnn_kv4_batch *batch, void *k_out, void *v_out,
+                          int rows);
+
+/* Attention of the batch's rows over the cache.  Query head h reads key head h / (q_heads / heads).  A row at position p
+ * sees the keys j < kv_len (causal: j <= p; with a window also j > p - window); masked places are never multiplied, whatever they hold.
+ *   Out = softmax(scale * q k^T) v;   lse = ln sum exp(scale * q k^T);   a row that sees no key: Out 0, lse -infinity.
+ * Products of levels are exact, softmax statistics and sums are held in 32 bits, the weights of the values in fp16
+ * relative to the row's maximum; one rounding at the store.  Results do not depend on timing (no atomics on values).
+ * workspace: apnn_kv4_attention_workspace_bytes of device memory, 16-byte aligned, for one call at a time. */
+typedef struct apnn_kv4_attention_args {
+  uint32_t struct_size;
+  int32_t rows;           /* rows of q, out and lse: none beyond is touched */
+  const void *q;          /* [rows][q_heads][D], rows q_stride elements apart (a multiple of 8), 16-byte aligned */
+  void *out;              /* the same form, out_stride */
+  float *lse;             /* [rows][q_heads] or null */
+  int64_t q_stride, out_stride;
+  int32_t q_heads;        /* a multiple of the cache's heads */
+  int32_t causal;         /* 0 or 1 */
+  int32_t window;         /* 0: none; only with causal */
+  float scale;
+} apnn_kv4_attention_args;
+#define APNN_KV4_ATTENTION_ARGS_INIT {(uint32_t)sizeof(apnn_kv4_attention_args)}
+size_t apnn_kv4_attention_workspace_bytes(const apnn_kv4_cache *cache, const apnn_kv4_batch *batch, int q_heads);
+apnn_status apnn_kv4_attention(void *stream, const apnn_kv4_cache *cache, const apnn_kv4_batch *batch,
+                               const apnn_kv4_attention_args *args, void *workspace, size_t workspace_bytes);
+/* Synchronises `stream`; APNN_ERR_TIMEOUT if a bounded wait of the last attention on this workspace expired. */
+apnn_status apnn_kv4_attention_check(void *stream, const void *workspace);
+
 /* ---- measurement aid ------------------------------------------------------------
  * Launches an operand-resident issue loop of one contraction instruction on every SM and
  * returns the operations one launch performs; the caller times the launch with events to
