@@ -84,6 +84,715 @@ __global__ void __launch_bounds__(128) kv4_attention_rows_kernel(const Attention
   if (p.lse && lane == 0) p.lse[(long long)t * p.q_heads + h] = sum == 0.0f ? -INFINITY : top + logf(sum);
 }
 
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// D(16x8, fp32) += A(16x16, fp16) * B(16x8, fp16)
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// transpose of an 8x8 block of 16-bit elements, two per lane
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+template <int WORDS>
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t* r) {
+  if (WORDS == 1) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r[0]) : "r"(a));
+  if (WORDS == 2) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(a));
+  if (WORDS == 4) asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+
+// Four elements of an output row from their sums: row r of the sequence's rows for key head h.
+template <bool BF16, int D, typename S>
+__device__ __forceinline__ void finish_row(const AttentionParams& p, const S& s, int h, int r, int d, float M, float L, float4 v) {
+  const int i = r / p.group, head = h * p.group + (r - i * p.group);
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;      // no key: 0; NaN stays NaN
+  const long long t = s.first + i;
+  *reinterpret_cast<uint2*>(p.out + t * p.out_stride + (long long)head * D + d) = make_uint2(pack2<BF16>(v.x * inv, v.y * inv), pack2<BF16>(v.z * inv, v.w * inv));
+  if (d == 0 && p.lse != nullptr) p.lse[t * p.q_heads + head] = L == 0.0f ? -INFINITY : M * LN2 + logf(L);
+}
+
+// ---------------------------------------------------------------------------------------------- single and few tokens
+// The rows of a sequence that share a key head (its queries times the group, at most 8 NQ) stand against tiles of 128 keys,
+// 32 for each of four warps, which run on their own until the end of a segment.  Scores are computed transposed: a tile of
+// 16 keys is the M operand of mma.sync m16n8k16 and the query rows its N, so eight rows fill the instruction and every key
+// is spread from its nibbles once.  A word of eight levels becomes fp16 operand pairs by masking alone:
+//   w & 0x000f000f, w & 0x00f000f0, (w >> 8) & 0x000f000f, (w >> 8) & 0x00f000f0
+// are pairs of fp16 subnormals, n 2^-24 and n 2^-20, which the tensor core multiplies exactly; the queries stand in the
+// matching order, those at the second and fourth mask divided by 16, scaled by a power of two to fp16's range (exact).
+//   s_j = scale (step_j sum_d q_d n_jd + low_j sum_d q_d)
+// The weights of the values carry the values' step, w_j = 2^(s_j - m) step_j 2^(14 - R) with 2^R above every step seen (at
+// most 2^14, 2^15 at the end of the range, so they keep fp16's eleven bits down to 2^-28 of the largest); they are rounded once, and
+//   sum_j p_j v_jd = 2^(R - 14) (sum_j w_j n_jd - 8 sum_j w_j) + sum_j p_j (low_j + 8 step_j)
+// takes the same rounded w in both sums, so the rounding meets levels centred at 8, not 0..15 (half the error of fp16
+// results).  Value words of two keys are put side by side by PRMT to give pairs along the keys.
+// HBM bounds it: (D + 8) bytes per key and head.
+constexpr int FLOW_WARPS = 4;
+constexpr int FLOW_KEYS = 32;                       // per warp and tile
+constexpr int FLOW_TILE = FLOW_WARPS * FLOW_KEYS;   // 128
+constexpr int FLOW_STAGES = 3;
+constexpr int UNSPLIT_KEYS = 512;   // tables of at most this many positions: no split, no second launch
+
+template <int D, int NQ>
+struct Flow {
+  static constexpr int WK = D / 32;    // words of a key row per lane (four lanes hold a row)
+  static constexpr int WV = D / 64;    // words of a value row per lane (eight lanes)
+  static constexpr int ROW = D / 2;
+  static constexpr int CHUNKS = ROW / 16;
+  static constexpr int V_AT = FLOW_KEYS * ROW, KP_AT = 2 * V_AT, VP_AT = KP_AT + FLOW_KEYS * 4, HEAD_AT = VP_AT + FLOW_KEYS * 4;
+  static constexpr int STAGE = HEAD_AT + 128;
+  static constexpr int RING = FLOW_STAGES * STAGE;
+  static constexpr int ROWS = 8 * NQ;
+  static constexpr int MERGE = ROWS * (D + 4) * 4;       // a warp's part of the exchange at a segment's end: o, then m and l
+  static constexpr int PER_WARP = RING > MERGE ? RING : MERGE;
+  static constexpr bool Q_IN_REGS = NQ * WK <= 4;
+  static constexpr int Q_BYTES = Q_IN_REGS ? 0 : 2 * WK * NQ * 32 * 8;
+  static constexpr int SMEM = FLOW_WARPS * PER_WARP + Q_BYTES + ROWS * 8 + 256;
+  static constexpr int BLOCKS = NQ == 1 ? (D == 256 ? 2 : 4) : NQ == 2 ? (D == 256 ? 2 : 3) : 2;   // per SM
+  static constexpr int SLOT = ROWS * (D + 2);            // floats of a partial result
+};
+
+// Byte offset of 16-byte chunk `chunk` of row `row` in a stage: rows of D/2 bytes in 128-byte lines whose chunks are
+// exchanged so that both readers are free of bank conflicts -- keys, eight lanes over whole lines; values, lanes over the
+// same chunk of rows 0, 2, 4, 6.
+template <int D>
+__device__ __forceinline__ int flow_offset(int row, int chunk) {
+  if (D == 64) return (row >> 2) * 128 + ((((row & 3) * 2 + chunk) ^ (((row >> 2) & 1) * 2)) << 4);
+  if (D == 128) return (row >> 1) * 128 + ((((row & 1) * 4 + chunk) ^ (((row >> 1) & 1) * 4) ^ (((row >> 2) & 1) * 2)) << 4);
+  return row * 128 + ((chunk ^ (row & 6) ^ ((row & 1) * 4)) << 4);
+}
+
+// One sequence of the call: which rows, which keys any of them sees.
+struct Span {
+  int first, n;        // rows first .. first + n - 1
+  int pos0;            // position of the first
+  int len;             // keys there are
+  int begin, end;      // keys that some row sees lie in [begin, end)
+  int tile0, tiles;    // tiles of `TILE` keys over them; one (empty) tile where there is no key, none without rows
+};
+template <int TILE>
+__device__ __forceinline__ Span span_of(const AttentionParams& p, int b) {
+  Span s;
+  s.first = __ldg(p.batch.cu_q + b);
+  const int all = __ldg(p.batch.cu_q + b + 1) - s.first;
+  s.n = s.first < 0 ? 0 : min(min(all, p.batch.max_q), p.batch.rows - s.first);
+  const int kv = __ldg(p.batch.kv_len + b);
+  s.pos0 = kv - all;
+  s.len = (int)min((long long)kv, (long long)p.batch.table_width << p.cache.page_shift);
+  s.begin = 0;
+  s.end = s.len;
+  if (p.causal) {
+    s.end = min(s.end, s.pos0 + s.n);
+    if (p.window > 0) s.begin = max(0, s.pos0 + 1 - p.window);
+  }
+  s.tile0 = s.begin / TILE;
+  s.tiles = s.n <= 0 ? 0 : s.end > s.begin ? (s.end + TILE - 1) / TILE - s.tile0 : 1;
+  return s;
+}
+
+struct FlowParams {
+  AttentionParams a;
+  int2* pieces;     // [sequences * heads]: first block and number of the partial results of a (sequence, head), 0: none
+  float* slots;     // [2 * blocks][Flow::SLOT]
+  int split;
+};
+
+template <bool BF16, int D, int NQ>
+__global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_attention_flow_kernel(const FlowParams fp) {
+  using F = Flow<D, NQ>;
+  const AttentionParams& p = fp.a;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  uint8_t* my_smem = smem + warp * F::PER_WARP;
+  const uint32_t ring = smem_u32(my_smem);
+  uint2* q_s = reinterpret_cast<uint2*>(smem + FLOW_WARPS * F::PER_WARP);
+  float2* qf_s = reinterpret_cast<float2*>(smem + FLOW_WARPS * F::PER_WARP + F::Q_BYTES);   // per row: factor of the products, of the lows
+  int* scan_s = reinterpret_cast<int*>(smem + FLOW_WARPS * F::PER_WARP + F::Q_BYTES + F::ROWS * 8);
+  const int heads = p.cache.heads, sequences = p.batch.sequences;
+  grid_dependency_wait();
+  grid_launch_dependents();   // the joining kernel waits for this whole grid anyway
+
+  // ---- which units (sequence, head, tile) this block takes: an equal share of all, in order
+  int u0, u1, b = 0, h = 0, t0 = 0, stride = 0;
+  long long total = 0, sharing = 0;
+  Span s;
+  if (fp.split) {
+    int sum = 0;
+    for (int i = threadIdx.x; i < sequences; i += 32 * FLOW_WARPS) sum += span_of<FLOW_TILE>(p, i).tiles;
+    sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == 0) scan_s[warp] = sum;
+    __syncthreads();
+    total = (long long)(scan_s[0] + scan_s[1] + scan_s[2] + scan_s[3]) * heads;
+    sharing = min(total, (long long)gridDim.x);     // so that no share is empty: the joining kernel counts on every block between
+    if (blockIdx.x >= sharing) return;
+    u0 = (int)(total * blockIdx.x / sharing);
+    u1 = (int)(total * (blockIdx.x + 1) / sharing);
+    // the sequence of unit u0, 128 sequences at a time
+    int before = 0;
+    for (int base = 0;; base += 32 * FLOW_WARPS) {
+      __syncthreads();
+      const int i = base + threadIdx.x;
+      const int mine = i < sequences ? span_of<FLOW_TILE>(p, i).tiles * heads : 0;
+      int inc = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const int o = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += o;
+      }
+      if (lane == 31) scan_s[4 + warp] = inc;
+      __syncthreads();
+      int at = before;
+      for (int w = 0; w < warp; w++) at += scan_s[4 + w];
+      if (u0 >= at + inc - mine && u0 < at + inc) {
+        scan_s[8] = i;
+        scan_s[9] = at + inc - mine;
+      }
+      before += scan_s[4] + scan_s[5] + scan_s[6] + scan_s[7];
+      if (before > u0) break;     // uniform; total > u0, so a sequence is found
+    }
+    __syncthreads();
+    b = scan_s[8];
+    s = span_of<FLOW_TILE>(p, b);
+    h = (u0 - scan_s[9]) / s.tiles;
+    t0 = (u0 - scan_s[9]) - h * s.tiles;
+  } else {
+    // one block takes a (sequence, head) whole
+    stride = gridDim.x;
+    u0 = blockIdx.x;
+    u1 = sequences * heads;
+  }
+
+  for (int u = u0; u < u1;) {
+    int nt;
+    if (fp.split) {
+      while (s.tiles == 0 || h == heads) {     // on to the next sequence with rows
+        h = 0;
+        s = span_of<FLOW_TILE>(p, ++b);
+      }
+      nt = min(s.tiles - t0, u1 - u);
+    } else {
+      b = u / heads;
+      h = u - b * heads;
+      s = span_of<FLOW_TILE>(p, b);
+      if (s.tiles == 0) {
+        u += stride;
+        continue;
+      }
+      nt = s.tiles;
+    }
+    const int rows = s.n * p.group;     // at most 8 NQ
+
+    // ---- pipeline of this warp's 32-key pieces of the segment
+    const int key0 = (s.tile0 + t0) * FLOW_TILE + warp * FLOW_KEYS;
+    const int* trow = p.batch.table + (long long)b * p.batch.table_stride;
+    const uint8_t* head_base = p.cache.data + h * p.cache.head_bytes;
+    const int page_mask = p.cache.page_size - 1;
+    // page number of the eight keys that lane % 4 answers for, of tile i; -1 where there is none to read
+    auto page_at = [&](int i) {
+      const int key = key0 + i * FLOW_TILE + (lane & 3) * 8;
+      if (i >= nt || key >= s.end || key < 0) return -1;      // key < len <= table_width * page_size: within the table
+      const int id = __ldg(trow + (key >> p.cache.page_shift));
+      return id < 0 || id >= p.cache.pages ? -1 : id;
+    };
+    auto issue = [&](int i, int stage, int ids) {
+      if (i < nt) {
+        const uint32_t at = ring + stage * F::STAGE;
+        const int key = key0 + i * FLOW_TILE;
+        constexpr int ROWS_PER = 32 / F::CHUNKS;     // rows a warp-wide copy takes
+#pragma unroll
+        for (int c = 0; c < FLOW_KEYS / ROWS_PER; c++) {
+          const int row = c * ROWS_PER + lane / F::CHUNKS, chunk = lane % F::CHUNKS;
+          const int id = __shfl_sync(0xffffffffu, ids, row >> 3);
+          const uint8_t* src = head_base + max(id, 0) * p.cache.page_stride + (long long)((key + row) & page_mask) * F::ROW + chunk * 16;
+          const uint32_t dst = at + flow_offset<D>(row, chunk);
+          cp_async16(dst, src, id < 0 ? 0 : 16);
+          cp_async16(dst + F::V_AT, src + (long long)p.cache.page_size * F::ROW, id < 0 ? 0 : 16);
+        }
+        const int grp = (lane >> 1) & 3, part = (lane >> 3) & 1;
+        const int id = __shfl_sync(0xffffffffu, ids, grp);
+        if (lane < 16) {
+          const uint8_t* src = head_base + max(id, 0) * p.cache.page_stride + (long long)p.cache.page_size * D +
+                               (part * p.cache.page_size + ((key + grp * 8) & page_mask)) * 4ll + (lane & 1) * 16;
+          cp_async16(at + F::KP_AT + part * (FLOW_KEYS * 4) + grp * 32 + (lane & 1) * 16, src, id < 0 ? 0 : 16);
+        }
+        const uint32_t live = __ballot_sync(0xffffffffu, lane < 4 && ids >= 0);
+        if (lane == 0) *reinterpret_cast<volatile uint32_t*>(my_smem + stage * F::STAGE + F::HEAD_AT) = live;
+      }
+      cp_async_commit();
+    };
+    int ids = page_at(0);
+#pragma unroll
+    for (int i = 0; i < FLOW_STAGES - 1; i++) {
+      const int next = page_at(i + 1);
+      issue(i, i, ids);
+      ids = next;
+    }
+
+    // ---- the queries as fp16 operands, while the first keys are on their way.  A group of four lanes (t) shares a row.
+    uint32_t qr[F::Q_IN_REGS ? 2 * F::WK * NQ * 2 : 1];
+    auto load_row = [&](int r, uint2* frags) {       // this lane's 8 WK elements of row r -> 2 WK operand pairs; factors to shared memory
+      float x[8 * F::WK];
+      const bool live = r < rows;
+      const int i = live ? r / p.group : 0;
+      const uint16_t* src = p.q + (long long)(s.first + i) * p.q_stride + (long long)(h * p.group + (live ? r - i * p.group : 0)) * D;
+#pragma unroll
+      for (int w = 0; w < F::WK; w++) {
+        // word w of this lane's key words: element 32 t + 8 w (D = 128), 16 t + 8 w (64), 128 (w / 4) + 32 t + 8 (w % 4) (256)
+        const int d = D == 64 ? 16 * t + 8 * w : 128 * (w / 4) + 32 * t + 8 * (w & 3);
+        const uint4 v = live ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float2 f = unpack2<BF16>(vv[j]);
+          x[8 * w + 2 * j] = f.x;
+          x[8 * w + 2 * j + 1] = f.y;
+        }
+      }
+      float top = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8 * F::WK; j++) {
+        top = fmaxf(top, fabsf(x[j]));
+        sum += x[j];
+      }
+#pragma unroll
+      for (int d = 1; d < 4; d *= 2) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      }
+      // power of two that takes the row's largest element to [2^14, 2^15); rows of zeros and of infinities as they are
+      const int e = (int)(__float_as_uint(top) >> 23) - 127;
+      const int shift = top > 0.0f && e < 128 ? 14 - max(e, -100) : 0;
+      const float up = __uint_as_float((uint32_t)(127 + shift) << 23);
+      if (t == 0) qf_s[r] = make_float2(p.scale * LOG2E * __uint_as_float((uint32_t)(127 - shift) << 23), p.scale * LOG2E * sum);
+#pragma unroll
+      for (int w = 0; w < F::WK; w++) {
+        const float* y = x + 8 * w;
+        const float down = up * 0.0625f;
+        frags[2 * w] = make_uint2(pack2<false>(y[0] * up, y[4] * up), pack2<false>(y[1] * down, y[5] * down));
+        frags[2 * w + 1] = make_uint2(pack2<false>(y[2] * up, y[6] * up), pack2<false>(y[3] * down, y[7] * down));
+      }
+    };
+    if (F::Q_IN_REGS) {
+#pragma unroll
+      for (int q = 0; q < NQ; q++) {
+        uint2 frags[2 * F::WK];
+        load_row(q * 8 + g, frags);     // every warp writes the same factors
+#pragma unroll
+        for (int k = 0; k < 2 * F::WK; k++) {
+          qr[(k * NQ + q) * 2] = frags[k].x;
+          qr[(k * NQ + q) * 2 + 1] = frags[k].y;
+        }
+      }
+    } else {
+      for (int q = warp; q < NQ; q += FLOW_WARPS) {
+        uint2 frags[2 * F::WK];
+        load_row(q * 8 + g, frags);
+#pragma unroll
+        for (int k = 0; k < 2 * F::WK; k++) q_s[(k * NQ + q) * 32 + lane] = frags[k];
+      }
+    }
+    __syncthreads();
+    float qf[2 * NQ], ql[2 * NQ];
+#pragma unroll
+    for (int c = 0; c < 2 * NQ; c++) {
+      const float2 f = qf_s[(c >> 1) * 8 + 2 * t + (c & 1)];
+      qf[c] = f.x;
+      ql[c] = f.y;
+    }
+    // the keys every row sees: no mask is looked at there
+    const int last_begin = p.causal && p.window > 0 ? max(0, s.pos0 + s.n - p.window) : 0;
+    const int first_end = p.causal ? min(s.len, s.pos0 + 1) : s.len;
+
+    float o[F::WV][4][NQ][4], ones[NQ][4];
+    float m[2 * NQ], l[2 * NQ], vsum[2 * NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; q++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        ones[q][c] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < F::WV; w++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) o[w][j][q][c] = 0.0f;
+      }
+#pragma unroll
+    for (int c = 0; c < 2 * NQ; c++) {
+      m[c] = -INFINITY;
+      l[c] = vsum[c] = 0.0f;
+    }
+    int R = -112;     // 2^R is above every value step met so far, within fp32's range
+
+    for (int i = 0, stage = 0, fill = FLOW_STAGES - 1; i < nt; i++) {
+      cp_async_wait<FLOW_STAGES - 2>();
+      __syncwarp();
+      const int next = page_at(i + FLOW_STAGES);
+      const int key = key0 + i * FLOW_TILE;
+      const uint32_t at = ring + stage * F::STAGE;
+      const uint32_t live = *reinterpret_cast<volatile uint32_t*>(my_smem + stage * F::STAGE + F::HEAD_AT);
+      if (key < s.end && key + FLOW_KEYS > s.begin) {       // warp-uniform
+        const bool whole = live == 15u && key >= last_begin && key + FLOW_KEYS <= first_end;
+        // ---- scores of two tiles of 16 keys
+        float sc[2][NQ][4];
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+          for (int q = 0; q < NQ; q++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) sc[mt][q][c] = 0.0f;
+        constexpr int WL = F::WK < 4 ? F::WK : 4;     // words of one load
+#pragma unroll
+        for (int w0 = 0; w0 < F::WK; w0 += WL) {
+          uint32_t kw[2][2][WL];
+#pragma unroll
+          for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+            for (int hi = 0; hi < 2; hi++) {
+              const int row = mt * 16 + hi * 8 + g;
+              const int byte = D == 64 ? 8 * t : 16 * (t + w0);      // w0 is 0 or, at D = 256, 4: chunk t or t + 4
+              lds_words<WL>(at + flow_offset<D>(row, byte >> 4) + (byte & 15), kw[mt][hi]);
+            }
+#pragma unroll
+          for (int w = 0; w < WL; w++) {
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+              const int k = 2 * (w0 + w) + half;
+              uint2 bq[NQ];
+#pragma unroll
+              for (int q = 0; q < NQ; q++)
+                bq[q] = F::Q_IN_REGS ? make_uint2(qr[(k * NQ + q) * 2], qr[(k * NQ + q) * 2 + 1]) : q_s[(k * NQ + q) * 32 + lane];
+#pragma unroll
+              for (int mt = 0; mt < 2; mt++) {
+                const uint32_t x = half ? kw[mt][0][w] >> 8 : kw[mt][0][w], y = half ? kw[mt][1][w] >> 8 : kw[mt][1][w];
+#pragma unroll
+                for (int q = 0; q < NQ; q++)
+                  mma_f16(sc[mt][q], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, bq[q].x, bq[q].y);
+              }
+            }
+          }
+        }
+        // ---- the rows' parameters; scores in the log2 domain; running maximum
+        float2 kp[4], vp[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          kp[r] = unpack2<BF16>(lds32(at + F::KP_AT + (r * 8 + g) * 4));
+          kp[r].x *= 16777216.0f;      // the levels are multiples of 2^-24
+          vp[r] = unpack2<BF16>(lds32(at + F::VP_AT + (r * 8 + g) * 4));
+        }
+        uint32_t seen[2 * NQ];     // bit r: the key of parameter r is visible to the row of column c
+        float top[2 * NQ];
+#pragma unroll
+        for (int c = 0; c < 2 * NQ; c++) {
+          seen[c] = 15u;
+          top[c] = m[c];
+        }
+        if (!whole) {
+#pragma unroll
+          for (int c = 0; c < 2 * NQ; c++) {
+            const int r = (c >> 1) * 8 + 2 * t + (c & 1);
+            const int pos = s.pos0 + min(r / p.group, s.n - 1);
+            const int end = p.causal ? min(s.len, pos + 1) : s.len;
+            const int begin = p.causal && p.window > 0 ? pos + 1 - p.window : 0;
+            seen[c] = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const int j = key + k * 8 + g;
+              if (j < end && j >= begin && ((live >> k) & 1u)) seen[c] |= 1u << k;
+            }
+          }
+        }
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+          for (int q = 0; q < NQ; q++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+              const int r = 2 * mt + (c >> 1), col = 2 * q + (c & 1);
+              const float v = fmaf(sc[mt][q][c] * kp[r].x, qf[col], kp[r].y * ql[col]);
+              sc[mt][q][c] = whole || ((seen[col] >> r) & 1u) ? v : -INFINITY;
+              top[col] = fmaxf(top[col], sc[mt][q][c]);
+            }
+        // exponent of the largest value step of these keys (a step that is not finite shows in its weight instead)
+        uint32_t bits = __float_as_uint(fabsf(unpack2<BF16>(lds32(at + F::VP_AT + lane * 4)).x));
+        if (bits >= 0x7f800000u || (!whole && (key + lane >= s.end || key + lane < s.begin || !((live >> (lane >> 3)) & 1u)))) bits = 0;
+        const int rise = max(R, min((int)(__reduce_max_sync(0xffffffffu, bits) >> 23) - 126, 127));
+        bool moved = rise != R;
+#pragma unroll
+        for (int c = 0; c < 2 * NQ; c++) {
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], d));
+          moved |= top[c] != m[c];
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+          const float shrink = __uint_as_float((uint32_t)max(127 + R - rise, 0) << 23);      // 2^(R - rise)
+          R = rise;
+#pragma unroll
+          for (int c = 0; c < 2 * NQ; c++) {
+            const float keep = m[c] == top[c] ? 1.0f : ex2(m[c] - top[c]);       // -inf - x: 0
+            m[c] = top[c];
+            l[c] *= keep;
+            vsum[c] *= keep;
+            const float k = keep * shrink;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              ones[c >> 1][(c & 1) + 2 * e] *= k;
+#pragma unroll
+              for (int w = 0; w < F::WV; w++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[w][j][c >> 1][(c & 1) + 2 * e] *= k;
+            }
+          }
+        }
+        // ---- weights, and their products with the values
+        const float lift = __uint_as_float((uint32_t)(127 + 14 - R) << 23);     // 2^(14 - R)
+        float step[4], mid[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          step[r] = vp[r].x * lift;
+          mid[r] = fmaf(8.0f, vp[r].x, vp[r].y);
+        }
+        uint32_t wt[2][NQ][2];
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+          for (int q = 0; q < NQ; q++) {
+            float w[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+              const int r = 2 * mt + (c >> 1), col = 2 * q + (c & 1);
+              const float base = m[col] == -INFINITY ? 0.0f : m[col];
+              const float e = ex2(sc[mt][q][c] - base);
+              l[col] += e;
+              const bool on = whole || ((seen[col] >> r) & 1u);      // a masked place may hold NaN
+              w[c] = on ? e * step[r] : 0.0f;
+              vsum[col] += on ? e * mid[r] : 0.0f;
+            }
+            wt[mt][q][0] = transpose8x8(pack2<false>(w[0], w[1]));
+            wt[mt][q][1] = transpose8x8(pack2<false>(w[2], w[3]));
+          }
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++) {
+          uint32_t vw[4][F::WV];
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const int row = mt * 16 + (k >> 1) * 8 + 2 * t + (k & 1);
+            const int byte = 4 * F::WV * g;
+            lds_words<F::WV>(at + F::V_AT + flow_offset<D>(row, byte >> 4) + (byte & 15), vw[k]);
+          }
+#pragma unroll
+          for (int q = 0; q < NQ; q++) mma_f16(ones[q], 0x00010001u, 0x00010001u, 0x00010001u, 0x00010001u, wt[mt][q][0], wt[mt][q][1]);
+#pragma unroll
+          for (int w = 0; w < F::WV; w++) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              uint32_t x = __byte_perm(vw[0][w], vw[1][w], j < 2 ? 0x5410 : 0x7632);
+              uint32_t y = __byte_perm(vw[2][w], vw[3][w], j < 2 ? 0x5410 : 0x7632);
+              if (j & 1) {
+                x >>= 8;
+                y >>= 8;
+              }
+#pragma unroll
+              for (int q = 0; q < NQ; q++)
+                mma_f16(o[w][j][q], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, wt[mt][q][0], wt[mt][q][1]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      issue(i + FLOW_STAGES - 1, fill, ids);
+      ids = next;
+      stage = stage + 1 == FLOW_STAGES ? 0 : stage + 1;
+      fill = fill + 1 == FLOW_STAGES ? 0 : fill + 1;
+    }
+    cp_async_wait<0>();
+    __syncwarp();
+
+    // ---- the four warps' results meet in shared memory
+    {
+      float* mine = reinterpret_cast<float*>(my_smem);
+      const float unit = __uint_as_float((uint32_t)(127 + 24 - 14) << 23);
+      const float lower = __uint_as_float((uint32_t)(127 + R) << 23);       // R >= -112
+#pragma unroll
+      for (int c = 0; c < 2 * NQ; c++) {
+        const int r = (c >> 1) * 8 + 2 * t + (c & 1);
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) {
+          l[c] += __shfl_xor_sync(0xffffffffu, l[c], d);
+          vsum[c] += __shfl_xor_sync(0xffffffffu, vsum[c], d);
+        }
+        const float eight = 8.0f * ones[c >> 1][c & 1];
+#pragma unroll
+        for (int w = 0; w < F::WV; w++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            float2 v;      // elements 2 j and 2 j + 1 of the word; the second stands 16 times too high
+            v.x = fmaf((o[w][j][c >> 1][c & 1] - eight) * unit, lower, vsum[c]);
+            v.y = fmaf((o[w][j][c >> 1][(c & 1) + 2] * 0.0625f - eight) * unit, lower, vsum[c]);
+            *reinterpret_cast<float2*>(mine + r * (D + 4) + 8 * (F::WV * g + w) + 2 * j) = v;
+          }
+        if (g == 0) *reinterpret_cast<float2*>(mine + r * (D + 4) + D) = make_float2(m[c], l[c]);
+      }
+    }
+    __syncthreads();
+    const bool complete = nt == s.tiles;
+    const int bh = b * heads + h;
+    float* slot = complete ? nullptr : fp.slots + (2ll * blockIdx.x + (t0 == 0 ? 1 : 0)) * F::SLOT;
+    if (threadIdx.x == 0 && fp.split && t0 == 0) {
+      // the last unit of this (sequence, head) lies with the block whose share holds it
+      const long long last = (long long)u + s.tiles - 1;
+      fp.pieces[bh] = complete ? make_int2(0, 0) : make_int2((int)blockIdx.x, (int)(((last + 1) * sharing - 1) / total) - (int)blockIdx.x + 1);
+    }
+    for (int e = threadIdx.x; e < rows * (D / 4); e += 32 * FLOW_WARPS) {
+      const int r = e / (D / 4), d = (e % (D / 4)) * 4;
+      float M = -INFINITY;
+      float2 ml[FLOW_WARPS];
+#pragma unroll
+      for (int w = 0; w < FLOW_WARPS; w++) {
+        ml[w] = *reinterpret_cast<const float2*>(smem + w * F::PER_WARP + (r * (D + 4) + D) * 4);
+        M = fmaxf(M, ml[w].x);
+      }
+      float L = 0.0f;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < FLOW_WARPS; w++) {
+        // a warp that saw no key adds nothing; NaN scores keep l at NaN
+        const float f = ml[w].x == -INFINITY ? (ml[w].y == 0.0f ? 0.0f : ml[w].y) : ex2(ml[w].x - M);
+        if (ml[w].x == -INFINITY && ml[w].y == 0.0f) continue;
+        const float4 x = *reinterpret_cast<const float4*>(smem + w * F::PER_WARP + (r * (D + 4) + d) * 4);
+        L += f * ml[w].y;
+        v.x += f * x.x;
+        v.y += f * x.y;
+        v.z += f * x.z;
+        v.w += f * x.w;
+      }
+      if (complete) {
+        finish_row<BF16, D>(p, s, h, r, d, M, L, v);
+      } else {
+        *reinterpret_cast<float4*>(slot + F::ROWS * 2 + r * D + d) = v;
+        if (d == 0) *reinterpret_cast<float2*>(slot + r * 2) = make_float2(M, L);
+      }
+    }
+    __syncthreads();     // the exchange area is the next segment's ring
+    if (fp.split) {
+      u += nt;
+      t0 = 0;
+      h++;
+    } else {
+      u += stride;
+    }
+  }
+}
+
+// Joins the partial results of the (sequence, head)s that lie in several blocks, in the order of their keys.
+template <bool BF16, int D, int NQ>
+__global__ void __launch_bounds__(128) kv4_attention_join_kernel(const FlowParams fp) {
+  using F = Flow<D, NQ>;
+  const AttentionParams& p = fp.a;
+  grid_dependency_wait();
+  const int bh = blockIdx.x, b = bh / p.cache.heads, h = bh - b * p.cache.heads;
+  const Span s = span_of<FLOW_TILE>(p, b);
+  if (s.n <= 0) return;
+  const int2 pc = __ldcg(fp.pieces + bh);
+  if (pc.y == 0) return;
+  for (int e = blockIdx.y * 128 + threadIdx.x; e < s.n * p.group * (D / 4); e += 128 * gridDim.y) {
+    const int r = e / (D / 4), d = (e % (D / 4)) * 4;
+    float M = -INFINITY, L = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int i = 0; i < pc.y; i++) {
+      const float* slot = fp.slots + (2ll * (pc.x + i) + (i == 0 ? 1 : 0)) * F::SLOT;
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(slot + r * 2));
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(slot + F::ROWS * 2 + r * D + d));
+      if (ml.x == -INFINITY && ml.y == 0.0f) continue;
+      const float top = fmaxf(M, ml.x);
+      const float f = M == top ? 1.0f : ex2(M - top), k = ml.x == top ? 1.0f : ex2(ml.x - top);
+      M = top;
+      L = L * f + k * ml.y;
+      v.x = v.x * f + k * x.x;
+      v.y = v.y * f + k * x.y;
+      v.z = v.z * f + k * x.z;
+      v.w = v.w * f + k * x.w;
+    }
+    finish_row<BF16, D>(p, s, h, r, d, M, L, v);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- host side
+int largest_rows(int D) { return D == 256 ? 16 : 32; }    // of a sequence and key head on the flow kernel
+
+struct FlowPlan {
+  int nq, blocks, join, split;     // query rows / 8, grid, sequences * heads, whether a (sequence, head) may be split
+  size_t pieces_at, slots_at, bytes;
+};
+
+FlowPlan flow_plan(const apnn_kv4_cache* c, const apnn_kv4_batch* b, int group) {
+  FlowPlan f;
+  const long long rows = (long long)b->max_q * group;
+  f.nq = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  const int D = c->head_dim;
+  const int per_sm = f.nq == 1 ? (D == 256 ? Flow<256, 1>::BLOCKS : Flow<128, 1>::BLOCKS) : f.nq == 2 ? (D == 256 ? Flow<256, 2>::BLOCKS : Flow<128, 2>::BLOCKS) : Flow<128, 4>::BLOCKS;
+  const long long keys = (long long)b->table_width * c->page_size;
+  const long long whole = (long long)b->sequences * c->heads;
+  f.split = keys > UNSPLIT_KEYS;
+  const long long units = whole * ((keys + FLOW_TILE - 1) / FLOW_TILE);
+  const long long most = (long long)device_sm_count() * per_sm;
+  f.blocks = (int)(f.split ? (units < most ? units : most) : (whole < (1ll << 30) ? whole : 1ll << 30));
+  f.join = (int)whole;
+  f.pieces_at = 256;
+  f.slots_at = (f.pieces_at + (f.split ? whole * 8 : 0) + 127) / 128 * 128;
+  f.bytes = f.slots_at + (f.split ? 2ull * f.blocks * (8 * f.nq * (D + 2)) * 4 : 0);
+  return f;
+}
+
+template <bool BF16, int D, int NQ>
+apnn_status launch_flow(cudaStream_t stream, const FlowPlan& f, const FlowParams& fp) {
+  const void* kernel = reinterpret_cast<const void*>(kv4_attention_flow_kernel<BF16, D, NQ>);
+  cudaError_t e = ensure_max_smem(kernel, Flow<D, NQ>::SMEM);
+  if (e != cudaSuccess) return cuda_fail(e, "kv4_attention_flow_kernel shared memory");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)f.blocks, 1, 1);
+  cfg.blockDim = dim3(32 * FLOW_WARPS, 1, 1);
+  cfg.dynamicSmemBytes = Flow<D, NQ>::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  cfg.numAttrs = pdl_attribute(attr);
+  cfg.attrs = attr;
+  e = cudaLaunchKernelEx(&cfg, kv4_attention_flow_kernel<BF16, D, NQ>, fp);
+  if (e != cudaSuccess) return cuda_fail(e, "kv4_attention_flow_kernel");
+  if (!f.split) return APNN_OK;
+  int parts = 1;     // blocks that share the rows of a (sequence, head): a few pairs alone would leave the device idle
+  while (parts < 8 && (long long)f.join * parts < 2 * device_sm_count() && parts * 128 * 4 < 8 * NQ * D) parts *= 2;
+  cfg.gridDim = dim3((unsigned)f.join, (unsigned)parts, 1);
+  cfg.blockDim = dim3(128, 1, 1);
+  cfg.dynamicSmemBytes = 0;
+  e = cudaLaunchKernelEx(&cfg, kv4_attention_join_kernel<BF16, D, NQ>, fp);
+  return e == cudaSuccess ? APNN_OK : cuda_fail(e, "kv4_attention_join_kernel");
+}
+
+template <bool BF16, int D>
+apnn_status launch_flow_rows(cudaStream_t stream, const FlowPlan& f, const FlowParams& fp) {
+  if (f.nq == 1) return launch_flow<BF16, D, 1>(stream, f, fp);
+  if (f.nq == 2) return launch_flow<BF16, D, 2>(stream, f, fp);
+  if constexpr (D != 256) return launch_flow<BF16, D, 4>(stream, f, fp);
+  return APNN_ERR_UNSUPPORTED;     // not reached: such rows take the other kernel
+}
+
 }  // namespace
 }  // namespace apnn
 
@@ -92,10 +801,12 @@ using namespace apnn;
 extern "C" {
 
 size_t apnn_kv4_attention_workspace_bytes(const apnn_kv4_cache* cache, const apnn_kv4_batch* batch, int q_heads) {
-  (void)cache;
-  (void)batch;
-  (void)q_heads;
-  return 256;
+  Kv4View view = {};
+  Kv4Batch geo = {};
+  if (kv4_view(cache, &view) != APNN_OK || kv4_batch(batch, 1, &geo) != APNN_OK || q_heads <= 0 || q_heads % cache->heads != 0) return 0;
+  const int group = q_heads / cache->heads;
+  if ((long long)batch->max_q * group > largest_rows(cache->head_dim)) return 256;
+  return flow_plan(cache, batch, group).bytes;
 }
 
 apnn_status apnn_kv4_attention(void* stream, const apnn_kv4_cache* cache, const apnn_kv4_batch* batch,
@@ -124,13 +835,23 @@ apnn_status apnn_kv4_attention(void* stream, const apnn_kv4_cache* cache, const 
   p.causal = a->causal;
   p.window = a->window;
   p.scale = a->scale;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if ((long long)batch->max_q * p.group <= largest_rows(cache->head_dim)) {
+    const FlowPlan f = flow_plan(cache, batch, p.group);
+    FlowParams fp = {p, reinterpret_cast<int2*>(static_cast<char*>(workspace) + f.pieces_at),
+                     reinterpret_cast<float*>(static_cast<char*>(workspace) + f.slots_at), f.split};
+    apnn_status (*const launch[2][3])(cudaStream_t, const FlowPlan&, const FlowParams&) = {
+        {launch_flow_rows<false, 64>, launch_flow_rows<false, 128>, launch_flow_rows<false, 256>},
+        {launch_flow_rows<true, 64>, launch_flow_rows<true, 128>, launch_flow_rows<true, 256>}};
+    return launch[cache->type == APNN_TYPE_BF16][cache->head_dim / 128](s, f, fp);
+  }
   void (*const kernels[2][3])(AttentionParams) = {
       {kv4_attention_rows_kernel<false, 64>, kv4_attention_rows_kernel<false, 128>, kv4_attention_rows_kernel<false, 256>},
       {kv4_attention_rows_kernel<true, 64>, kv4_attention_rows_kernel<true, 128>, kv4_attention_rows_kernel<true, 256>}};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(((long long)a->rows * a->q_heads + 3) / 4), 1, 1);
   cfg.blockDim = dim3(128, 1, 1);
-  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cfg.stream = s;
   cudaLaunchAttribute attr[1];
   cfg.numAttrs = pdl_attribute(attr);
   cfg.attrs = attr;
