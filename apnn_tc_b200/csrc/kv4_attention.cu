@@ -1,5 +1,6 @@
 // Attention over the 4-bit cache.
 #include <cmath>
+#include <type_traits>
 
 #include "kv4.cuh"
 #include "tc5_common.cuh"
@@ -137,9 +138,10 @@ __device__ __forceinline__ void finish_row(const AttentionParams& p, const S& s,
 // are pairs of fp16 subnormals, n 2^-24 and n 2^-20, which the tensor core multiplies exactly; the queries stand in the
 // matching order, those at the second and fourth mask divided by 16, scaled by a power of two to fp16's range (exact).
 //   s_j = scale (step_j sum_d q_d n_jd + low_j sum_d q_d)
-// The weights of the values carry the values' step, w_j = 2^(s_j - m) step_j 2^(14 - R) with 2^R above every step seen (at
-// most 2^14, 2^15 at the end of the range, so they keep fp16's eleven bits down to 2^-28 of the largest); they are rounded once, and
-//   sum_j p_j v_jd = 2^(R - 14) (sum_j w_j n_jd - 8 sum_j w_j) + sum_j p_j (low_j + 8 step_j)
+// The weights of the values carry the values' step, w_j = 2^(s_j - m) step_j 2^(6 - R) with 2^R above every step seen and m
+// at most 8 below the largest s (so at most 2^14, 2^15 at the end of the range; fp16's eleven bits hold down to 2^-20 of the
+// reference point); they are rounded once, and
+//   sum_j p_j v_jd = 2^(R - 6) (sum_j w_j n_jd - 8 sum_j w_j) + sum_j p_j (low_j + 8 step_j)
 // takes the same rounded w in both sums, so the rounding meets levels centred at 8, not 0..15 (half the error of fp16
 // results).  Value words of two keys are put side by side by PRMT to give pairs along the keys.
 // HBM bounds it: (D + 8) bytes per key and head.
@@ -304,43 +306,46 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
     const int* trow = p.batch.table + (long long)b * p.batch.table_stride;
     const uint8_t* head_base = p.cache.data + h * p.cache.head_bytes;
     const int page_mask = p.cache.page_size - 1;
-    // page number of the eight keys that lane % 4 answers for, of tile i; -1 where there is none to read
-    auto page_at = [&](int i) {
+    const long long v_off = (long long)p.cache.page_size * F::ROW;     // from a key row to its value row
+    // where the eight keys that lane % 4 answers for start in head h, of tile i, as an offset into the cache; -1 where there is
+    // nothing to read
+    auto rows_at = [&](int i) -> long long {
       const int key = key0 + i * FLOW_TILE + (lane & 3) * 8;
       if (i >= nt || key >= s.end || key < 0) return -1;      // key < len <= table_width * page_size: within the table
       const int id = __ldg(trow + (key >> p.cache.page_shift));
-      return id < 0 || id >= p.cache.pages ? -1 : id;
+      return id < 0 || id >= p.cache.pages ? -1 : id * p.cache.page_stride + (long long)(key & page_mask) * F::ROW;
     };
-    auto issue = [&](int i, int stage, int ids) {
+    auto issue = [&](int i, int stage, long long rows_off) {
       if (i < nt) {
         const uint32_t at = ring + stage * F::STAGE;
-        const int key = key0 + i * FLOW_TILE;
-        constexpr int ROWS_PER = 32 / F::CHUNKS;     // rows a warp-wide copy takes
+        constexpr int ROWS_PER = 32 / F::CHUNKS;     // rows a warp-wide copy takes: they lie one behind the other in a page
 #pragma unroll
         for (int c = 0; c < FLOW_KEYS / ROWS_PER; c++) {
-          const int row = c * ROWS_PER + lane / F::CHUNKS, chunk = lane % F::CHUNKS;
-          const int id = __shfl_sync(0xffffffffu, ids, row >> 3);
-          const uint8_t* src = head_base + max(id, 0) * p.cache.page_stride + (long long)((key + row) & page_mask) * F::ROW + chunk * 16;
-          const uint32_t dst = at + flow_offset<D>(row, chunk);
-          cp_async16(dst, src, id < 0 ? 0 : 16);
-          cp_async16(dst + F::V_AT, src + (long long)p.cache.page_size * F::ROW, id < 0 ? 0 : 16);
+          const int row = c * ROWS_PER + lane / F::CHUNKS;
+          const long long off = __shfl_sync(0xffffffffu, rows_off, row >> 3);
+          const uint8_t* src = head_base + max(off, 0ll) + ((row & 7) * F::ROW + (lane % F::CHUNKS) * 16);
+          const uint32_t dst = at + flow_offset<D>(row, lane % F::CHUNKS);
+          const int bytes = off < 0 ? 0 : 16;
+          cp_async16(dst, src, bytes);
+          cp_async16(dst + F::V_AT, src + v_off, bytes);
         }
-        const int grp = (lane >> 1) & 3, part = (lane >> 3) & 1;
-        const int id = __shfl_sync(0xffffffffu, ids, grp);
+        // parameters: 32 bytes for each eight keys; lanes 0..7 of the keys, 8..15 of the values
+        const int key = key0 + i * FLOW_TILE + ((lane >> 1) & 3) * 8;
+        const long long off = __shfl_sync(0xffffffffu, rows_off, (lane >> 1) & 3);
         if (lane < 16) {
-          const uint8_t* src = head_base + max(id, 0) * p.cache.page_stride + (long long)p.cache.page_size * D +
-                               (part * p.cache.page_size + ((key + grp * 8) & page_mask)) * 4ll + (lane & 1) * 16;
-          cp_async16(at + F::KP_AT + part * (FLOW_KEYS * 4) + grp * 32 + (lane & 1) * 16, src, id < 0 ? 0 : 16);
+          const int slot = key & page_mask;
+          const uint8_t* src = head_base + max(off, 0ll) + (2 * v_off - (long long)slot * F::ROW) + (((lane >> 3) * p.cache.page_size + slot) * 4 + (lane & 1) * 16);
+          cp_async16(at + F::KP_AT + lane * 16, src, off < 0 ? 0 : 16);
         }
-        const uint32_t live = __ballot_sync(0xffffffffu, lane < 4 && ids >= 0);
+        const uint32_t live = __ballot_sync(0xffffffffu, lane < 4 && rows_off >= 0);
         if (lane == 0) *reinterpret_cast<volatile uint32_t*>(my_smem + stage * F::STAGE + F::HEAD_AT) = live;
       }
       cp_async_commit();
     };
-    int ids = page_at(0);
+    long long ids = rows_at(0);
 #pragma unroll
     for (int i = 0; i < FLOW_STAGES - 1; i++) {
-      const int next = page_at(i + 1);
+      const long long next = rows_at(i + 1);
       issue(i, i, ids);
       ids = next;
     }
@@ -439,180 +444,184 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
     }
     int R = -112;     // 2^R is above every value step met so far, within fp32's range
 
-    for (int i = 0, stage = 0, fill = FLOW_STAGES - 1; i < nt; i++) {
-      cp_async_wait<FLOW_STAGES - 2>();
-      __syncwarp();
-      const int next = page_at(i + FLOW_STAGES);
-      const int key = key0 + i * FLOW_TILE;
-      const uint32_t at = ring + stage * F::STAGE;
-      const uint32_t live = *reinterpret_cast<volatile uint32_t*>(my_smem + stage * F::STAGE + F::HEAD_AT);
-      if (key < s.end && key + FLOW_KEYS > s.begin) {       // warp-uniform
-        const bool whole = live == 15u && key >= last_begin && key + FLOW_KEYS <= first_end;
-        // ---- scores of two tiles of 16 keys
-        float sc[2][NQ][4];
+    auto attend = [&](auto tag, int key, uint32_t at, uint32_t live) {
+      constexpr bool WHOLE = decltype(tag)::value;      // every row sees every key: no mask is looked at
+      // ---- scores of two tiles of 16 keys
+      float sc[2][NQ][4];
+#pragma unroll
+      for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+        for (int q = 0; q < NQ; q++)
+#pragma unroll
+          for (int c = 0; c < 4; c++) sc[mt][q][c] = 0.0f;
+      constexpr int WL = F::WK < 4 ? F::WK : 4;     // words of one load
+#pragma unroll
+      for (int w0 = 0; w0 < F::WK; w0 += WL) {
+        uint32_t kw[2][2][WL];
 #pragma unroll
         for (int mt = 0; mt < 2; mt++)
 #pragma unroll
-          for (int q = 0; q < NQ; q++)
+          for (int hi = 0; hi < 2; hi++) {
+            const int row = mt * 16 + hi * 8 + g;
+            const int byte = D == 64 ? 8 * t : 16 * (t + w0);      // w0 is 0 or, at D = 256, 4: chunk t or t + 4
+            lds_words<WL>(at + flow_offset<D>(row, byte >> 4) + (byte & 15), kw[mt][hi]);
+          }
 #pragma unroll
-            for (int c = 0; c < 4; c++) sc[mt][q][c] = 0.0f;
-        constexpr int WL = F::WK < 4 ? F::WK : 4;     // words of one load
+        for (int w = 0; w < WL; w++) {
 #pragma unroll
-        for (int w0 = 0; w0 < F::WK; w0 += WL) {
-          uint32_t kw[2][2][WL];
+          for (int half = 0; half < 2; half++) {
+            const int k = 2 * (w0 + w) + half;
+            uint2 bq[NQ];
 #pragma unroll
-          for (int mt = 0; mt < 2; mt++)
+            for (int q = 0; q < NQ; q++)
+              bq[q] = F::Q_IN_REGS ? make_uint2(qr[(k * NQ + q) * 2], qr[(k * NQ + q) * 2 + 1]) : q_s[(k * NQ + q) * 32 + lane];
 #pragma unroll
-            for (int hi = 0; hi < 2; hi++) {
-              const int row = mt * 16 + hi * 8 + g;
-              const int byte = D == 64 ? 8 * t : 16 * (t + w0);      // w0 is 0 or, at D = 256, 4: chunk t or t + 4
-              lds_words<WL>(at + flow_offset<D>(row, byte >> 4) + (byte & 15), kw[mt][hi]);
-            }
-#pragma unroll
-          for (int w = 0; w < WL; w++) {
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-              const int k = 2 * (w0 + w) + half;
-              uint2 bq[NQ];
+            for (int mt = 0; mt < 2; mt++) {
+              const uint32_t x = half ? kw[mt][0][w] >> 8 : kw[mt][0][w], y = half ? kw[mt][1][w] >> 8 : kw[mt][1][w];
 #pragma unroll
               for (int q = 0; q < NQ; q++)
-                bq[q] = F::Q_IN_REGS ? make_uint2(qr[(k * NQ + q) * 2], qr[(k * NQ + q) * 2 + 1]) : q_s[(k * NQ + q) * 32 + lane];
-#pragma unroll
-              for (int mt = 0; mt < 2; mt++) {
-                const uint32_t x = half ? kw[mt][0][w] >> 8 : kw[mt][0][w], y = half ? kw[mt][1][w] >> 8 : kw[mt][1][w];
-#pragma unroll
-                for (int q = 0; q < NQ; q++)
-                  mma_f16(sc[mt][q], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, bq[q].x, bq[q].y);
-              }
+                mma_f16(sc[mt][q], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, bq[q].x, bq[q].y);
             }
           }
         }
-        // ---- the rows' parameters; scores in the log2 domain; running maximum
-        float2 kp[4], vp[4];
+      }
+      // ---- the rows' parameters; scores in the log2 domain; running maximum
+      float2 kp[4], vp[4];
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          kp[r] = unpack2<BF16>(lds32(at + F::KP_AT + (r * 8 + g) * 4));
-          kp[r].x *= 16777216.0f;      // the levels are multiples of 2^-24
-          vp[r] = unpack2<BF16>(lds32(at + F::VP_AT + (r * 8 + g) * 4));
-        }
-        uint32_t seen[2 * NQ];     // bit r: the key of parameter r is visible to the row of column c
-        float top[2 * NQ];
+      for (int r = 0; r < 4; r++) {
+        kp[r] = unpack2<BF16>(lds32(at + F::KP_AT + (r * 8 + g) * 4));
+        kp[r].x *= 16777216.0f;      // the levels are multiples of 2^-24
+        vp[r] = unpack2<BF16>(lds32(at + F::VP_AT + (r * 8 + g) * 4));
+      }
+      uint32_t seen[2 * NQ];     // bit r: the key of parameter r is visible to the row of column c
+      if (!WHOLE) {
 #pragma unroll
         for (int c = 0; c < 2 * NQ; c++) {
-          seen[c] = 15u;
-          top[c] = m[c];
-        }
-        if (!whole) {
+          const int r = (c >> 1) * 8 + 2 * t + (c & 1);
+          const int pos = s.pos0 + min(r / p.group, s.n - 1);
+          const int end = p.causal ? min(s.len, pos + 1) : s.len;
+          const int begin = p.causal && p.window > 0 ? pos + 1 - p.window : 0;
+          seen[c] = 0;
 #pragma unroll
-          for (int c = 0; c < 2 * NQ; c++) {
-            const int r = (c >> 1) * 8 + 2 * t + (c & 1);
-            const int pos = s.pos0 + min(r / p.group, s.n - 1);
-            const int end = p.causal ? min(s.len, pos + 1) : s.len;
-            const int begin = p.causal && p.window > 0 ? pos + 1 - p.window : 0;
-            seen[c] = 0;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-              const int j = key + k * 8 + g;
-              if (j < end && j >= begin && ((live >> k) & 1u)) seen[c] |= 1u << k;
-            }
+          for (int k = 0; k < 4; k++) {
+            const int j = key + k * 8 + g;
+            if (j < end && j >= begin && ((live >> k) & 1u)) seen[c] |= 1u << k;
           }
         }
+      }
+      float top[2 * NQ];
 #pragma unroll
-        for (int mt = 0; mt < 2; mt++)
+      for (int c = 0; c < 2 * NQ; c++) top[c] = m[c];
 #pragma unroll
-          for (int q = 0; q < NQ; q++)
+      for (int mt = 0; mt < 2; mt++)
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-              const int r = 2 * mt + (c >> 1), col = 2 * q + (c & 1);
-              const float v = fmaf(sc[mt][q][c] * kp[r].x, qf[col], kp[r].y * ql[col]);
-              sc[mt][q][c] = whole || ((seen[col] >> r) & 1u) ? v : -INFINITY;
-              top[col] = fmaxf(top[col], sc[mt][q][c]);
-            }
-        // exponent of the largest value step of these keys (a step that is not finite shows in its weight instead)
-        uint32_t bits = __float_as_uint(fabsf(unpack2<BF16>(lds32(at + F::VP_AT + lane * 4)).x));
-        if (bits >= 0x7f800000u || (!whole && (key + lane >= s.end || key + lane < s.begin || !((live >> (lane >> 3)) & 1u)))) bits = 0;
-        const int rise = max(R, min((int)(__reduce_max_sync(0xffffffffu, bits) >> 23) - 126, 127));
-        bool moved = rise != R;
+        for (int q = 0; q < NQ; q++)
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            const int r = 2 * mt + (c >> 1), col = 2 * q + (c & 1);
+            const float v = fmaf(sc[mt][q][c] * kp[r].x, qf[col], kp[r].y * ql[col]);
+            sc[mt][q][c] = WHOLE || ((seen[col] >> r) & 1u) ? v : -INFINITY;
+            top[col] = fmaxf(top[col], sc[mt][q][c]);
+          }
+      // exponent of the largest value step of these keys (a step that is not finite shows in its weight instead)
+      uint32_t bits = __float_as_uint(fabsf(unpack2<BF16>(lds32(at + F::VP_AT + lane * 4)).x));
+      if (bits >= 0x7f800000u || (!WHOLE && (key + lane >= s.end || key + lane < s.begin || !((live >> (lane >> 3)) & 1u)))) bits = 0;
+      const int rise = max(R, min((int)(__reduce_max_sync(0xffffffffu, bits) >> 23) - 126, 127));
+      // The reference point m follows the running maximum only where that has risen by more than 2^8: weights then stay below
+      // 2^8 of it, and most tiles after a segment's first neither exchange maxima nor touch the sums.
+      bool moved = rise != R;
+#pragma unroll
+      for (int c = 0; c < 2 * NQ; c++) moved |= top[c] > m[c] + 8.0f;      // m = -inf: any key at all
+      if (__any_sync(0xffffffffu, moved)) {
+        const float shrink = __uint_as_float((uint32_t)max(127 + R - rise, 0) << 23);      // 2^(R - rise)
+        R = rise;
 #pragma unroll
         for (int c = 0; c < 2 * NQ; c++) {
 #pragma unroll
           for (int d = 4; d < 32; d *= 2) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], d));
-          moved |= top[c] != m[c];
+          const float keep = m[c] == top[c] ? 1.0f : ex2(m[c] - top[c]);       // -inf - x: 0
+          m[c] = top[c];
+          l[c] *= keep;
+          vsum[c] *= keep;
+          const float k = keep * shrink;
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            ones[c >> 1][(c & 1) + 2 * e] *= k;
+#pragma unroll
+            for (int w = 0; w < F::WV; w++)
+#pragma unroll
+              for (int j = 0; j < 4; j++) o[w][j][c >> 1][(c & 1) + 2 * e] *= k;
+          }
         }
-        if (__any_sync(0xffffffffu, moved)) {
-          const float shrink = __uint_as_float((uint32_t)max(127 + R - rise, 0) << 23);      // 2^(R - rise)
-          R = rise;
+      }
+      // ---- weights, and their products with the values
+      const float lift = __uint_as_float((uint32_t)(127 + 6 - R) << 23);     // 2^(6 - R)
+      float base[2 * NQ];
 #pragma unroll
-          for (int c = 0; c < 2 * NQ; c++) {
-            const float keep = m[c] == top[c] ? 1.0f : ex2(m[c] - top[c]);       // -inf - x: 0
-            m[c] = top[c];
-            l[c] *= keep;
-            vsum[c] *= keep;
-            const float k = keep * shrink;
+      for (int c = 0; c < 2 * NQ; c++) base[c] = m[c] == -INFINITY ? 0.0f : m[c];
+      float step[4], mid[4];
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-              ones[c >> 1][(c & 1) + 2 * e] *= k;
+      for (int r = 0; r < 4; r++) {
+        step[r] = vp[r].x * lift;
+        mid[r] = fmaf(8.0f, vp[r].x, vp[r].y);
+      }
+      uint32_t wt[2][NQ][2];
 #pragma unroll
-              for (int w = 0; w < F::WV; w++)
+      for (int mt = 0; mt < 2; mt++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) o[w][j][c >> 1][(c & 1) + 2 * e] *= k;
+        for (int q = 0; q < NQ; q++) {
+          float w[4];
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            const int r = 2 * mt + (c >> 1), col = 2 * q + (c & 1);
+            const float e = ex2(sc[mt][q][c] - base[col]);
+            l[col] += e;
+            const bool on = WHOLE || ((seen[col] >> r) & 1u);      // a masked place may hold NaN
+            w[c] = on ? e * step[r] : 0.0f;
+            vsum[col] += on ? e * mid[r] : 0.0f;
+          }
+          wt[mt][q][0] = transpose8x8(pack2<false>(w[0], w[1]));
+          wt[mt][q][1] = transpose8x8(pack2<false>(w[2], w[3]));
+        }
+#pragma unroll
+      for (int mt = 0; mt < 2; mt++) {
+        uint32_t vw[4][F::WV];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int row = mt * 16 + (k >> 1) * 8 + 2 * t + (k & 1);
+          const int byte = 4 * F::WV * g;
+          lds_words<F::WV>(at + F::V_AT + flow_offset<D>(row, byte >> 4) + (byte & 15), vw[k]);
+        }
+#pragma unroll
+        for (int q = 0; q < NQ; q++) mma_f16(ones[q], 0x00010001u, 0x00010001u, 0x00010001u, 0x00010001u, wt[mt][q][0], wt[mt][q][1]);
+#pragma unroll
+        for (int w = 0; w < F::WV; w++) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            uint32_t x = __byte_perm(vw[0][w], vw[1][w], j < 2 ? 0x5410 : 0x7632);
+            uint32_t y = __byte_perm(vw[2][w], vw[3][w], j < 2 ? 0x5410 : 0x7632);
+            if (j & 1) {
+              x >>= 8;
+              y >>= 8;
             }
+#pragma unroll
+            for (int q = 0; q < NQ; q++)
+              mma_f16(o[w][j][q], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, wt[mt][q][0], wt[mt][q][1]);
           }
         }
-        // ---- weights, and their products with the values
-        const float lift = __uint_as_float((uint32_t)(127 + 14 - R) << 23);     // 2^(14 - R)
-        float step[4], mid[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          step[r] = vp[r].x * lift;
-          mid[r] = fmaf(8.0f, vp[r].x, vp[r].y);
-        }
-        uint32_t wt[2][NQ][2];
-#pragma unroll
-        for (int mt = 0; mt < 2; mt++)
-#pragma unroll
-          for (int q = 0; q < NQ; q++) {
-            float w[4];
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-              const int r = 2 * mt + (c >> 1), col = 2 * q + (c & 1);
-              const float base = m[col] == -INFINITY ? 0.0f : m[col];
-              const float e = ex2(sc[mt][q][c] - base);
-              l[col] += e;
-              const bool on = whole || ((seen[col] >> r) & 1u);      // a masked place may hold NaN
-              w[c] = on ? e * step[r] : 0.0f;
-              vsum[col] += on ? e * mid[r] : 0.0f;
-            }
-            wt[mt][q][0] = transpose8x8(pack2<false>(w[0], w[1]));
-            wt[mt][q][1] = transpose8x8(pack2<false>(w[2], w[3]));
-          }
-#pragma unroll
-        for (int mt = 0; mt < 2; mt++) {
-          uint32_t vw[4][F::WV];
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            const int row = mt * 16 + (k >> 1) * 8 + 2 * t + (k & 1);
-            const int byte = 4 * F::WV * g;
-            lds_words<F::WV>(at + F::V_AT + flow_offset<D>(row, byte >> 4) + (byte & 15), vw[k]);
-          }
-#pragma unroll
-          for (int q = 0; q < NQ; q++) mma_f16(ones[q], 0x00010001u, 0x00010001u, 0x00010001u, 0x00010001u, wt[mt][q][0], wt[mt][q][1]);
-#pragma unroll
-          for (int w = 0; w < F::WV; w++) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-              uint32_t x = __byte_perm(vw[0][w], vw[1][w], j < 2 ? 0x5410 : 0x7632);
-              uint32_t y = __byte_perm(vw[2][w], vw[3][w], j < 2 ? 0x5410 : 0x7632);
-              if (j & 1) {
-                x >>= 8;
-                y >>= 8;
-              }
-#pragma unroll
-              for (int q = 0; q < NQ; q++)
-                mma_f16(o[w][j][q], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, wt[mt][q][0], wt[mt][q][1]);
-            }
-          }
-        }
+      }
+    };
+
+    for (int i = 0, stage = 0, fill = FLOW_STAGES - 1; i < nt; i++) {
+      cp_async_wait<FLOW_STAGES - 2>();
+      __syncwarp();
+      const long long next = rows_at(i + FLOW_STAGES);
+      const int key = key0 + i * FLOW_TILE;
+      const uint32_t at = ring + stage * F::STAGE;
+      const uint32_t live = *reinterpret_cast<volatile uint32_t*>(my_smem + stage * F::STAGE + F::HEAD_AT);
+      if (key < s.end && key + FLOW_KEYS > s.begin) {       // warp-uniform
+        if (live == 15u && key >= last_begin && key + FLOW_KEYS <= first_end) attend(std::true_type(), key, at, live);
+        else attend(std::false_type(), key, at, live);
       }
       __syncwarp();
       issue(i + FLOW_STAGES - 1, fill, ids);
@@ -626,7 +635,7 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
     // ---- the four warps' results meet in shared memory
     {
       float* mine = reinterpret_cast<float*>(my_smem);
-      const float unit = __uint_as_float((uint32_t)(127 + 24 - 14) << 23);
+      const float unit = __uint_as_float((uint32_t)(127 + 24 - 6) << 23);
       const float lower = __uint_as_float((uint32_t)(127 + R) << 23);       // R >= -112
 #pragma unroll
       for (int c = 0; c < 2 * NQ; c++) {
@@ -699,37 +708,74 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
   }
 }
 
-// Joins the partial results of the (sequence, head)s that lie in several blocks, in the order of their keys.
+// Joins the partial results of the (sequence, head)s that lie in several blocks.  A warp takes one row and every WARPS-th piece
+// of it, lanes over the row's elements; the warps meet in shared memory.  The order is fixed by the shares.
+constexpr int JOIN_WARPS = 8;
+
 template <bool BF16, int D, int NQ>
-__global__ void __launch_bounds__(128) kv4_attention_join_kernel(const FlowParams fp) {
+__global__ void __launch_bounds__(32 * JOIN_WARPS) kv4_attention_join_kernel(const FlowParams fp) {
   using F = Flow<D, NQ>;
   const AttentionParams& p = fp.a;
+  constexpr int V = D / 128 > 0 ? D / 128 : 1;     // float4 per lane (D = 64: half the lanes)
+  __shared__ float4 part_s[JOIN_WARPS][D / 4];
+  __shared__ float2 ml_s[JOIN_WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependency_wait();
   const int bh = blockIdx.x, b = bh / p.cache.heads, h = bh - b * p.cache.heads;
   const Span s = span_of<FLOW_TILE>(p, b);
   if (s.n <= 0) return;
   const int2 pc = __ldcg(fp.pieces + bh);
   if (pc.y == 0) return;
-  for (int e = blockIdx.y * 128 + threadIdx.x; e < s.n * p.group * (D / 4); e += 128 * gridDim.y) {
-    const int r = e / (D / 4), d = (e % (D / 4)) * 4;
+  for (int r = blockIdx.y; r < s.n * p.group; r += gridDim.y) {
     float M = -INFINITY, L = 0.0f;
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float4 v[V];
+#pragma unroll
+    for (int k = 0; k < V; k++) v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-    for (int i = 0; i < pc.y; i++) {
+    for (int i = warp; i < pc.y; i += JOIN_WARPS) {
       const float* slot = fp.slots + (2ll * (pc.x + i) + (i == 0 ? 1 : 0)) * F::SLOT;
       const float2 ml = __ldcg(reinterpret_cast<const float2*>(slot + r * 2));
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(slot + F::ROWS * 2 + r * D + d));
-      if (ml.x == -INFINITY && ml.y == 0.0f) continue;
+      float4 x[V];
+#pragma unroll
+      for (int k = 0; k < V; k++)
+        if (D >= 128 || lane < D / 4) x[k] = __ldcg(reinterpret_cast<const float4*>(slot + F::ROWS * 2 + r * D) + k * 32 + lane);
+      if (ml.x == -INFINITY && ml.y == 0.0f) continue;      // no key: nothing was written that counts
       const float top = fmaxf(M, ml.x);
-      const float f = M == top ? 1.0f : ex2(M - top), k = ml.x == top ? 1.0f : ex2(ml.x - top);
+      const float f = M == top ? 1.0f : ex2(M - top), g = ml.x == top ? 1.0f : ex2(ml.x - top);
       M = top;
-      L = L * f + k * ml.y;
-      v.x = v.x * f + k * x.x;
-      v.y = v.y * f + k * x.y;
-      v.z = v.z * f + k * x.z;
-      v.w = v.w * f + k * x.w;
+      L = L * f + g * ml.y;
+#pragma unroll
+      for (int k = 0; k < V; k++)
+        if (D >= 128 || lane < D / 4) {
+          v[k].x = v[k].x * f + g * x[k].x;
+          v[k].y = v[k].y * f + g * x[k].y;
+          v[k].z = v[k].z * f + g * x[k].z;
+          v[k].w = v[k].w * f + g * x[k].w;
+        }
     }
-    finish_row<BF16, D>(p, s, h, r, d, M, L, v);
+#pragma unroll
+    for (int k = 0; k < V; k++)
+      if (D >= 128 || lane < D / 4) part_s[warp][k * 32 + lane] = v[k];
+    if (lane == 0) ml_s[warp] = make_float2(M, L);
+    __syncthreads();
+    if (threadIdx.x < D / 4) {
+      float top = -INFINITY, sum = 0.0f;
+      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int w = 0; w < JOIN_WARPS; w++) top = fmaxf(top, ml_s[w].x);
+      for (int w = 0; w < JOIN_WARPS; w++) {
+        const float2 ml = ml_s[w];
+        if (ml.x == -INFINITY && ml.y == 0.0f) continue;
+        const float f = ml.x == top ? 1.0f : ex2(ml.x - top);
+        const float4 x = part_s[w][threadIdx.x];
+        sum += f * ml.y;
+        o.x += f * x.x;
+        o.y += f * x.y;
+        o.z += f * x.z;
+        o.w += f * x.w;
+      }
+      finish_row<BF16, D>(p, s, h, r, threadIdx.x * 4, top, sum, o);
+    }
+    __syncthreads();
   }
 }
 
@@ -776,10 +822,10 @@ apnn_status launch_flow(cudaStream_t stream, const FlowPlan& f, const FlowParams
   e = cudaLaunchKernelEx(&cfg, kv4_attention_flow_kernel<BF16, D, NQ>, fp);
   if (e != cudaSuccess) return cuda_fail(e, "kv4_attention_flow_kernel");
   if (!f.split) return APNN_OK;
-  int parts = 1;     // blocks that share the rows of a (sequence, head): a few pairs alone would leave the device idle
-  while (parts < 8 && (long long)f.join * parts < 2 * device_sm_count() && parts * 128 * 4 < 8 * NQ * D) parts *= 2;
+  int parts = 1;     // blocks that share the rows of a (sequence, head)
+  while (parts < 8 * NQ && (long long)f.join * parts < 2 * device_sm_count()) parts *= 2;
   cfg.gridDim = dim3((unsigned)f.join, (unsigned)parts, 1);
-  cfg.blockDim = dim3(128, 1, 1);
+  cfg.blockDim = dim3(32 * JOIN_WARPS, 1, 1);
   cfg.dynamicSmemBytes = 0;
   e = cudaLaunchKernelEx(&cfg, kv4_attention_join_kernel<BF16, D, NQ>, fp);
   return e == cudaSuccess ? APNN_OK : cuda_fail(e, "kv4_attention_join_kernel");
