@@ -19,6 +19,7 @@ struct AttentionParams {
   long long q_stride, out_stride;
   int q_heads, group, causal, window;
   float scale;
+  int* status_flag;
 };
 
 // One warp per row and query head, lanes over the head's elements.
@@ -29,6 +30,7 @@ __global__ void __launch_bounds__(128) kv4_attention_rows_kernel(const Attention
   const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int t = (int)(item / p.q_heads), h = (int)(item % p.q_heads);
   grid_dependency_wait();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.status_flag = 0;
   if (t >= p.batch.rows) return;
   const int b = sequence_of(p.batch.cu_q, p.batch.sequences, t, lane);
   if (b < 0) return;
@@ -149,6 +151,10 @@ constexpr int FLOW_WARPS = 4;
 constexpr int FLOW_KEYS = 32;                       // per warp and tile
 constexpr int FLOW_TILE = FLOW_WARPS * FLOW_KEYS;   // 128
 constexpr int FLOW_STAGES = 3;
+#ifndef SEGC
+#define SEGC 2
+#endif
+constexpr int FLOW_SEGMENT = SEGC;   // what beginning and ending a (sequence, head) costs, in tiles, when work is shared out
 constexpr int UNSPLIT_KEYS = 512;   // tables of at most this many positions: no split, no second launch
 
 template <int D, int NQ>
@@ -156,28 +162,53 @@ struct Flow {
   static constexpr int WK = D / 32;    // words of a key row per lane (four lanes hold a row)
   static constexpr int WV = D / 64;    // words of a value row per lane (eight lanes)
   static constexpr int ROW = D / 2;
-  static constexpr int CHUNKS = ROW / 16;
-  static constexpr int V_AT = FLOW_KEYS * ROW, KP_AT = 2 * V_AT, VP_AT = KP_AT + FLOW_KEYS * 4, HEAD_AT = VP_AT + FLOW_KEYS * 4;
-  static constexpr int STAGE = HEAD_AT + 128;
+  static constexpr int V_AT = FLOW_KEYS * ROW, KP_AT = 2 * V_AT, VP_AT = KP_AT + FLOW_KEYS * 4;
+  static constexpr int STAGE = VP_AT + FLOW_KEYS * 4;
   static constexpr int RING = FLOW_STAGES * STAGE;
   static constexpr int ROWS = 8 * NQ;
   static constexpr int MERGE = ROWS * (D + 4) * 4;       // a warp's part of the exchange at a segment's end: o, then m and l
   static constexpr int PER_WARP = RING > MERGE ? RING : MERGE;
   static constexpr bool Q_IN_REGS = NQ * WK <= 4;
   static constexpr int Q_BYTES = Q_IN_REGS ? 0 : 2 * WK * NQ * 32 * 8;
-  static constexpr int SMEM = FLOW_WARPS * PER_WARP + Q_BYTES + ROWS * 8 + 256;
+  static constexpr int SMEM = FLOW_WARPS * PER_WARP + Q_BYTES + ROWS * 8 + 512;
   static constexpr int BLOCKS = NQ == 1 ? (D == 256 ? 2 : 4) : NQ == 2 ? (D == 256 ? 2 : 3) : 2;   // per SM
   static constexpr int SLOT = ROWS * (D + 2);            // floats of a partial result
 };
 
-// Byte offset of 16-byte chunk `chunk` of row `row` in a stage: rows of D/2 bytes in 128-byte lines whose chunks are
-// exchanged so that both readers are free of bank conflicts -- keys, eight lanes over whole lines; values, lanes over the
-// same chunk of rows 0, 2, 4, 6.
-template <int D>
-__device__ __forceinline__ int flow_offset(int row, int chunk) {
-  if (D == 64) return (row >> 2) * 128 + ((((row & 3) * 2 + chunk) ^ (((row >> 2) & 1) * 2)) << 4);
-  if (D == 128) return (row >> 1) * 128 + ((((row & 1) * 4 + chunk) ^ (((row >> 1) & 1) * 4) ^ (((row >> 2) & 1) * 2)) << 4);
-  return row * 128 + ((chunk ^ (row & 6) ^ ((row & 1) * 4)) << 4);
+// The key of row r of an MMA operand, within eight: keys 2 t of the four lanes that read different value rows at once then lie
+// in different banks (D = 64; two by two at D = 128), while eight lanes that read key rows still take whole 128-byte lines.
+__device__ __forceinline__ int flow_key(int r) { return r ^ ((r >> 1) & 1) ^ ((r >> 2) & 1); }
+
+// Two fp32 in one instruction.
+struct Pair { unsigned long long v; };
+__device__ __forceinline__ Pair pair(float x, float y) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(x), "f"(y));
+  return p;
+}
+__device__ __forceinline__ float2 unpair(Pair p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+  return f;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
 }
 
 // One sequence of the call: which rows, which keys any of them sees.
@@ -213,6 +244,7 @@ struct FlowParams {
   int2* pieces;     // [sequences * heads]: first block and number of the partial results of a (sequence, head), 0: none
   float* slots;     // [2 * blocks][Flow::SLOT]
   int split;
+  int run_shift;    // log2 of the keys of a tile's 32 that lie in one page: 3, 4 or 5
 };
 
 template <bool BF16, int D, int NQ>
@@ -227,22 +259,31 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
   uint2* q_s = reinterpret_cast<uint2*>(smem + FLOW_WARPS * F::PER_WARP);
   float2* qf_s = reinterpret_cast<float2*>(smem + FLOW_WARPS * F::PER_WARP + F::Q_BYTES);   // per row: factor of the products, of the lows
   int* scan_s = reinterpret_cast<int*>(smem + FLOW_WARPS * F::PER_WARP + F::Q_BYTES + F::ROWS * 8);
+  // per warp and stage: a barrier that the copies complete on, and which of the four groups of eight keys there are
+  const uint32_t bars = smem_u32(scan_s) + 128 + warp * (FLOW_STAGES * 8);
+  volatile uint32_t* live_s = reinterpret_cast<volatile uint32_t*>(scan_s + 64) + warp * FLOW_STAGES;
   const int heads = p.cache.heads, sequences = p.batch.sequences;
+  if (lane < FLOW_STAGES) mbar_init(bars + 8 * lane, 1);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  __syncthreads();
   grid_dependency_wait();
   grid_launch_dependents();   // the joining kernel waits for this whole grid anyway
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.status_flag = 0;
 
-  // ---- which units (sequence, head, tile) this block takes: an equal share of all, in order
-  int u0, u1, b = 0, h = 0, t0 = 0, stride = 0;
-  long long total = 0, sharing = 0;
+  // ---- which units this block takes: an equal share of all, in order.  A (sequence, head) is FLOW_SEGMENT units of overhead,
+  // then a unit for each tile.
+  int u0, u1, b = 0, h = 0, loc = 0;
+  long long total = 0, sharing = 0;     // blocks that take part
   Span s;
+  auto weight = [&](const Span& x) { return x.tiles == 0 ? 0 : (x.tiles + FLOW_SEGMENT) * heads; };
   if (fp.split) {
     int sum = 0;
-    for (int i = threadIdx.x; i < sequences; i += 32 * FLOW_WARPS) sum += span_of<FLOW_TILE>(p, i).tiles;
+    for (int i = threadIdx.x; i < sequences; i += 32 * FLOW_WARPS) sum += weight(span_of<FLOW_TILE>(p, i));
     sum = __reduce_add_sync(0xffffffffu, sum);
     if (lane == 0) scan_s[warp] = sum;
     __syncthreads();
-    total = (long long)(scan_s[0] + scan_s[1] + scan_s[2] + scan_s[3]) * heads;
-    sharing = min(total, (long long)gridDim.x);     // so that no share is empty: the joining kernel counts on every block between
+    total = (long long)scan_s[0] + scan_s[1] + scan_s[2] + scan_s[3];
+    sharing = min(total, (long long)gridDim.x);     // no share is empty: the joining kernel counts on every block between two
     if (blockIdx.x >= sharing) return;
     u0 = (int)(total * blockIdx.x / sharing);
     u1 = (int)(total * (blockIdx.x + 1) / sharing);
@@ -251,7 +292,7 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
     for (int base = 0;; base += 32 * FLOW_WARPS) {
       __syncthreads();
       const int i = base + threadIdx.x;
-      const int mine = i < sequences ? span_of<FLOW_TILE>(p, i).tiles * heads : 0;
+      const int mine = i < sequences ? weight(span_of<FLOW_TILE>(p, i)) : 0;
       int inc = mine;
 #pragma unroll
       for (int d = 1; d < 32; d *= 2) {
@@ -272,82 +313,75 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
     __syncthreads();
     b = scan_s[8];
     s = span_of<FLOW_TILE>(p, b);
-    h = (u0 - scan_s[9]) / s.tiles;
-    t0 = (u0 - scan_s[9]) - h * s.tiles;
+    h = (u0 - scan_s[9]) / (s.tiles + FLOW_SEGMENT);
+    loc = (u0 - scan_s[9]) - h * (s.tiles + FLOW_SEGMENT);
   } else {
-    // one block takes a (sequence, head) whole
-    stride = gridDim.x;
+    // a block takes a (sequence, head) whole
     u0 = blockIdx.x;
     u1 = sequences * heads;
   }
+  int stage = 0, fill = 0;      // ring slot to read, to fill; both have passed the same number of tiles between segments
+  uint32_t phase = 0;           // of the slot to read
+  bool ok = true;
 
   for (int u = u0; u < u1;) {
-    int nt;
+    int t0 = 0, nt, bh_unit = 0;
     if (fp.split) {
       while (s.tiles == 0 || h == heads) {     // on to the next sequence with rows
         h = 0;
         s = span_of<FLOW_TILE>(p, ++b);
       }
-      nt = min(s.tiles - t0, u1 - u);
+      bh_unit = u - loc;
+      t0 = max(loc - FLOW_SEGMENT, 0);
+      nt = min(s.tiles, u1 - bh_unit - FLOW_SEGMENT) - t0;
     } else {
       b = u / heads;
       h = u - b * heads;
       s = span_of<FLOW_TILE>(p, b);
-      if (s.tiles == 0) {
-        u += stride;
-        continue;
-      }
       nt = s.tiles;
+    }
+    const int next_u = fp.split ? bh_unit + s.tiles + FLOW_SEGMENT : u + gridDim.x;
+    if (nt <= 0) {      // only overhead units lie in this share, or a sequence without rows
+      u = next_u;
+      loc = 0;
+      if (fp.split) h++;
+      continue;
     }
     const int rows = s.n * p.group;     // at most 8 NQ
 
-    // ---- pipeline of this warp's 32-key pieces of the segment
+    // ---- copies of this warp's 32-key pieces of the segment: per run of keys in one page its key levels, value levels and
+    // the parameters of both, a lane each
     const int key0 = (s.tile0 + t0) * FLOW_TILE + warp * FLOW_KEYS;
+    const int run = lane >> 2, part = lane & 3, run_keys = 1 << fp.run_shift;
+    const bool copies = run < (FLOW_KEYS >> fp.run_shift);
+    const int unit_bytes = part < 2 ? F::ROW : 4;
+    const uint8_t* part_base = p.cache.data + h * p.cache.head_bytes + (long long)p.cache.page_size * (part < 2 ? part * F::ROW : D + (part - 2) * 4);
+    const uint32_t part_dst = ring + (part == 0 ? 0 : part == 1 ? F::V_AT : part == 2 ? F::KP_AT : F::VP_AT) + run * run_keys * unit_bytes;
     const int* trow = p.batch.table + (long long)b * p.batch.table_stride;
-    const uint8_t* head_base = p.cache.data + h * p.cache.head_bytes;
-    const int page_mask = p.cache.page_size - 1;
-    const long long v_off = (long long)p.cache.page_size * F::ROW;     // from a key row to its value row
-    // where the eight keys that lane % 4 answers for start in head h, of tile i, as an offset into the cache; -1 where there is
-    // nothing to read
-    auto rows_at = [&](int i) -> long long {
-      const int key = key0 + i * FLOW_TILE + (lane & 3) * 8;
-      if (i >= nt || key >= s.end || key < 0) return -1;      // key < len <= table_width * page_size: within the table
+    auto source = [&](int i) -> const uint8_t* {
+      const int key = key0 + i * FLOW_TILE + run * run_keys;
+      if (!copies || i >= nt || key >= s.end || key < 0) return nullptr;      // key < len <= table_width * page_size: within the table
       const int id = __ldg(trow + (key >> p.cache.page_shift));
-      return id < 0 || id >= p.cache.pages ? -1 : id * p.cache.page_stride + (long long)(key & page_mask) * F::ROW;
+      return id < 0 || id >= p.cache.pages ? nullptr : part_base + id * p.cache.page_stride + (long long)(key & (p.cache.page_size - 1)) * unit_bytes;
     };
-    auto issue = [&](int i, int stage, long long rows_off) {
-      if (i < nt) {
-        const uint32_t at = ring + stage * F::STAGE;
-        constexpr int ROWS_PER = 32 / F::CHUNKS;     // rows a warp-wide copy takes: they lie one behind the other in a page
-#pragma unroll
-        for (int c = 0; c < FLOW_KEYS / ROWS_PER; c++) {
-          const int row = c * ROWS_PER + lane / F::CHUNKS;
-          const long long off = __shfl_sync(0xffffffffu, rows_off, row >> 3);
-          const uint8_t* src = head_base + max(off, 0ll) + ((row & 7) * F::ROW + (lane % F::CHUNKS) * 16);
-          const uint32_t dst = at + flow_offset<D>(row, lane % F::CHUNKS);
-          const int bytes = off < 0 ? 0 : 16;
-          cp_async16(dst, src, bytes);
-          cp_async16(dst + F::V_AT, src + v_off, bytes);
-        }
-        // parameters: 32 bytes for each eight keys; lanes 0..7 of the keys, 8..15 of the values
-        const int key = key0 + i * FLOW_TILE + ((lane >> 1) & 3) * 8;
-        const long long off = __shfl_sync(0xffffffffu, rows_off, (lane >> 1) & 3);
-        if (lane < 16) {
-          const int slot = key & page_mask;
-          const uint8_t* src = head_base + max(off, 0ll) + (2 * v_off - (long long)slot * F::ROW) + (((lane >> 3) * p.cache.page_size + slot) * 4 + (lane & 1) * 16);
-          cp_async16(at + F::KP_AT + lane * 16, src, off < 0 ? 0 : 16);
-        }
-        const uint32_t live = __ballot_sync(0xffffffffu, lane < 4 && rows_off >= 0);
-        if (lane == 0) *reinterpret_cast<volatile uint32_t*>(my_smem + stage * F::STAGE + F::HEAD_AT) = live;
+    auto issue = [&](int i, const uint8_t* src) {
+      if (i >= nt || !ok) return;
+      const bool group_live = __shfl_sync(0xffffffffu, src != nullptr, (((lane & 3) * 8) >> fp.run_shift) * 4);
+      const uint32_t live = __ballot_sync(0xffffffffu, group_live) & 15u;
+      if (lane == 0) {
+        live_s[fill] = live;
+        mbar_expect_tx(bars + 8 * fill, __popc(live) * 8 * (2 * F::ROW + 8));
       }
-      cp_async_commit();
+      __syncwarp();
+      if (src != nullptr) bulk_load(part_dst + fill * F::STAGE, src, run_keys * unit_bytes, bars + 8 * fill);
+      fill = fill + 1 == FLOW_STAGES ? 0 : fill + 1;
     };
-    long long ids = rows_at(0);
+    const uint8_t* src = source(0);
 #pragma unroll
     for (int i = 0; i < FLOW_STAGES - 1; i++) {
-      const long long next = rows_at(i + 1);
-      issue(i, i, ids);
-      ids = next;
+      const uint8_t* next = source(i + 1);
+      issue(i, src);
+      src = next;
     }
 
     // ---- the queries as fp16 operands, while the first keys are on their way.  A group of four lanes (t) shares a row.
@@ -414,19 +448,20 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
       }
     }
     __syncthreads();
-    float qf[2 * NQ], ql[2 * NQ];
+    Pair qf[NQ], ql[NQ];
 #pragma unroll
-    for (int c = 0; c < 2 * NQ; c++) {
-      const float2 f = qf_s[(c >> 1) * 8 + 2 * t + (c & 1)];
-      qf[c] = f.x;
-      ql[c] = f.y;
+    for (int q = 0; q < NQ; q++) {
+      const float2 f0 = qf_s[q * 8 + 2 * t], f1 = qf_s[q * 8 + 2 * t + 1];
+      qf[q] = pair(f0.x, f1.x);
+      ql[q] = pair(f0.y, f1.y);
     }
     // the keys every row sees: no mask is looked at there
     const int last_begin = p.causal && p.window > 0 ? max(0, s.pos0 + s.n - p.window) : 0;
     const int first_end = p.causal ? min(s.len, s.pos0 + 1) : s.len;
 
     float o[F::WV][4][NQ][4], ones[NQ][4];
-    float m[2 * NQ], l[2 * NQ], vsum[2 * NQ];
+    float m[2 * NQ];
+    Pair l[NQ], vsum[NQ];
 #pragma unroll
     for (int q = 0; q < NQ; q++)
 #pragma unroll
@@ -438,10 +473,10 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
           for (int j = 0; j < 4; j++) o[w][j][q][c] = 0.0f;
       }
 #pragma unroll
-    for (int c = 0; c < 2 * NQ; c++) {
-      m[c] = -INFINITY;
-      l[c] = vsum[c] = 0.0f;
-    }
+    for (int c = 0; c < 2 * NQ; c++) m[c] = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < NQ; q++) l[q] = vsum[q] = pair(0.0f, 0.0f);
+    const int fk = flow_key(g), fv = flow_key(2 * t);
     int R = -112;     // 2^R is above every value step met so far, within fp32's range
 
     auto attend = [&](auto tag, int key, uint32_t at, uint32_t live) {
@@ -462,9 +497,8 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
         for (int mt = 0; mt < 2; mt++)
 #pragma unroll
           for (int hi = 0; hi < 2; hi++) {
-            const int row = mt * 16 + hi * 8 + g;
-            const int byte = D == 64 ? 8 * t : 16 * (t + w0);      // w0 is 0 or, at D = 256, 4: chunk t or t + 4
-            lds_words<WL>(at + flow_offset<D>(row, byte >> 4) + (byte & 15), kw[mt][hi]);
+            // w0 is 0 or, at D = 256, 4: bytes 16 t or 64 + 16 t
+            lds_words<WL>(at + (mt * 16 + hi * 8) * F::ROW + fk * F::ROW + 4 * WL * t + 16 * w0, kw[mt][hi]);
           }
 #pragma unroll
         for (int w = 0; w < WL; w++) {
@@ -489,9 +523,9 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
       float2 kp[4], vp[4];
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        kp[r] = unpack2<BF16>(lds32(at + F::KP_AT + (r * 8 + g) * 4));
+        kp[r] = unpack2<BF16>(lds32(at + F::KP_AT + r * 32 + fk * 4));
         kp[r].x *= 16777216.0f;      // the levels are multiples of 2^-24
-        vp[r] = unpack2<BF16>(lds32(at + F::VP_AT + (r * 8 + g) * 4));
+        vp[r] = unpack2<BF16>(lds32(at + F::VP_AT + r * 32 + fk * 4));
       }
       uint32_t seen[2 * NQ];     // bit r: the key of parameter r is visible to the row of column c
       if (!WHOLE) {
@@ -504,7 +538,7 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
           seen[c] = 0;
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            const int j = key + k * 8 + g;
+            const int j = key + k * 8 + fk;
             if (j < end && j >= begin && ((live >> k) & 1u)) seen[c] |= 1u << k;
           }
         }
@@ -513,16 +547,16 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
 #pragma unroll
       for (int c = 0; c < 2 * NQ; c++) top[c] = m[c];
 #pragma unroll
-      for (int mt = 0; mt < 2; mt++)
+      for (int r = 0; r < 4; r++)
 #pragma unroll
-        for (int q = 0; q < NQ; q++)
-#pragma unroll
-          for (int c = 0; c < 4; c++) {
-            const int r = 2 * mt + (c >> 1), col = 2 * q + (c & 1);
-            const float v = fmaf(sc[mt][q][c] * kp[r].x, qf[col], kp[r].y * ql[col]);
-            sc[mt][q][c] = WHOLE || ((seen[col] >> r) & 1u) ? v : -INFINITY;
-            top[col] = fmaxf(top[col], sc[mt][q][c]);
-          }
+        for (int q = 0; q < NQ; q++) {
+          float* x = sc[r >> 1][q] + 2 * (r & 1);
+          const float2 v = unpair(fma2(mul2(pair(x[0], x[1]), pair(kp[r].x, kp[r].x)), qf[q], mul2(pair(kp[r].y, kp[r].y), ql[q])));
+          x[0] = WHOLE || ((seen[2 * q] >> r) & 1u) ? v.x : -INFINITY;
+          x[1] = WHOLE || ((seen[2 * q + 1] >> r) & 1u) ? v.y : -INFINITY;
+          top[2 * q] = fmaxf(top[2 * q], x[0]);
+          top[2 * q + 1] = fmaxf(top[2 * q + 1], x[1]);
+        }
       // exponent of the largest value step of these keys (a step that is not finite shows in its weight instead)
       uint32_t bits = __float_as_uint(fabsf(unpack2<BF16>(lds32(at + F::VP_AT + lane * 4)).x));
       if (bits >= 0x7f800000u || (!WHOLE && (key + lane >= s.end || key + lane < s.begin || !((live >> (lane >> 3)) & 1u)))) bits = 0;
@@ -535,15 +569,15 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
       if (__any_sync(0xffffffffu, moved)) {
         const float shrink = __uint_as_float((uint32_t)max(127 + R - rise, 0) << 23);      // 2^(R - rise)
         R = rise;
+        float kept[2 * NQ];
 #pragma unroll
         for (int c = 0; c < 2 * NQ; c++) {
 #pragma unroll
           for (int d = 4; d < 32; d *= 2) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], d));
           const float keep = m[c] == top[c] ? 1.0f : ex2(m[c] - top[c]);       // -inf - x: 0
           m[c] = top[c];
-          l[c] *= keep;
-          vsum[c] *= keep;
           const float k = keep * shrink;
+          kept[c] = keep;
 #pragma unroll
           for (int e = 0; e < 2; e++) {
             ones[c >> 1][(c & 1) + 2 * e] *= k;
@@ -553,44 +587,46 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
               for (int j = 0; j < 4; j++) o[w][j][c >> 1][(c & 1) + 2 * e] *= k;
           }
         }
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+          l[q] = mul2(l[q], pair(kept[2 * q], kept[2 * q + 1]));
+          vsum[q] = mul2(vsum[q], pair(kept[2 * q], kept[2 * q + 1]));
+        }
       }
       // ---- weights, and their products with the values
       const float lift = __uint_as_float((uint32_t)(127 + 6 - R) << 23);     // 2^(6 - R)
-      float base[2 * NQ];
+      Pair below[NQ];     // minus the reference points
 #pragma unroll
-      for (int c = 0; c < 2 * NQ; c++) base[c] = m[c] == -INFINITY ? 0.0f : m[c];
-      float step[4], mid[4];
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        step[r] = vp[r].x * lift;
-        mid[r] = fmaf(8.0f, vp[r].x, vp[r].y);
-      }
+      for (int q = 0; q < NQ; q++)
+        below[q] = pair(m[2 * q] == -INFINITY ? 0.0f : -m[2 * q], m[2 * q + 1] == -INFINITY ? 0.0f : -m[2 * q + 1]);
       uint32_t wt[2][NQ][2];
 #pragma unroll
-      for (int mt = 0; mt < 2; mt++)
+      for (int r = 0; r < 4; r++) {
+        const float step = vp[r].x * lift, mid = fmaf(8.0f, vp[r].x, vp[r].y);
 #pragma unroll
         for (int q = 0; q < NQ; q++) {
-          float w[4];
-#pragma unroll
-          for (int c = 0; c < 4; c++) {
-            const int r = 2 * mt + (c >> 1), col = 2 * q + (c & 1);
-            const float e = ex2(sc[mt][q][c] - base[col]);
-            l[col] += e;
-            const bool on = WHOLE || ((seen[col] >> r) & 1u);      // a masked place may hold NaN
-            w[c] = on ? e * step[r] : 0.0f;
-            vsum[col] += on ? e * mid[r] : 0.0f;
+          const float* x = sc[r >> 1][q] + 2 * (r & 1);
+          const float2 z = unpair(add2(pair(x[0], x[1]), below[q]));
+          const Pair e = pair(ex2(z.x), ex2(z.y));
+          l[q] = add2(l[q], e);
+          float2 w = unpair(mul2(e, pair(step, step)));
+          if (WHOLE) {
+            vsum[q] = fma2(e, pair(mid, mid), vsum[q]);
+          } else {      // a masked place may hold NaN
+            const bool on0 = (seen[2 * q] >> r) & 1u, on1 = (seen[2 * q + 1] >> r) & 1u;
+            w.x = on0 ? w.x : 0.0f;
+            w.y = on1 ? w.y : 0.0f;
+            vsum[q] = fma2(e, pair(on0 ? mid : 0.0f, on1 ? mid : 0.0f), vsum[q]);
           }
-          wt[mt][q][0] = transpose8x8(pack2<false>(w[0], w[1]));
-          wt[mt][q][1] = transpose8x8(pack2<false>(w[2], w[3]));
+          wt[r >> 1][q][r & 1] = transpose8x8(pack2<false>(w.x, w.y));
         }
+      }
 #pragma unroll
       for (int mt = 0; mt < 2; mt++) {
         uint32_t vw[4][F::WV];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          const int row = mt * 16 + (k >> 1) * 8 + 2 * t + (k & 1);
-          const int byte = 4 * F::WV * g;
-          lds_words<F::WV>(at + F::V_AT + flow_offset<D>(row, byte >> 4) + (byte & 15), vw[k]);
+          lds_words<F::WV>(at + F::V_AT + (mt * 16 + (k >> 1) * 8) * F::ROW + (fv ^ (k & 1)) * F::ROW + 4 * F::WV * g, vw[k]);
         }
 #pragma unroll
         for (int q = 0; q < NQ; q++) mma_f16(ones[q], 0x00010001u, 0x00010001u, 0x00010001u, 0x00010001u, wt[mt][q][0], wt[mt][q][1]);
@@ -612,24 +648,27 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
       }
     };
 
-    for (int i = 0, stage = 0, fill = FLOW_STAGES - 1; i < nt; i++) {
-      cp_async_wait<FLOW_STAGES - 2>();
-      __syncwarp();
-      const long long next = rows_at(i + FLOW_STAGES);
+    for (int i = 0; i < nt && ok; i++) {
+      const uint8_t* next = source(i + FLOW_STAGES);
+      if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, phase))) {
+        // never seen.  Give up; the copies still on their way get one more bounded wait each.
+        ok = false;
+        if (lane == 0) atomicExch(p.status_flag, 1);
+        for (int k = 1; k < FLOW_STAGES - 1 && i + k < nt; k++) mbar_wait(bars + 8 * ((stage + k) % FLOW_STAGES), phase ^ (stage + k >= FLOW_STAGES ? 1u : 0u));
+        break;
+      }
       const int key = key0 + i * FLOW_TILE;
-      const uint32_t at = ring + stage * F::STAGE;
-      const uint32_t live = *reinterpret_cast<volatile uint32_t*>(my_smem + stage * F::STAGE + F::HEAD_AT);
       if (key < s.end && key + FLOW_KEYS > s.begin) {       // warp-uniform
+        const uint32_t at = ring + stage * F::STAGE, live = live_s[stage];
         if (live == 15u && key >= last_begin && key + FLOW_KEYS <= first_end) attend(std::true_type(), key, at, live);
         else attend(std::false_type(), key, at, live);
       }
       __syncwarp();
-      issue(i + FLOW_STAGES - 1, fill, ids);
-      ids = next;
+      issue(i + FLOW_STAGES - 1, src);
+      src = next;
       stage = stage + 1 == FLOW_STAGES ? 0 : stage + 1;
-      fill = fill + 1 == FLOW_STAGES ? 0 : fill + 1;
+      if (stage == 0) phase ^= 1u;
     }
-    cp_async_wait<0>();
     __syncwarp();
 
     // ---- the four warps' results meet in shared memory
@@ -640,10 +679,12 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
 #pragma unroll
       for (int c = 0; c < 2 * NQ; c++) {
         const int r = (c >> 1) * 8 + 2 * t + (c & 1);
+        const float2 l2 = unpair(l[c >> 1]), v2 = unpair(vsum[c >> 1]);
+        float lc = c & 1 ? l2.y : l2.x, vc = c & 1 ? v2.y : v2.x;
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) {
-          l[c] += __shfl_xor_sync(0xffffffffu, l[c], d);
-          vsum[c] += __shfl_xor_sync(0xffffffffu, vsum[c], d);
+          lc += __shfl_xor_sync(0xffffffffu, lc, d);
+          vc += __shfl_xor_sync(0xffffffffu, vc, d);
         }
         const float eight = 8.0f * ones[c >> 1][c & 1];
 #pragma unroll
@@ -651,11 +692,11 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             float2 v;      // elements 2 j and 2 j + 1 of the word; the second stands 16 times too high
-            v.x = fmaf((o[w][j][c >> 1][c & 1] - eight) * unit, lower, vsum[c]);
-            v.y = fmaf((o[w][j][c >> 1][(c & 1) + 2] * 0.0625f - eight) * unit, lower, vsum[c]);
+            v.x = fmaf((o[w][j][c >> 1][c & 1] - eight) * unit, lower, vc);
+            v.y = fmaf((o[w][j][c >> 1][(c & 1) + 2] * 0.0625f - eight) * unit, lower, vc);
             *reinterpret_cast<float2*>(mine + r * (D + 4) + 8 * (F::WV * g + w) + 2 * j) = v;
           }
-        if (g == 0) *reinterpret_cast<float2*>(mine + r * (D + 4) + D) = make_float2(m[c], l[c]);
+        if (g == 0) *reinterpret_cast<float2*>(mine + r * (D + 4) + D) = make_float2(m[c], lc);
       }
     }
     __syncthreads();
@@ -664,7 +705,7 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
     float* slot = complete ? nullptr : fp.slots + (2ll * blockIdx.x + (t0 == 0 ? 1 : 0)) * F::SLOT;
     if (threadIdx.x == 0 && fp.split && t0 == 0) {
       // the last unit of this (sequence, head) lies with the block whose share holds it
-      const long long last = (long long)u + s.tiles - 1;
+      const long long last = (long long)bh_unit + FLOW_SEGMENT + s.tiles - 1;
       fp.pieces[bh] = complete ? make_int2(0, 0) : make_int2((int)blockIdx.x, (int)(((last + 1) * sharing - 1) / total) - (int)blockIdx.x + 1);
     }
     for (int e = threadIdx.x; e < rows * (D / 4); e += 32 * FLOW_WARPS) {
@@ -697,14 +738,11 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
         if (d == 0) *reinterpret_cast<float2*>(slot + r * 2) = make_float2(M, L);
       }
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();     // the exchange area is the next segment's ring
-    if (fp.split) {
-      u += nt;
-      t0 = 0;
-      h++;
-    } else {
-      u += stride;
-    }
+    u = next_u;
+    loc = 0;
+    if (fp.split) h++;
   }
 }
 
@@ -796,7 +834,7 @@ FlowPlan flow_plan(const apnn_kv4_cache* c, const apnn_kv4_batch* b, int group) 
   const long long keys = (long long)b->table_width * c->page_size;
   const long long whole = (long long)b->sequences * c->heads;
   f.split = keys > UNSPLIT_KEYS;
-  const long long units = whole * ((keys + FLOW_TILE - 1) / FLOW_TILE);
+  const long long units = whole * ((keys + FLOW_TILE - 1) / FLOW_TILE + FLOW_SEGMENT);
   const long long most = (long long)device_sm_count() * per_sm;
   f.blocks = (int)(f.split ? (units < most ? units : most) : (whole < (1ll << 30) ? whole : 1ll << 30));
   f.join = (int)whole;
@@ -881,11 +919,12 @@ apnn_status apnn_kv4_attention(void* stream, const apnn_kv4_cache* cache, const 
   p.causal = a->causal;
   p.window = a->window;
   p.scale = a->scale;
+  p.status_flag = static_cast<int*>(workspace);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if ((long long)batch->max_q * p.group <= largest_rows(cache->head_dim)) {
     const FlowPlan f = flow_plan(cache, batch, p.group);
-    FlowParams fp = {p, reinterpret_cast<int2*>(static_cast<char*>(workspace) + f.pieces_at),
-                     reinterpret_cast<float*>(static_cast<char*>(workspace) + f.slots_at), f.split};
+    FlowParams fp = {p, reinterpret_cast<int2*>(static_cast<char*>(workspace) + f.pieces_at), reinterpret_cast<float*>(static_cast<char*>(workspace) + f.slots_at),
+                     f.split, p.cache.page_shift < 5 ? p.cache.page_shift : 5};
     apnn_status (*const launch[2][3])(cudaStream_t, const FlowPlan&, const FlowParams&) = {
         {launch_flow_rows<false, 64>, launch_flow_rows<false, 128>, launch_flow_rows<false, 256>},
         {launch_flow_rows<true, 64>, launch_flow_rows<true, 128>, launch_flow_rows<true, 256>}};
@@ -907,8 +946,12 @@ apnn_status apnn_kv4_attention(void* stream, const apnn_kv4_cache* cache, const 
 
 apnn_status apnn_kv4_attention_check(void* stream, const void* workspace) {
   if (!workspace) return APNN_ERR_INVALID_ARG;
-  const cudaError_t e = cudaStreamSynchronize(reinterpret_cast<cudaStream_t>(stream));
-  return e == cudaSuccess ? APNN_OK : cuda_fail(e, "apnn_kv4_attention_check");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  int flag = -1;
+  cudaError_t e = cudaMemcpyAsync(&flag, workspace, sizeof(int), cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e != cudaSuccess) return cuda_fail(e, "apnn_kv4_attention_check");
+  return flag == 0 ? APNN_OK : APNN_ERR_TIMEOUT;
 }
 
 }  // extern "C"
