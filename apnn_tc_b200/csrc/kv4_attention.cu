@@ -353,33 +353,38 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
     // the parameters of both, a lane each
     const int key0 = (s.tile0 + t0) * FLOW_TILE + warp * FLOW_KEYS;
     const int run = lane >> 2, part = lane & 3, run_keys = 1 << fp.run_shift;
-    const bool copies = run < (FLOW_KEYS >> fp.run_shift);
     const int unit_bytes = part < 2 ? F::ROW : 4;
     const uint8_t* part_base = p.cache.data + h * p.cache.head_bytes + (long long)p.cache.page_size * (part < 2 ? part * F::ROW : D + (part - 2) * 4);
     const uint32_t part_dst = ring + (part == 0 ? 0 : part == 1 ? F::V_AT : part == 2 ? F::KP_AT : F::VP_AT) + run * run_keys * unit_bytes;
     const int* trow = p.batch.table + (long long)b * p.batch.table_stride;
-    auto source = [&](int i) -> const uint8_t* {
-      const int key = key0 + i * FLOW_TILE + run * run_keys;
-      if (!copies || i >= nt || key >= s.end || key < 0) return nullptr;      // key < len <= table_width * page_size: within the table
-      const int id = __ldg(trow + (key >> p.cache.page_shift));
-      return id < 0 || id >= p.cache.pages ? nullptr : part_base + id * p.cache.page_stride + (long long)(key & (p.cache.page_size - 1)) * unit_bytes;
+    // the key this lane copies next, and where its copying ends (end <= table_width * page_size: within the table)
+    int at_key = key0 + run * run_keys;
+    const int stop = run < (FLOW_KEYS >> fp.run_shift) ? min(s.end, key0 + nt * FLOW_TILE) : 0;
+    const uint32_t all_live = 0xffffu >> (16 - 4 * (FLOW_KEYS >> fp.run_shift));
+    auto source = [&]() -> const uint8_t* {
+      const uint8_t* src = nullptr;
+      if (at_key < stop) {
+        const int id = __ldg(trow + (at_key >> p.cache.page_shift));
+        if ((uint32_t)id < (uint32_t)p.cache.pages) src = part_base + id * p.cache.page_stride + (at_key & (p.cache.page_size - 1)) * unit_bytes;
+      }
+      at_key += FLOW_TILE;
+      return src;
     };
     auto issue = [&](int i, const uint8_t* src) {
       if (i >= nt || !ok) return;
-      const bool group_live = __shfl_sync(0xffffffffu, src != nullptr, (((lane & 3) * 8) >> fp.run_shift) * 4);
-      const uint32_t live = __ballot_sync(0xffffffffu, group_live) & 15u;
+      const uint32_t live = __ballot_sync(0xffffffffu, src != nullptr);     // four bits for each run
       if (lane == 0) {
         live_s[fill] = live;
-        mbar_expect_tx(bars + 8 * fill, __popc(live) * 8 * (2 * F::ROW + 8));
+        mbar_expect_tx(bars + 8 * fill, __popc(live) * (run_keys * (2 * F::ROW + 8) / 4));
       }
       __syncwarp();
       if (src != nullptr) bulk_load(part_dst + fill * F::STAGE, src, run_keys * unit_bytes, bars + 8 * fill);
       fill = fill + 1 == FLOW_STAGES ? 0 : fill + 1;
     };
-    const uint8_t* src = source(0);
+    const uint8_t* src = source();
 #pragma unroll
     for (int i = 0; i < FLOW_STAGES - 1; i++) {
-      const uint8_t* next = source(i + 1);
+      const uint8_t* next = source();
       issue(i, src);
       src = next;
     }
@@ -460,7 +465,6 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
     const int first_end = p.causal ? min(s.len, s.pos0 + 1) : s.len;
 
     float o[F::WV][4][NQ][4], ones[NQ][4];
-    float m[2 * NQ];
     Pair l[NQ], vsum[NQ];
 #pragma unroll
     for (int q = 0; q < NQ; q++)
@@ -473,11 +477,23 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
           for (int j = 0; j < 4; j++) o[w][j][q][c] = 0.0f;
       }
 #pragma unroll
-    for (int c = 0; c < 2 * NQ; c++) m[c] = -INFINITY;
-#pragma unroll
     for (int q = 0; q < NQ; q++) l[q] = vsum[q] = pair(0.0f, 0.0f);
     const int fk = flow_key(g), fv = flow_key(2 * t);
-    int R = -112;     // 2^R is above every value step met so far, within fp32's range
+    // reference points, negated (0 where no key was met), and 8 above them; 2^R is above every value step met so far, within
+    // fp32's range; lift = 2^(6 - R)
+    Pair below[NQ];
+    float rise_at[2 * NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; q++) below[q] = pair(0.0f, 0.0f);
+#pragma unroll
+    for (int c = 0; c < 2 * NQ; c++) rise_at[c] = -INFINITY;
+    auto reference = [&](int c) {
+      const float2 f = unpair(below[c >> 1]);
+      return rise_at[c] == -INFINITY ? -INFINITY : c & 1 ? -f.y : -f.x;
+    };
+    int R = -112;
+    uint32_t step_bits = 0;     // the fp32 bits of 2^R, 0 before the first key: larger steps raise R
+    float lift = __uint_as_float((uint32_t)(127 + 6 + 112) << 23);
 
     auto attend = [&](auto tag, int key, uint32_t at, uint32_t live) {
       constexpr bool WHOLE = decltype(tag)::value;      // every row sees every key: no mask is looked at
@@ -539,13 +555,13 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
 #pragma unroll
           for (int k = 0; k < 4; k++) {
             const int j = key + k * 8 + fk;
-            if (j < end && j >= begin && ((live >> k) & 1u)) seen[c] |= 1u << k;
+            if (j < end && j >= begin && ((live >> (((k * 8) >> fp.run_shift) * 4)) & 1u)) seen[c] |= 1u << k;
           }
         }
       }
       float top[2 * NQ];
 #pragma unroll
-      for (int c = 0; c < 2 * NQ; c++) top[c] = m[c];
+      for (int c = 0; c < 2 * NQ; c++) top[c] = -INFINITY;
 #pragma unroll
       for (int r = 0; r < 4; r++)
 #pragma unroll
@@ -559,23 +575,27 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
         }
       // exponent of the largest value step of these keys (a step that is not finite shows in its weight instead)
       uint32_t bits = __float_as_uint(fabsf(unpack2<BF16>(lds32(at + F::VP_AT + lane * 4)).x));
-      if (bits >= 0x7f800000u || (!WHOLE && (key + lane >= s.end || key + lane < s.begin || !((live >> (lane >> 3)) & 1u)))) bits = 0;
-      const int rise = max(R, min((int)(__reduce_max_sync(0xffffffffu, bits) >> 23) - 126, 127));
+      if (bits >= 0x7f800000u || (!WHOLE && (key + lane >= s.end || key + lane < s.begin || !((live >> ((lane >> fp.run_shift) * 4)) & 1u)))) bits = 0;
       // The reference point m follows the running maximum only where that has risen by more than 2^8: weights then stay below
       // 2^8 of it, and most tiles after a segment's first neither exchange maxima nor touch the sums.
-      bool moved = rise != R;
+      bool moved = bits > step_bits;
 #pragma unroll
-      for (int c = 0; c < 2 * NQ; c++) moved |= top[c] > m[c] + 8.0f;      // m = -inf: any key at all
+      for (int c = 0; c < 2 * NQ; c++) moved |= top[c] > rise_at[c];
       if (__any_sync(0xffffffffu, moved)) {
+        const int rise = max(R, min((int)(__reduce_max_sync(0xffffffffu, bits) >> 23) - 126, 127));
         const float shrink = __uint_as_float((uint32_t)max(127 + R - rise, 0) << 23);      // 2^(R - rise)
         R = rise;
+        step_bits = (uint32_t)(127 + R) << 23;
+        lift = __uint_as_float((uint32_t)(127 + 6 - R) << 23);
         float kept[2 * NQ];
 #pragma unroll
         for (int c = 0; c < 2 * NQ; c++) {
 #pragma unroll
           for (int d = 4; d < 32; d *= 2) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], d));
-          const float keep = m[c] == top[c] ? 1.0f : ex2(m[c] - top[c]);       // -inf - x: 0
-          m[c] = top[c];
+          const float m = reference(c);
+          top[c] = fmaxf(top[c], m);
+          const float keep = m == top[c] ? 1.0f : ex2(m - top[c]);       // -inf - x: 0
+          rise_at[c] = top[c] + 8.0f;
           const float k = keep * shrink;
           kept[c] = keep;
 #pragma unroll
@@ -591,14 +611,10 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
         for (int q = 0; q < NQ; q++) {
           l[q] = mul2(l[q], pair(kept[2 * q], kept[2 * q + 1]));
           vsum[q] = mul2(vsum[q], pair(kept[2 * q], kept[2 * q + 1]));
+          below[q] = pair(top[2 * q] == -INFINITY ? 0.0f : -top[2 * q], top[2 * q + 1] == -INFINITY ? 0.0f : -top[2 * q + 1]);
         }
       }
       // ---- weights, and their products with the values
-      const float lift = __uint_as_float((uint32_t)(127 + 6 - R) << 23);     // 2^(6 - R)
-      Pair below[NQ];     // minus the reference points
-#pragma unroll
-      for (int q = 0; q < NQ; q++)
-        below[q] = pair(m[2 * q] == -INFINITY ? 0.0f : -m[2 * q], m[2 * q + 1] == -INFINITY ? 0.0f : -m[2 * q + 1]);
       uint32_t wt[2][NQ][2];
 #pragma unroll
       for (int r = 0; r < 4; r++) {
@@ -649,7 +665,7 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
     };
 
     for (int i = 0; i < nt && ok; i++) {
-      const uint8_t* next = source(i + FLOW_STAGES);
+      const uint8_t* next = source();
       if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, phase))) {
         // never seen.  Give up; the copies still on their way get one more bounded wait each.
         ok = false;
@@ -660,7 +676,7 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
       const int key = key0 + i * FLOW_TILE;
       if (key < s.end && key + FLOW_KEYS > s.begin) {       // warp-uniform
         const uint32_t at = ring + stage * F::STAGE, live = live_s[stage];
-        if (live == 15u && key >= last_begin && key + FLOW_KEYS <= first_end) attend(std::true_type(), key, at, live);
+        if (live == all_live && key >= last_begin && key + FLOW_KEYS <= first_end) attend(std::true_type(), key, at, live);
         else attend(std::false_type(), key, at, live);
       }
       __syncwarp();
@@ -696,7 +712,7 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
             v.y = fmaf((o[w][j][c >> 1][(c & 1) + 2] * 0.0625f - eight) * unit, lower, vc);
             *reinterpret_cast<float2*>(mine + r * (D + 4) + 8 * (F::WV * g + w) + 2 * j) = v;
           }
-        if (g == 0) *reinterpret_cast<float2*>(mine + r * (D + 4) + D) = make_float2(m[c], lc);
+        if (g == 0) *reinterpret_cast<float2*>(mine + r * (D + 4) + D) = make_float2(reference(c), lc);
       }
     }
     __syncthreads();
