@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libapnn_b200.so")
@@ -100,6 +101,17 @@ class Kv4AttentionArgs(_Sized):
     _fields_ = [("struct_size", ctypes.c_uint32), ("rows", ctypes.c_int32), ("q", ctypes.c_void_p), ("out", ctypes.c_void_p),
                 ("lse", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64), ("q_heads", ctypes.c_int32),
                 ("causal", ctypes.c_int32), ("window", ctypes.c_int32), ("scale", ctypes.c_float)]
+
+
+_FORMATS = {ctypes.c_uint32: "I", ctypes.c_int32: "i", ctypes.c_int64: "q", ctypes.c_void_p: "P", ctypes.c_float: "f", ctypes.c_double: "d"}
+
+
+def packer(descriptor):
+    """A function that packs a descriptor's fields (all but ``struct_size``, null pointers as 0) into bytes of its layout."""
+    layout = struct.Struct("@" + "".join(_FORMATS[t] for _, t in descriptor._fields_) + "0q")
+    assert layout.size == ctypes.sizeof(descriptor), descriptor
+    pack, size = layout.pack, layout.size
+    return lambda *fields: pack(size, *fields)
 
 
 class ApnnError(RuntimeError):

@@ -12,7 +12,6 @@ the tensors' device; nothing here computes on the CPU, and nothing synchronises 
 from __future__ import annotations
 
 import ctypes
-import math
 from typing import Optional, Tuple
 
 import torch
@@ -20,28 +19,30 @@ import torch
 from . import _cabi
 
 _TYPES = {torch.bfloat16: _cabi.TYPE_BF16, torch.float16: _cabi.TYPE_FP16, torch.float32: _cabi.TYPE_FP32}
+_INPUTS = {torch.bfloat16: _cabi.TYPE_BF16, torch.float16: _cabi.TYPE_FP16}
+
+# The call's descriptor is packed in one go (a few hundred nanoseconds; a ctypes structure filled field by field takes several
+# microseconds, as long as a small call takes on the device).
+_LINEAR, _APPEND, _ATTENTION = (_cabi.packer(t) for t in (_cabi.LinearDesc, _cabi.Kv4AppendArgs, _cabi.Kv4AttentionArgs))
+_get_device, _get_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-def _launch(device: torch.device, what: str, call) -> None:
-    """``call(stream)`` with ``device`` current, on its current stream."""
-    index = device.index
-    if index == torch.cuda.current_device():
-        status = call(torch._C._cuda_getCurrentRawStream(index))
+def _launch(index: int, what: str, fn, *args) -> None:
+    """``fn(stream, *args)`` with device ``index`` current, on its current stream."""
+    if index == _get_device():
+        status = fn(_get_stream(index), *args)
     else:
         with torch.cuda.device(index):
-            status = call(torch._C._cuda_getCurrentRawStream(index))
+            status = fn(_get_stream(index), *args)
     if status:
         _cabi.check(status, what)
 
 
-def _same_device(device: torch.device, **tensors: Optional[torch.Tensor]) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, the call runs on {device}")
-
-
-def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
+def _on(index: int, name: str, t: torch.Tensor) -> int:
+    """The address of a tensor that has to lie on device ``index``."""
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, the call runs on cuda:{index}")
+    return t.data_ptr()
 
 
 # ------------------------------------------------------------------------------------------------------------ product
@@ -62,50 +63,64 @@ def linear_planes(x: torch.Tensor, planes: torch.Tensor, scale: torch.Tensor, *,
         raise ValueError("x must be [M, K] and planes [wbits, N, K/32]")
     M, K = x.shape
     wbits, N, words = planes.shape
-    if x.dtype not in (torch.bfloat16, torch.float16):
+    x_dtype = x.dtype
+    x_type = _INPUTS.get(x_dtype)
+    if x_type is None:
         raise ValueError("x must be bfloat16 or float16")
     if planes.dtype not in (torch.int32, torch.uint32) or not planes.is_contiguous():
         raise ValueError("planes must be contiguous 32-bit words (torch.int32)")
     if words != (K + 127) // 128 * 4:
         raise ValueError(f"planes hold rows of {words} words, K = {K} needs {(K + 127) // 128 * 4}")
-    if activation not in _cabi.ACTIVATIONS:
+    act = _cabi.ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of {sorted(_cabi.ACTIVATIONS)}")
-    for name, t in (("scale", scale), ("bias", bias)):
-        if t is not None and (t.dtype != torch.float32 or t.shape != (N,) or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous float32 [{N}]")
-    device = x.device
-    _same_device(device, planes=planes, scale=scale, bias=bias, residual=residual, out=out, status_flag=status_flag)
-    if out is None:
-        out = torch.empty((M, N), dtype=out_dtype or x.dtype, device=device)
-    elif out_dtype is not None and out.dtype != out_dtype:
+    index = x.get_device()
+    scale_ptr = _vector(index, "scale", scale, N)
+    bias_ptr = None if bias is None else _vector(index, "bias", bias, N)
+    made = out is None
+    if made:
+        out = x.new_empty((M, N)) if out_dtype is None or out_dtype is x_dtype else x.new_empty((M, N), dtype=out_dtype)
+    elif out_dtype is not None and out.dtype is not out_dtype:
         raise ValueError("out and out_dtype disagree")
-    if out.dtype not in (x.dtype, torch.float32):
+    out_dtype = out.dtype
+    if out_dtype is not x_dtype and out_dtype is not torch.float32:
         raise ValueError("out must be of x's type or float32")
-    for name, t in (("out", out), ("residual", residual)):
-        if t is not None and (t.shape != (M, N) or t.dtype != out.dtype or (t.stride(1) != 1 and N > 1)):
-            raise ValueError(f"{name} must be [{M}, {N}] of {out.dtype} with unit element stride")
-    if x.stride(1) != 1 and K > 1:
+    # a single row may carry any stride: it is never stepped over
+    ldx, step = x.stride()
+    if step != 1 and K > 1:
         raise ValueError("x must have unit element stride")
-    if status_flag is not None and (status_flag.dtype != torch.int32 or status_flag.numel() < 1):
-        raise ValueError("status_flag must be int32")
+    ldx = ldx if M > 1 else (K + 7) // 8 * 8
+    ldo = N if made else _matrix("out", out, M, N, out_dtype)
+    residual_ptr, ldr = (None, 0) if residual is None else (_on(index, "residual", residual), _matrix("residual", residual, M, N, out_dtype))
+    flag_ptr = None
+    if status_flag is not None:
+        if status_flag.dtype != torch.int32 or status_flag.numel() < 1:
+            raise ValueError("status_flag must be int32")
+        flag_ptr = _on(index, "status_flag", status_flag)
     if M == 0:
         if status_flag is not None:
             status_flag.zero_()
         return out
-    d = _cabi.LinearDesc()
-    d.x_type, d.out_type, d.activation = _TYPES[x.dtype], _TYPES[out.dtype], _cabi.ACTIVATIONS[activation]
-    d.zero = zero
-    d.scale = scale.data_ptr()
-    if bias is not None:
-        d.bias = bias.data_ptr()
-    # a single row may carry any stride: it is never stepped over
-    d.ldx, d.ldo = (x.stride(0), out.stride(0)) if M > 1 else ((K + 7) // 8 * 8, N)
-    if residual is not None:
-        d.residual, d.ldr = residual.data_ptr(), residual.stride(0) if M > 1 else N
-    lib = _cabi.lib()
-    _launch(device, "apnn_linear_planes", lambda stream: lib.apnn_linear_planes(
-        stream, wbits, planes.data_ptr(), x.data_ptr(), out.data_ptr(), M, N, K, ctypes.addressof(d), _ptr(status_flag)))
+    desc = _LINEAR(x_type, _TYPES[out_dtype], act, zero, scale_ptr, bias_ptr or 0, residual_ptr or 0, ldx, ldo, ldr)
+    _launch(index, "apnn_linear_planes", _cabi.lib().apnn_linear_planes, wbits, _on(index, "planes", planes), x.data_ptr(),
+            _on(index, "out", out), M, N, K, desc, flag_ptr)
     return out
+
+
+def _vector(index: int, name: str, t: torch.Tensor, n: int) -> int:
+    if t.dtype is not torch.float32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 [{n}]")
+    return _on(index, name, t)
+
+
+def _matrix(name: str, t: torch.Tensor, M: int, N: int, dtype: torch.dtype) -> int:
+    """Checks [M, N] with unit element stride; returns the row stride."""
+    if t.dtype is not dtype or tuple(t.shape) != (M, N):
+        raise ValueError(f"{name} must be [{M}, {N}] of {dtype}")
+    rows, step = t.stride()
+    if step != 1 and N > 1:
+        raise ValueError(f"{name} must have unit element stride")
+    return rows if M > 1 else N
 
 
 # ------------------------------------------------------------------------------------------------------------ cache
@@ -137,8 +152,10 @@ class KVCache4:
         self.data, self.dtype = data, dtype
         self.pages, self.heads, self.page_size, self.head_dim = pages, heads, page_size, head_dim
         stride = data.stride(0) * 4 if pages > 1 else heads * words * 4
+        self._index = data.get_device()
         self._c = _cabi.Kv4Cache(type=_TYPES[dtype], data=data.data_ptr(), page_stride=stride, pages=pages, heads=heads,
                                  page_size=page_size, head_dim=head_dim)
+        self._ptr = ctypes.addressof(self._c)
 
     @property
     def device(self) -> torch.device:
@@ -167,18 +184,30 @@ class KVBatch:
         if max_q < 1:
             raise ValueError("max_q must be positive")
         self.cu_q, self.kv_len, self.table, self.max_q = cu_q, kv_len, table, int(max_q)
+        self._index = cu_q.get_device()
         self._c = _cabi.Kv4Batch(sequences=B, cu_q=cu_q.data_ptr(), kv_len=kv_len.data_ptr(), table=table.data_ptr(),
                                  table_stride=table.stride(0) if B > 1 else table.shape[1], table_width=table.shape[1], max_q=int(max_q))
+        self._ptr = ctypes.addressof(self._c)
 
 
-def _rows(name: str, t: torch.Tensor, heads: Optional[int], cache: KVCache4) -> int:
-    """Checks [rows, heads, D] of the cache's type with dense heads; returns the row stride in elements."""
+def _rows(name: str, t: torch.Tensor, cache: KVCache4) -> Tuple[int, int, int]:
+    """Checks [rows, heads, D] of the cache's type with dense heads; returns rows, heads and the row stride in elements."""
     D = cache.head_dim
-    if t.dtype != cache.dtype or t.dim() != 3 or t.shape[2] != D or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be [rows, {heads if heads is not None else 'heads'}, {D}] of {cache.dtype}")
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != D):
+    if t.dtype is not cache.dtype or t.dim() != 3:
+        raise ValueError(f"{name} must be [rows, heads, {D}] of {cache.dtype}")
+    rows, heads, d = t.shape
+    row, head, step = t.stride()
+    if d != D:
+        raise ValueError(f"{name} must be [rows, heads, {D}] of {cache.dtype}")
+    if step != 1 or (head != D and heads > 1):
         raise ValueError(f"the heads of a row of {name} must be dense")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * D
+    return rows, heads, row if rows > 1 else heads * D
+
+
+def _same(cache: KVCache4, batch: KVBatch) -> int:
+    if batch._index != cache._index:
+        raise ValueError(f"the batch is on cuda:{batch._index}, the cache on cuda:{cache._index}")
+    return cache._index
 
 
 def kv4_append(cache: KVCache4, batch: KVBatch, k: torch.Tensor, v: torch.Tensor, *, q: Optional[torch.Tensor] = None,
@@ -189,39 +218,43 @@ def kv4_append(cache: KVCache4, batch: KVBatch, k: torch.Tensor, v: torch.Tensor
     k, v: [rows, heads, D]; q: [rows, q_heads, D] or None; views of one fused projection are taken as they are.  q_norm,
     k_norm: [D] weights in the cache's type.  rotary: float32 [positions, rotary_dim], rotary_dim/2 cosines and as many sines.
     """
-    device = cache.device
-    _same_device(device, k=k, v=v, q=q, q_out=q_out, q_norm=q_norm, k_norm=k_norm, rotary=rotary, batch=batch.cu_q)
-    a = _cabi.Kv4AppendArgs()
-    a.k_stride, a.v_stride = _rows("k", k, cache.heads, cache), _rows("v", v, cache.heads, cache)
-    a.rows = k.shape[0]
-    if v.shape[0] != k.shape[0] or (q is not None and q.shape[0] != k.shape[0]):
-        raise ValueError("q, k and v disagree on the rows")
+    index = _same(cache, batch)
+    rows, heads, k_stride = _rows("k", k, cache)
+    v_rows, v_heads, v_stride = _rows("v", v, cache)
+    if heads != cache.heads or v_heads != heads:
+        raise ValueError(f"k and v must have the cache's {cache.heads} heads")
+    q_ptr = q_out_ptr = q_stride = q_out_stride = q_heads = q_rows = 0
     if q is not None:
-        a.q_stride, a.q_heads = _rows("q", q, None, cache), q.shape[1]
+        q_rows, q_heads, q_stride = _rows("q", q, cache)
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        a.q_out_stride = _rows("q_out", q_out, q.shape[1], cache)
-        if q_out.shape != q.shape:
-            raise ValueError("q_out must have q's shape")
-        a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
+            q_out, q_out_stride = q.new_empty((q_rows, q_heads, cache.head_dim)), q_heads * cache.head_dim
+        else:
+            out_rows, out_heads, q_out_stride = _rows("q_out", q_out, cache)
+            if out_rows != q_rows or out_heads != q_heads:
+                raise ValueError("q_out must have q's shape")
+        q_ptr, q_out_ptr = _on(index, "q", q), _on(index, "q_out", q_out)
     elif q_out is not None or q_norm is not None:
         raise ValueError("q_out and q_norm need q")
-    a.k, a.v = k.data_ptr(), v.data_ptr()
+    if v_rows != rows or (q is not None and q_rows != rows):
+        raise ValueError("q, k and v disagree on the rows")
+    norms = []
     for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if t is not None:
-            if t.dtype != cache.dtype or t.shape != (cache.head_dim,) or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous [{cache.head_dim}] of {cache.dtype}")
-            setattr(a, name, t.data_ptr())
-    a.eps = eps
+        if t is None:
+            norms.append(0)
+            continue
+        if t.dtype is not cache.dtype or t.dim() != 1 or t.numel() != cache.head_dim or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous [{cache.head_dim}] of {cache.dtype}")
+        norms.append(_on(index, name, t))
+    rotary_ptr = rotary_rows = rotary_dim = 0
     if rotary is not None:
-        if rotary.dtype != torch.float32 or rotary.dim() != 2 or not rotary.is_contiguous() or rotary.numel() == 0:
+        if rotary.dtype is not torch.float32 or rotary.dim() != 2 or not rotary.is_contiguous() or rotary.numel() == 0:
             raise ValueError("rotary must be a contiguous float32 [positions, rotary_dim]")
-        a.rotary, a.rotary_rows, a.rotary_dim = rotary.data_ptr(), rotary.shape[0], rotary.shape[1]
-        a.interleaved = 1 if interleaved else 0
-    if a.rows > 0:
-        lib = _cabi.lib()
-        _launch(device, "apnn_kv4_append", lambda stream: lib.apnn_kv4_append(
-            stream, ctypes.addressof(cache._c), ctypes.addressof(batch._c), ctypes.addressof(a)))
+        rotary_rows, rotary_dim = rotary.shape
+        rotary_ptr = _on(index, "rotary", rotary)
+    if rows > 0:
+        args = _APPEND(rows, _on(index, "k", k), _on(index, "v", v), k_stride, v_stride, q_ptr, q_out_ptr, q_stride, q_out_stride,
+                       q_heads, rotary_dim, norms[0], norms[1], eps, 1 if interleaved and rotary is not None else 0, rotary_ptr, rotary_rows)
+        _launch(index, "apnn_kv4_append", _cabi.lib().apnn_kv4_append, cache._ptr, batch._ptr, args)
     return q_out
 
 
@@ -237,26 +270,25 @@ def kv4_read(cache: KVCache4, batch: KVBatch, rows: Optional[int] = None, *, k_o
         if given is None:
             raise ValueError("kv4_read needs rows, k_out or v_out")
         rows = given.shape[0]
+    index = _same(cache, batch)
     shape = (rows, cache.heads, cache.head_dim)
-    outs = []
     for name, t in (("k_out", k_out), ("v_out", v_out)):
-        if t is None:
-            t = torch.empty(shape, dtype=cache.dtype, device=cache.device)
-        elif t.shape != shape or t.dtype != cache.dtype or not t.is_contiguous():
+        if t is not None and (t.dtype is not cache.dtype or tuple(t.shape) != shape or not t.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous [{rows}, {cache.heads}, {cache.head_dim}] of {cache.dtype}")
-        outs.append(t)
-    _same_device(cache.device, k_out=outs[0], v_out=outs[1], batch=batch.cu_q)
+    if k_out is None:
+        k_out = cache.data.new_empty(shape, dtype=cache.dtype)
+    if v_out is None:
+        v_out = torch.empty_like(k_out)
     if rows > 0:
-        lib = _cabi.lib()
-        _launch(cache.device, "apnn_kv4_read", lambda stream: lib.apnn_kv4_read(
-            stream, ctypes.addressof(cache._c), ctypes.addressof(batch._c), outs[0].data_ptr(), outs[1].data_ptr(), rows))
-    return outs[0], outs[1]
+        _launch(index, "apnn_kv4_read", _cabi.lib().apnn_kv4_read, cache._ptr, batch._ptr, _on(index, "k_out", k_out),
+                _on(index, "v_out", v_out), rows)
+    return k_out, v_out
 
 
 # ------------------------------------------------------------------------------------------------------------ attention
 def kv4_attention_workspace_bytes(cache: KVCache4, batch: KVBatch, q_heads: int) -> int:
     """Device memory that ``kv4_attention`` needs for batches of these bounds (sequences, table width, max_q)."""
-    return int(_cabi.lib().apnn_kv4_attention_workspace_bytes(ctypes.addressof(cache._c), ctypes.addressof(batch._c), q_heads))
+    return int(_cabi.lib().apnn_kv4_attention_workspace_bytes(cache._ptr, batch._ptr, q_heads))
 
 
 def kv4_attention(cache: KVCache4, batch: KVBatch, q: torch.Tensor, *, scale: Optional[float] = None, causal: bool = True,
@@ -267,40 +299,36 @@ def kv4_attention(cache: KVCache4, batch: KVBatch, q: torch.Tensor, *, scale: Op
     positions back a row sees, itself included (0: all); needs causal.  lse: True, or a float32 [rows, q_heads] to write.
     workspace: ``kv4_attention_workspace_bytes`` bytes (uint8), used by one call at a time; allocated here if None.
     """
-    device = cache.device
-    a = _cabi.Kv4AttentionArgs()
-    a.q_stride = _rows("q", q, None, cache)
-    rows, q_heads, D = q.shape
+    index = _same(cache, batch)
+    rows, q_heads, q_stride = _rows("q", q, cache)
     if out is None:
-        out = torch.empty((rows, q_heads, D), dtype=q.dtype, device=device)
-    a.out_stride = _rows("out", out, q_heads, cache)
-    if out.shape != q.shape:
-        raise ValueError("out must have q's shape")
+        out_stride = q_heads * cache.head_dim
+        out = torch.empty_like(q) if q_stride == out_stride else q.new_empty((rows, q_heads, cache.head_dim))
+    else:
+        out_rows, out_heads, out_stride = _rows("out", out, cache)
+        if out_rows != rows or out_heads != q_heads:
+            raise ValueError("out must have q's shape")
     with_lse = lse is not False and lse is not None
-    if lse is True:
-        lse = torch.empty((rows, q_heads), dtype=torch.float32, device=device)
-    if with_lse and (lse.dtype != torch.float32 or lse.shape != (rows, q_heads) or not lse.is_contiguous()):
-        raise ValueError(f"lse must be a contiguous float32 [{rows}, {q_heads}]")
+    lse_ptr = 0
+    if with_lse:
+        if lse is True:
+            lse = torch.empty((rows, q_heads), dtype=torch.float32, device=q.device)
+        if lse.dtype is not torch.float32 or tuple(lse.shape) != (rows, q_heads) or not lse.is_contiguous():
+            raise ValueError(f"lse must be a contiguous float32 [{rows}, {q_heads}]")
+        lse_ptr = _on(index, "lse", lse)
     if window and not causal:
         raise ValueError("a window needs causal")
+    q_ptr = _on(index, "q", q)
     if workspace is None:
-        workspace = torch.empty(max(1, kv4_attention_workspace_bytes(cache, batch, q_heads)), dtype=torch.uint8, device=device)
-    _same_device(device, q=q, out=out, lse=lse if with_lse else None, workspace=workspace, batch=batch.cu_q)
-    a.rows, a.q_heads = rows, q_heads
-    a.q, a.out = q.data_ptr(), out.data_ptr()
-    if with_lse:
-        a.lse = lse.data_ptr()
-    a.causal, a.window = (1 if causal else 0), window
-    a.scale = 1.0 / math.sqrt(D) if scale is None else scale
+        workspace = torch.empty(max(1, kv4_attention_workspace_bytes(cache, batch, q_heads)), dtype=torch.uint8, device=q.device)
     if rows > 0:
-        lib = _cabi.lib()
-        size = workspace.numel() * workspace.element_size()
-        _launch(device, "apnn_kv4_attention", lambda stream: lib.apnn_kv4_attention(
-            stream, ctypes.addressof(cache._c), ctypes.addressof(batch._c), ctypes.addressof(a), workspace.data_ptr(), size))
+        args = _ATTENTION(rows, q_ptr, _on(index, "out", out), lse_ptr, q_stride, out_stride, q_heads, 1 if causal else 0, window,
+                          cache.head_dim ** -0.5 if scale is None else scale)
+        _launch(index, "apnn_kv4_attention", _cabi.lib().apnn_kv4_attention, cache._ptr, batch._ptr, args,
+                _on(index, "workspace", workspace), workspace.numel() * workspace.element_size())
     return (out, lse) if with_lse else out
 
 
 def kv4_attention_check(workspace: torch.Tensor) -> None:
     """Synchronise and raise if the attention that last used ``workspace`` gave up on a wait."""
-    lib = _cabi.lib()
-    _launch(workspace.device, "apnn_kv4_attention_check", lambda stream: lib.apnn_kv4_attention_check(stream, workspace.data_ptr()))
+    _launch(workspace.get_device(), "apnn_kv4_attention_check", _cabi.lib().apnn_kv4_attention_check, workspace.data_ptr())
