@@ -3,6 +3,7 @@
 #include <cmath>
 
 #include "kv4.cuh"
+#include "spread.cuh"
 #include "tc5_common.cuh"
 
 namespace apnn {
@@ -21,6 +22,7 @@ struct LinearParams {
   int M, N, K, kwords, wbits, act, out_f32;
   float zero;
   int* status_flag;
+  int split;       // few rows: blocks of a cluster, which share K
 };
 
 __device__ __forceinline__ float activate(float v, int act) {
@@ -56,6 +58,204 @@ __global__ void __launch_bounds__(256) linear_rows_kernel(const LinearParams p) 
   if (p.residual) v += p.out_f32 ? static_cast<const float*>(p.residual)[m * p.ldr + n] : unpack2<BF16>(static_cast<const uint16_t*>(p.residual)[m * p.ldr + n]).x;
   if (p.out_f32) static_cast<float*>(p.out)[m * p.ldo + n] = v;
   else static_cast<uint16_t*>(p.out)[m * p.ldo + n] = (uint16_t)pack2<BF16>(v, 0.0f);
+}
+
+// The epilogue of one output element.
+template <bool BF16>
+__device__ __forceinline__ void store_element(const LinearParams& p, long long m, long long n, float sum, float scale, float bias) {
+  float v = activate(fmaf(sum, scale, bias), p.act);
+  if (p.out_f32) {
+    if (p.residual) v += static_cast<const float*>(p.residual)[m * p.ldr + n];
+    static_cast<float*>(p.out)[m * p.ldo + n] = v;
+  } else {
+    if (p.residual) v += unpack2<BF16>(static_cast<const uint16_t*>(p.residual)[m * p.ldr + n]).x;
+    static_cast<uint16_t*>(p.out)[m * p.ldo + n] = (uint16_t)pack2<BF16>(v, 0.0f);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- few rows
+// At most 16 rows of X: the weights are read once and bound it, so nothing of them goes through shared memory.  A warp takes 16
+// weight rows, the M operand of mma.sync m16n8k16; the rows of X are its N.  A lane (g, t) reads 16 bytes of each plane of rows
+// g and g + 8, 128 elements of K, the four lanes of a row 64 contiguous bytes, a 512-element block ahead.  Which elements of K
+// meet in one instruction is free as long as both operands agree, so the fields of a word are taken as they lie, bits b and
+// b + 16 side by side: elements 31 - b and 15 - b.  The block pairs its part of X the same way in shared memory, once for its
+// eight warps.  K is split over the blocks of a cluster where the weight rows alone are too few warps for the device, and where
+// X would not fit; their sums meet in distributed shared memory, added in the order of the ranks.
+constexpr int FEW_WARPS = 8;
+constexpr int FEW_TILE = 16 * FEW_WARPS;      // weight rows of a block
+constexpr int FEW_ROWS = 16;                  // rows of X
+constexpr int FEW_SPLIT = 8;                  // largest cluster
+constexpr int FEW_X_BYTES = 96 * 1024;        // two blocks to an SM
+
+template <bool BF16>
+__device__ __forceinline__ void mma_16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 load_stream(const uint32_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int j) { return j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w; }
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Where the pairs 4 c .. 4 c + 3 of word j (of the four that lane t takes of a block) of row m of X lie: 16-byte pieces,
+// exchanged so that the lanes of two rows read different banks.
+__device__ __forceinline__ int few_x_at(int m, int blocks, int kb, int j, int t, int c) {
+  return (((m * blocks + kb) * 4 + j) * 4 + t) * 4 + (c ^ t ^ (m & 1));
+}
+
+template <int WB, bool BF16, int NT>
+__global__ void __launch_bounds__(32 * FEW_WARPS, 2) linear_few_rows_kernel(const LinearParams p) {
+  using F = Fields<WB>;
+  extern __shared__ __align__(16) uint4 x_s[];
+  __shared__ float part_s[FEW_TILE][8 * NT + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int rank = blockIdx.x % p.split;
+  const long long n0 = (long long)(blockIdx.x / p.split) * FEW_TILE;
+  // this block's 512-element blocks of K
+  const int all = (p.kwords + 15) / 16, kb0 = all * rank / p.split, blocks = all * (rank + 1) / p.split - kb0;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  if (p.status_flag && blockIdx.x == 0 && threadIdx.x == 0) *p.status_flag = 0;
+  const ZeroPoint<BF16> zero(p.zero);
+  float acc[NT][4];
+#pragma unroll
+  for (int i = 0; i < NT; i++)
+#pragma unroll
+    for (int c = 0; c < 4; c++) acc[i][c] = 0.0f;
+
+  // this lane's chunk of the planes for block kb; zeros beyond the edges
+  auto load_weights = [&](int kb, uint4 (&w)[2][WB]) {
+    const int word = (kb0 + kb) * 16 + t * 4;
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+      const long long n = n0 + warp * 16 + r * 8 + g;
+      const bool live = kb < blocks && n < p.N && word < p.kwords;
+#pragma unroll
+      for (int b = 0; b < WB; b++) w[r][b] = live ? load_stream(p.W + b * p.plane_words + n * p.kwords + word) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  uint4 w[2][WB], next[2][WB];
+  load_weights(0, w);
+
+  // X, 32 elements to a thread: pair b of a word is elements 31 - b (low half) and 15 - b; zeros behind the row's end
+  for (int e = threadIdx.x; e < p.M * blocks * 16; e += 32 * FEW_WARPS) {
+    const int m = e / (blocks * 16), word = e - m * (blocks * 16), kb = word >> 4, tt = (word >> 2) & 3, j = word & 3;
+    const int k0 = (kb0 * 16 + word) * 32;
+    const uint16_t* src = p.X + m * p.ldx + k0;
+    uint32_t x[16];
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      const int left = p.K - k0 - c * 8;
+      if (left >= 8) {
+        v = __ldg(reinterpret_cast<const uint4*>(src + c * 8));
+      } else if (left > 0) {
+        uint32_t q[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) q[i] = i < left ? src[c * 8 + i] : 0;
+        v = make_uint4(q[0] | q[1] << 16, q[2] | q[3] << 16, q[4] | q[5] << 16, q[6] | q[7] << 16);
+      }
+      x[c * 4] = v.x;
+      x[c * 4 + 1] = v.y;
+      x[c * 4 + 2] = v.z;
+      x[c * 4 + 3] = v.w;
+    }
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      uint32_t y[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int b = c * 4 + i;
+        y[i] = __byte_perm(x[(31 - b) >> 1], x[(15 - b) >> 1], b & 1 ? 0x5410 : 0x7632);
+      }
+      x_s[few_x_at(m, blocks, kb, j, tt, c)] = make_uint4(y[0], y[1], y[2], y[3]);
+    }
+  }
+  __syncthreads();
+
+  for (int kb = 0; kb < blocks; kb++) {
+    load_weights(kb + 1, next);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      uint32_t f0[F::WORDS], f1[F::WORDS], p0[WB], p1[WB];
+#pragma unroll
+      for (int b = 0; b < WB; b++) {
+        p0[b] = word_of(w[0][b], j);
+        p1[b] = word_of(w[1][b], j);
+      }
+      gather_fields<WB>(p0, f0);
+      gather_fields<WB>(p1, f1);
+      uint32_t y[NT][16];
+#pragma unroll
+      for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          const int m = i * 8 + g;
+          const uint4 v = m < p.M ? x_s[few_x_at(m, blocks, kb, j, t, c)] : make_uint4(0u, 0u, 0u, 0u);
+          y[i][4 * c] = v.x;
+          y[i][4 * c + 1] = v.y;
+          y[i][4 * c + 2] = v.z;
+          y[i][4 * c + 3] = v.w;
+        }
+#pragma unroll
+      for (int q = 0; q < F::WORDS; q++)
+#pragma unroll
+        for (int f = 0; f < F::PER_HALF; f += 2) {
+          const int b0 = F::WIDTH * f + q, b1 = F::WIDTH * (f + 1) + q;
+          const uint32_t a0 = level_pair<F::WIDTH, BF16>(f0[q], f, zero), a1 = level_pair<F::WIDTH, BF16>(f1[q], f, zero);
+          const uint32_t a2 = level_pair<F::WIDTH, BF16>(f0[q], f + 1, zero), a3 = level_pair<F::WIDTH, BF16>(f1[q], f + 1, zero);
+#pragma unroll
+          for (int i = 0; i < NT; i++) mma_16<BF16>(acc[i], a0, a1, a2, a3, y[i][b0], y[i][b1]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; r++)
+#pragma unroll
+      for (int b = 0; b < WB; b++) w[r][b] = next[r][b];
+  }
+#pragma unroll
+  for (int i = 0; i < NT; i++)
+#pragma unroll
+    for (int c = 0; c < 4; c++) part_s[warp * 16 + g + (c >> 1) * 8][i * 8 + 2 * t + (c & 1)] = acc[i][c];
+  const int rows = FEW_TILE / p.split;      // of the block's, finished by this rank
+  if (p.split > 1) cluster_sync_all();
+  else __syncthreads();
+  const uint32_t mine = smem_u32(&part_s[0][0]);
+  for (int e = threadIdx.x; e < rows * p.M; e += 32 * FEW_WARPS) {
+    const int row = rank * rows + e % rows, m = e / rows;
+    const long long n = n0 + row;
+    if (n >= p.N) continue;
+    float sum = 0.0f;
+    if (p.split > 1) {
+      for (int k = 0; k < p.split; k++) sum += ld_cluster(map_to_cta(mine + (row * (8 * NT + 1) + m) * 4, k));
+    } else {
+      sum = part_s[row][m];
+    }
+    store_element<BF16>(p, m, n, sum, __ldg(p.scale + n), p.bias ? __ldg(p.bias + n) : 0.0f);
+  }
+  if (p.split > 1) cluster_sync_all();      // no rank leaves while another reads its sums
+}
+
+template <bool BF16, int NT>
+void (*few_rows_kernel(int wbits))(LinearParams) {
+  return wbits == 1 ? linear_few_rows_kernel<1, BF16, NT> : wbits == 2 ? linear_few_rows_kernel<2, BF16, NT> : wbits == 3 ? linear_few_rows_kernel<3, BF16, NT> : linear_few_rows_kernel<4, BF16, NT>;
 }
 
 }  // namespace
@@ -99,6 +299,37 @@ extern "C" apnn_status apnn_linear_planes(void* stream, int wbits, const void* W
   p.zero = d->zero;
   p.status_flag = status_flag;
   cudaLaunchConfig_t cfg = {};
+  if (M <= FEW_ROWS) {
+    // Split until there are two blocks for every SM, at least 512 elements of K to a block; then until X fits.
+    const int tiles = (N + FEW_TILE - 1) / FEW_TILE, blocks = (p.kwords + 15) / 16;
+    int split = 1;
+    auto x_bytes = [&](int s) { return (long long)M * ((blocks + s - 1) / s) * 1024; };
+    while (split < FEW_SPLIT && 2 * split <= blocks && ((long long)tiles * split < 2 * device_sm_count() || x_bytes(split) > FEW_X_BYTES)) split *= 2;
+    if (x_bytes(split) <= FEW_X_BYTES) {
+      p.split = split;
+      const bool bf16 = d->x_type == APNN_TYPE_BF16;
+      void (*const kernel)(LinearParams) = M <= 8 ? (bf16 ? few_rows_kernel<true, 1>(wbits) : few_rows_kernel<false, 1>(wbits))
+                                                  : (bf16 ? few_rows_kernel<true, 2>(wbits) : few_rows_kernel<false, 2>(wbits));
+      cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(kernel), FEW_X_BYTES);
+      if (e != cudaSuccess) return cuda_fail(e, "linear_few_rows_kernel shared memory");
+      cfg.gridDim = dim3((unsigned)(tiles * split), 1, 1);
+      cfg.blockDim = dim3(32 * FEW_WARPS, 1, 1);
+      cfg.dynamicSmemBytes = (size_t)x_bytes(split);
+      cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+      cudaLaunchAttribute attr[2];
+      cfg.numAttrs = pdl_attribute(attr);
+      if (split > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = (unsigned)split;
+        attr[cfg.numAttrs].val.clusterDim.y = 1;
+        attr[cfg.numAttrs].val.clusterDim.z = 1;
+        cfg.numAttrs++;
+      }
+      cfg.attrs = attr;
+      e = cudaLaunchKernelEx(&cfg, kernel, p);
+      return e == cudaSuccess ? APNN_OK : cuda_fail(e, "linear_few_rows_kernel");
+    }
+  }
   cfg.gridDim = dim3((unsigned)((N + 7) / 8), (unsigned)M, 1);
   cfg.blockDim = dim3(256, 1, 1);
   cfg.stream = reinterpret_cast<cudaStream_t>(stream);
