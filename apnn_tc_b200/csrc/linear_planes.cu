@@ -119,10 +119,20 @@ __device__ __forceinline__ int few_x_at(int m, int blocks, int kb, int j, int t,
   return (((m * blocks + kb) * 4 + j) * 4 + t) * 4 + (c ^ t ^ (m & 1));
 }
 
+// four elements of X of which `left` lie before the row's end
+__device__ __forceinline__ uint2 few_x_load(const uint16_t* src, int left) {
+  if (left >= 4) return __ldg(reinterpret_cast<const uint2*>(src));
+  uint2 v = make_uint2(0u, 0u);
+  if (left > 0) v.x = src[0];
+  if (left > 1) v.x |= (uint32_t)src[1] << 16;
+  if (left > 2) v.y = src[2];
+  return v;
+}
+
 template <int WB, bool BF16, int NT>
 __global__ void __launch_bounds__(32 * FEW_WARPS, 2) linear_few_rows_kernel(const LinearParams p) {
   using F = Fields<WB>;
-  extern __shared__ __align__(16) uint4 x_s[];
+  extern __shared__ __align__(64) uint4 x_s[];
   __shared__ float part_s[FEW_TILE][8 * NT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
@@ -140,58 +150,56 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) linear_few_rows_kernel(cons
 #pragma unroll
     for (int c = 0; c < 4; c++) acc[i][c] = 0.0f;
 
-  // this lane's chunk of the planes for block kb; zeros beyond the edges
+  // This lane's chunk of the planes for block kb.  Beyond the edges it reads what is there: sums of rows behind N are not
+  // stored, and X is zero behind K.
+  const uint32_t* base[2];
+#pragma unroll
+  for (int r = 0; r < 2; r++) base[r] = p.W + min(n0 + warp * 16 + r * 8 + g, (long long)p.N - 1) * p.kwords;
   auto load_weights = [&](int kb, uint4 (&w)[2][WB]) {
-    const int word = (kb0 + kb) * 16 + t * 4;
+    const int word = min((kb0 + min(kb, blocks - 1)) * 16 + t * 4, p.kwords - 4);
 #pragma unroll
-    for (int r = 0; r < 2; r++) {
-      const long long n = n0 + warp * 16 + r * 8 + g;
-      const bool live = kb < blocks && n < p.N && word < p.kwords;
+    for (int r = 0; r < 2; r++)
 #pragma unroll
-      for (int b = 0; b < WB; b++) w[r][b] = live ? load_stream(p.W + b * p.plane_words + n * p.kwords + word) : make_uint4(0u, 0u, 0u, 0u);
-    }
+      for (int b = 0; b < WB; b++) w[r][b] = load_stream(base[r] + b * p.plane_words + word);
   };
-  uint4 w[2][WB], next[2][WB];
-  load_weights(0, w);
+  uint4 w0[2][WB], w1[2][WB];
+  load_weights(0, w0);
 
-  // X, 32 elements to a thread: pair b of a word is elements 31 - b (low half) and 15 - b; zeros behind the row's end
-  for (int e = threadIdx.x; e < p.M * blocks * 16; e += 32 * FEW_WARPS) {
-    const int m = e / (blocks * 16), word = e - m * (blocks * 16), kb = word >> 4, tt = (word >> 2) & 3, j = word & 3;
-    const int k0 = (kb0 * 16 + word) * 32;
-    const uint16_t* src = p.X + m * p.ldx + k0;
-    uint32_t x[16];
-#pragma unroll
-    for (int c = 0; c < 4; c++) {
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      const int left = p.K - k0 - c * 8;
-      if (left >= 8) {
-        v = __ldg(reinterpret_cast<const uint4*>(src + c * 8));
-      } else if (left > 0) {
-        uint32_t q[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) q[i] = i < left ? src[c * 8 + i] : 0;
-        v = make_uint4(q[0] | q[1] << 16, q[2] | q[3] << 16, q[4] | q[5] << 16, q[6] | q[7] << 16);
-      }
-      x[c * 4] = v.x;
-      x[c * 4 + 1] = v.y;
-      x[c * 4 + 2] = v.z;
-      x[c * 4 + 3] = v.w;
-    }
-#pragma unroll
-    for (int c = 0; c < 4; c++) {
-      uint32_t y[4];
+  // X in pieces of four pairs (pair b of a word is elements 31 - b, low half, and 15 - b), zeros behind the row's end; four
+  // pieces of a thread in flight at a time
+  {
+    const int per_row = blocks * 64, total = p.M * per_row;
+    int m = 0, at = threadIdx.x;       // row and piece within it
+    for (int u = threadIdx.x; u < total; u += 4 * 32 * FEW_WARPS) {
+      uint2 hi[4], lo[4];
+      int where[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const int b = c * 4 + i;
-        y[i] = __byte_perm(x[(31 - b) >> 1], x[(15 - b) >> 1], b & 1 ? 0x5410 : 0x7632);
+        while (at >= per_row) {
+          at -= per_row;
+          m++;
+        }
+        const int word = at >> 2, c = at & 3, k0 = (kb0 * 16 + word) * 32 + 12 - 4 * c;      // elements k0 .. + 3 and k0 + 16 .. + 19
+        where[i] = m < p.M ? few_x_at(m, blocks, word >> 4, word & 3, (word >> 2) & 3, c) : -1;
+        const uint16_t* src = p.X + m * p.ldx + k0;
+        lo[i] = where[i] >= 0 ? few_x_load(src, p.K - k0) : make_uint2(0u, 0u);
+        hi[i] = where[i] >= 0 ? few_x_load(src + 16, p.K - k0 - 16) : make_uint2(0u, 0u);
+        at += 32 * FEW_WARPS;
       }
-      x_s[few_x_at(m, blocks, kb, j, tt, c)] = make_uint4(y[0], y[1], y[2], y[3]);
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (where[i] >= 0)
+          x_s[where[i]] = make_uint4(__byte_perm(hi[i].y, lo[i].y, 0x7632), __byte_perm(hi[i].y, lo[i].y, 0x5410), __byte_perm(hi[i].x, lo[i].x, 0x7632),
+                                     __byte_perm(hi[i].x, lo[i].x, 0x5410));
     }
   }
   __syncthreads();
 
-  for (int kb = 0; kb < blocks; kb++) {
-    load_weights(kb + 1, next);
+  // lanes behind the last row of X repeat it: their columns are not stored
+  const uint4* x_row[NT];
+#pragma unroll
+  for (int i = 0; i < NT; i++) x_row[i] = x_s + few_x_at(min(i * 8 + g, p.M - 1), blocks, 0, 0, t, 0);
+  auto contract = [&](int kb, const uint4 (&w)[2][WB]) {
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       uint32_t f0[F::WORDS], f1[F::WORDS], p0[WB], p1[WB];
@@ -207,8 +215,8 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) linear_few_rows_kernel(cons
       for (int i = 0; i < NT; i++)
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-          const int m = i * 8 + g;
-          const uint4 v = m < p.M ? x_s[few_x_at(m, blocks, kb, j, t, c)] : make_uint4(0u, 0u, 0u, 0u);
+          // x_row stands at piece t ^ (m & 1) of its group of four; piece c lies c exchanged bits from there
+          const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(x_row[i] + (kb * 4 + j) * 16) ^ (uintptr_t)(c * 16));
           y[i][4 * c] = v.x;
           y[i][4 * c + 1] = v.y;
           y[i][4 * c + 2] = v.z;
@@ -225,10 +233,23 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) linear_few_rows_kernel(cons
           for (int i = 0; i < NT; i++) mma_16<BF16>(acc[i], a0, a1, a2, a3, y[i][b0], y[i][b1]);
         }
     }
+  };
+  if (NT == 2 && WB > 2) {     // no registers for a second set: the next block waits in L2
+    for (int kb = 0; kb < blocks; kb++) {
+      if (kb > 0) load_weights(kb, w0);
+      const int word = min((kb0 + min(kb + 1, blocks - 1)) * 16 + t * 4, p.kwords - 4);
 #pragma unroll
-    for (int r = 0; r < 2; r++)
+      for (int r = 0; r < 2; r++)
 #pragma unroll
-      for (int b = 0; b < WB; b++) w[r][b] = next[r][b];
+        for (int b = 0; b < WB; b++) asm volatile("prefetch.global.L2 [%0];" ::"l"(base[r] + b * p.plane_words + word));
+      contract(kb, w0);
+    }
+  } else for (int kb = 0; kb < blocks; kb += 2) {
+    load_weights(kb + 1, w1);
+    contract(kb, w0);
+    if (kb + 1 == blocks) break;
+    load_weights(kb + 2, w0);
+    contract(kb + 1, w1);
   }
 #pragma unroll
   for (int i = 0; i < NT; i++)
@@ -300,11 +321,19 @@ extern "C" apnn_status apnn_linear_planes(void* stream, int wbits, const void* W
   p.status_flag = status_flag;
   cudaLaunchConfig_t cfg = {};
   if (M <= FEW_ROWS) {
-    // Split until there are two blocks for every SM, at least 512 elements of K to a block; then until X fits.
-    const int tiles = (N + FEW_TILE - 1) / FEW_TILE, blocks = (p.kwords + 15) / 16;
-    int split = 1;
+    // The split whose waves (two blocks to an SM) of 512-element steps are fewest; beginning and ending a block counts as two
+    // steps.  A split is taken as soon as X fits.
+    const int tiles = (N + FEW_TILE - 1) / FEW_TILE, blocks = (p.kwords + 15) / 16, slots = 2 * device_sm_count();
     auto x_bytes = [&](int s) { return (long long)M * ((blocks + s - 1) / s) * 1024; };
-    while (split < FEW_SPLIT && 2 * split <= blocks && ((long long)tiles * split < 2 * device_sm_count() || x_bytes(split) > FEW_X_BYTES)) split *= 2;
+    int split = 1;
+    long long best = -1;
+    for (int s = 1; s <= FEW_SPLIT && s <= blocks; s *= 2) {
+      const long long steps = ((long long)tiles * s + slots - 1) / slots * ((blocks + s - 1) / s + 2);
+      if (x_bytes(s) <= FEW_X_BYTES && (best < 0 || steps < best)) {
+        best = steps;
+        split = s;
+      }
+    }
     if (x_bytes(split) <= FEW_X_BYTES) {
       p.split = split;
       const bool bf16 = d->x_type == APNN_TYPE_BF16;

@@ -14,6 +14,18 @@
 
 namespace apnn {
 
+// (a & b) | c and (a & b) | (c & ~b), one instruction each whatever the compiler makes of the constants
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t select_bits(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xE2;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+
 template <int WB>
 struct Fields {
   static constexpr int WORDS = WB == 1 ? 1 : WB == 2 ? 2 : 4;       // three planes count as four
@@ -27,7 +39,7 @@ __device__ __forceinline__ void gather_fields(const uint32_t (&p)[WB], uint32_t 
   if constexpr (WB == 1) {
     f[0] = p[0];
   } else {
-    const uint32_t a0 = (p[0] & 0x55555555u) | ((p[1] << 1) & 0xaaaaaaaau), a1 = ((p[0] >> 1) & 0x55555555u) | (p[1] & 0xaaaaaaaau);
+    const uint32_t a0 = select_bits(p[0], 0x55555555u, p[1] << 1), a1 = select_bits(p[0] >> 1, 0x55555555u, p[1]);
     if constexpr (WB == 2) {
       f[0] = a0;
       f[1] = a1;
@@ -37,13 +49,13 @@ __device__ __forceinline__ void gather_fields(const uint32_t (&p)[WB], uint32_t 
         c0 = p[2] & 0x55555555u;
         c1 = (p[2] >> 1) & 0x55555555u;
       } else {
-        c0 = (p[2] & 0x55555555u) | ((p[3] << 1) & 0xaaaaaaaau);
-        c1 = ((p[2] >> 1) & 0x55555555u) | (p[3] & 0xaaaaaaaau);
+        c0 = select_bits(p[2], 0x55555555u, p[3] << 1);
+        c1 = select_bits(p[2] >> 1, 0x55555555u, p[3]);
       }
-      f[0] = (a0 & 0x33333333u) | ((c0 << 2) & 0xccccccccu);
-      f[1] = (a1 & 0x33333333u) | ((c1 << 2) & 0xccccccccu);
-      f[2] = ((a0 >> 2) & 0x33333333u) | (c0 & 0xccccccccu);
-      f[3] = ((a1 >> 2) & 0x33333333u) | (c1 & 0xccccccccu);
+      f[0] = select_bits(a0, 0x33333333u, c0 << 2);
+      f[1] = select_bits(a1, 0x33333333u, c1 << 2);
+      f[2] = select_bits(a0 >> 2, 0x33333333u, c0);
+      f[3] = select_bits(a1 >> 2, 0x33333333u, c1);
     }
   }
 }
@@ -92,7 +104,7 @@ __device__ __forceinline__ uint32_t level_pair(uint32_t w, int j, const ZeroPoin
   const int shift = field_shift<WIDTH, BF16>(j), pos = WIDTH * j - shift;
   const uint32_t mask = (((1u << WIDTH) - 1u) << pos) * 0x00010001u;
   const uint32_t exponent = (uint32_t)(((BF16 ? 127 : 15) + MANTISSA - pos) << MANTISSA) * 0x00010001u;
-  const uint32_t v = add16x2<BF16>(((w >> shift) & mask) | exponent, z.at[pos]);
+  const uint32_t v = add16x2<BF16>(and_or(w >> shift, mask, exponent), z.at[pos]);
   return pos == 0 ? add16x2<BF16>(v, z.none) : v;
 }
 
