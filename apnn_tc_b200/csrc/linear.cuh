@@ -1,0 +1,49 @@
+// The product over weight planes: parameters, activations and the store that its kernels share.
+#pragma once
+#include "kv4.cuh"
+#include "spread.cuh"
+#include "tc5_common.cuh"
+
+namespace apnn {
+
+struct LinearParams {
+  const uint32_t* W;
+  const uint16_t* X;
+  void* out;
+  const float* scale;
+  const float* bias;
+  const void* residual;
+  long long ldx, ldo, ldr, plane_words;
+  int M, N, K, kwords, wbits, act, out_f32;
+  float zero;
+  int* status_flag;
+  int split;       // few rows: blocks of a cluster, which share K
+};
+
+__device__ __forceinline__ float activate(float v, int act) {
+  switch (act) {
+    case APNN_ACT_RELU: return v > 0.0f ? v : (v == v ? 0.0f : v);
+    case APNN_ACT_SILU: return v / (1.0f + expf(-v));
+    case APNN_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678f));
+    case APNN_ACT_GELU_TANH: return 0.5f * v * (1.0f + tanhf(0.79788456f * (v + 0.044715f * v * v * v)));
+    default: return v;
+  }
+}
+
+// The epilogue of one output element.
+template <bool BF16>
+__device__ __forceinline__ void store_element(const LinearParams& p, long long m, long long n, float sum, float scale, float bias) {
+  float v = activate(fmaf(sum, scale, bias), p.act);
+  if (p.out_f32) {
+    if (p.residual) v += static_cast<const float*>(p.residual)[m * p.ldr + n];
+    static_cast<float*>(p.out)[m * p.ldo + n] = v;
+  } else {
+    if (p.residual) v += unpack2<BF16>(static_cast<const uint16_t*>(p.residual)[m * p.ldr + n]).x;
+    static_cast<uint16_t*>(p.out)[m * p.ldo + n] = (uint16_t)pack2<BF16>(v, 0.0f);
+  }
+}
+
+// More than a few rows (linear_tile.cu).
+apnn_status linear_tile(cudaStream_t s, const LinearParams& p, bool bf16);
+
+}  // namespace apnn

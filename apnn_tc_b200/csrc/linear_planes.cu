@@ -2,76 +2,13 @@
 // epilogue.
 #include <cmath>
 
-#include "kv4.cuh"
-#include "spread.cuh"
+#include "linear.cuh"
 #include "tc5_common.cuh"
 
 namespace apnn {
 namespace {
 
 using namespace tc5;
-
-struct LinearParams {
-  const uint32_t* W;
-  const uint16_t* X;
-  void* out;
-  const float* scale;
-  const float* bias;
-  const void* residual;
-  long long ldx, ldo, ldr, plane_words;
-  int M, N, K, kwords, wbits, act, out_f32;
-  float zero;
-  int* status_flag;
-  int split;       // few rows: blocks of a cluster, which share K
-};
-
-__device__ __forceinline__ float activate(float v, int act) {
-  switch (act) {
-    case APNN_ACT_RELU: return v > 0.0f ? v : (v == v ? 0.0f : v);
-    case APNN_ACT_SILU: return v / (1.0f + expf(-v));
-    case APNN_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678f));
-    case APNN_ACT_GELU_TANH: return 0.5f * v * (1.0f + tanhf(0.79788456f * (v + 0.044715f * v * v * v)));
-    default: return v;
-  }
-}
-
-// One warp per output element.
-template <bool BF16>
-__global__ void __launch_bounds__(256) linear_rows_kernel(const LinearParams p) {
-  const int lane = threadIdx.x & 31;
-  const long long n = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int m = blockIdx.y;
-  grid_dependency_wait();
-  if (p.status_flag && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.status_flag = 0;
-  if (n >= p.N) return;
-  float sum = 0.0f;
-  for (int w = 0; w < p.kwords; w++) {
-    const int k = w * 32 + lane;
-    uint32_t level = 0;
-    for (int b = 0; b < p.wbits; b++) level |= ((__ldg(p.W + b * p.plane_words + n * p.kwords + w) >> (31 - lane)) & 1u) << b;
-    if (k < p.K) sum += unpack2<BF16>(p.X[m * p.ldx + k]).x * ((float)level - p.zero);
-  }
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  if (lane != 0) return;
-  float v = activate(fmaf(sum, __ldg(p.scale + n), p.bias ? __ldg(p.bias + n) : 0.0f), p.act);
-  if (p.residual) v += p.out_f32 ? static_cast<const float*>(p.residual)[m * p.ldr + n] : unpack2<BF16>(static_cast<const uint16_t*>(p.residual)[m * p.ldr + n]).x;
-  if (p.out_f32) static_cast<float*>(p.out)[m * p.ldo + n] = v;
-  else static_cast<uint16_t*>(p.out)[m * p.ldo + n] = (uint16_t)pack2<BF16>(v, 0.0f);
-}
-
-// The epilogue of one output element.
-template <bool BF16>
-__device__ __forceinline__ void store_element(const LinearParams& p, long long m, long long n, float sum, float scale, float bias) {
-  float v = activate(fmaf(sum, scale, bias), p.act);
-  if (p.out_f32) {
-    if (p.residual) v += static_cast<const float*>(p.residual)[m * p.ldr + n];
-    static_cast<float*>(p.out)[m * p.ldo + n] = v;
-  } else {
-    if (p.residual) v += unpack2<BF16>(static_cast<const uint16_t*>(p.residual)[m * p.ldr + n]).x;
-    static_cast<uint16_t*>(p.out)[m * p.ldo + n] = (uint16_t)pack2<BF16>(v, 0.0f);
-  }
-}
 
 // ---------------------------------------------------------------------------------------------- few rows
 // At most 16 rows of X: the weights are read once and bound it, so nothing of them goes through shared memory.  A warp takes 16
@@ -319,8 +256,8 @@ extern "C" apnn_status apnn_linear_planes(void* stream, int wbits, const void* W
   p.out_f32 = d->out_type == APNN_TYPE_FP32;
   p.zero = d->zero;
   p.status_flag = status_flag;
-  cudaLaunchConfig_t cfg = {};
   if (M <= FEW_ROWS) {
+    cudaLaunchConfig_t cfg = {};
     // The split whose waves (two blocks to an SM) of 512-element steps are fewest; beginning and ending a block counts as two
     // steps.  A split is taken as soon as X fits.
     const int tiles = (N + FEW_TILE - 1) / FEW_TILE, blocks = (p.kwords + 15) / 16, slots = 2 * device_sm_count();
@@ -359,12 +296,5 @@ extern "C" apnn_status apnn_linear_planes(void* stream, int wbits, const void* W
       return e == cudaSuccess ? APNN_OK : cuda_fail(e, "linear_few_rows_kernel");
     }
   }
-  cfg.gridDim = dim3((unsigned)((N + 7) / 8), (unsigned)M, 1);
-  cfg.blockDim = dim3(256, 1, 1);
-  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  cfg.numAttrs = pdl_attribute(attr);
-  cfg.attrs = attr;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, d->x_type == APNN_TYPE_BF16 ? linear_rows_kernel<true> : linear_rows_kernel<false>, p);
-  return e == cudaSuccess ? APNN_OK : cuda_fail(e, "linear_rows_kernel");
+  return linear_tile(reinterpret_cast<cudaStream_t>(stream), p, d->x_type == APNN_TYPE_BF16);
 }

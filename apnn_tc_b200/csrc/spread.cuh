@@ -97,15 +97,49 @@ __device__ __forceinline__ uint32_t add16x2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Field j of both halves of w (WIDTH * j bits up) as level - zero.
-template <int WIDTH, bool BF16>
+// Field j of both halves of w (STRIDE * j bits up, BITS wide) as level - zero.
+template <int STRIDE, bool BF16, int BITS = STRIDE>
 __device__ __forceinline__ uint32_t level_pair(uint32_t w, int j, const ZeroPoint<BF16>& z) {
   constexpr int MANTISSA = BF16 ? 7 : 10;
-  const int shift = field_shift<WIDTH, BF16>(j), pos = WIDTH * j - shift;
-  const uint32_t mask = (((1u << WIDTH) - 1u) << pos) * 0x00010001u;
+  const int shift = field_shift<STRIDE, BF16>(j), pos = STRIDE * j - shift;
+  const uint32_t mask = (((1u << BITS) - 1u) << pos) * 0x00010001u;
   const uint32_t exponent = (uint32_t)(((BF16 ? 127 : 15) + MANTISSA - pos) << MANTISSA) * 0x00010001u;
   const uint32_t v = add16x2<BF16>(and_or(w >> shift, mask, exponent), z.at[pos]);
   return pos == 0 ? add16x2<BF16>(v, z.none) : v;
+}
+
+// The 32 elements of a word of each plane as 16 pairs in order, pair j = elements 2 j (low half) and 2 j + 1.
+template <int WB, bool BF16>
+__device__ __forceinline__ void spread_in_order(const uint32_t (&p)[WB], const ZeroPoint<BF16>& z, uint32_t (&out)[16]) {
+  if constexpr (WB <= 2) {
+    uint32_t even, odd;      // field i: elements 30 - 2 i, 31 - 2 i
+    if constexpr (WB == 1) {
+      even = p[0] >> 1;
+      odd = p[0];
+    } else {
+      uint32_t f[2];
+      gather_fields<2>(p, f);
+      even = f[1];
+      odd = f[0];
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const uint32_t x = __byte_perm(even, odd, h ? 0x7632 : 0x5410);
+#pragma unroll
+      for (int i = 0; i < 8; i++) out[15 - 8 * h - i] = level_pair<2, BF16, WB>(x, i, z);
+    }
+  } else {
+    uint32_t f[4];           // field i of f[q]: element 31 - 4 i - q
+    gather_fields<WB>(p, f);
+#pragma unroll
+    for (int q = 0; q < 4; q += 2)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const uint32_t x = __byte_perm(f[q + 1], f[q], h ? 0x7632 : 0x5410);
+#pragma unroll
+        for (int i = 0; i < 4; i++) out[15 - q / 2 - 2 * (4 * h + i)] = level_pair<4, BF16>(x, i, z);
+      }
+  }
 }
 
 }  // namespace apnn

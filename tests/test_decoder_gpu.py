@@ -46,7 +46,8 @@ def close(got, want, off, dtype):
 @pytest.mark.parametrize("wbits", [1, 2, 3, 4])
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("M,N,K", [(1, 64, 128), (1, 1, 1), (3, 33, 200), (8, 256, 1024), (9, 40, 136), (17, 129, 392), (33, 65, 256),
-                                   (64, 128, 2048), (65, 300, 520), (130, 257, 776), (257, 513, 129), (300, 1000, 1000)])
+                                   (64, 128, 2048), (65, 300, 520), (130, 257, 776), (257, 513, 129), (300, 1000, 1000), (40, 64, 8),
+                                   (20, 4096, 1), (513, 2300, 264), (48, 130, 4096), (700, 6000, 640)])
 def test_product(cuda_device, M, N, K, wbits, dtype):
     product(M + N + K, M, N, K, wbits, dtype)
 
