@@ -2,11 +2,12 @@
 //
 // The weights are the M operand of tcgen05.mma kind::f16 (128 of them to a block, 256 to a pair of blocks with cta_group::2), rows of X
 // the N operand (tiles of 32 to 256), so a thread of the epilogue owns one weight row: its scale and bias stay in registers and a warp
-// stores 32 neighbouring columns of one row of the output.  X comes by TMA (128-byte swizzle, zeros beyond its edges).  The
-// weights never exist as 16-bit floats in memory: eight warps read the planes, spread them to level - zero (spread.cuh) and write
-// the swizzled operand tile themselves, two groups of four warps on alternate stages of 64 elements of K; a warp that loads nothing
-// meets each group on a named barrier and publishes the stage (a release at cluster scope waits for every load its warp has in
-// flight).  Roles: warp 0 TMA, 1 MMA, 2-5 epilogue, 6-13 spread, 14 publish; every wait is bounded.
+// stores 32 neighbouring columns of one row of the output.  X comes by TMA (128-byte swizzle, zeros beyond its edges), and so do the
+// planes, 512 elements of K of every row at a time into a ring of two (loads of 8 bytes from 128 rows took as many L1
+// cycles as a stage's MMAs: 0.74 against 0.43 ms at 4096 x 16384 x 4096, 4 bits).  The weights never exist as 16-bit floats in
+// memory: eight warps spread the planes to level - zero (spread.cuh) and write the swizzled operand tile themselves, two groups
+// of four warps on alternate pairs of stages of 64 elements of K; a warp that loads nothing meets each group on a named barrier and
+// publishes the stage.  Roles: warp 0 TMA, 1 MMA, 2-5 epilogue, 6-13 spread, 14 publish; every wait is bounded.
 //
 // What bounds a stage of 64 elements: shared memory, 32 KiB in and out for the weight tile and 256 bytes for each row of X a block
 // holds, at 128 bytes a clock -- 512 clk for the pair's 256 x 256 tile, as long as its MMAs.  Spreading takes about 250.
@@ -23,11 +24,14 @@ namespace {
 using namespace tc5;
 
 constexpr int ROWS = 128;                       // weight rows of a block
-constexpr int STAGES = 6;
-constexpr int A_BYTES = ROWS * BK, STAGE_BYTES = 2 * A_BYTES;
+constexpr int MAX_STAGES = 8;
+constexpr int A_BYTES = ROWS * BK;
+constexpr int CHUNK = 8;                        // stages of 64 elements that one load of the planes covers
+constexpr int PLANE_BYTES = ROWS * CHUNK * 8;   // of one plane
+constexpr int CHUNKS = 2;
 constexpr int SPREAD_WARPS = 8, GROUP_THREADS = 128;
 constexpr int THREADS = 32 * (6 + SPREAD_WARPS + 1);
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 1024;
+constexpr int SMEM_BYTES = 232448;              // all an SM has: alignment, barriers, planes, stages
 constexpr int MAX_SPLIT = 8;
 
 struct TileParams {
@@ -36,6 +40,7 @@ struct TileParams {
   int tiles_x, tiles_w;
   int kblocks;              // of 64 elements: even
   int split;                // blocks of a cluster that share K (1: none)
+  int stages, stage_bytes;
   uint32_t idesc;
 };
 
@@ -142,17 +147,23 @@ __device__ __forceinline__ void finish_columns(const LinearParams& p, float (&v)
   }
 }
 
+// The named barrier on which the group of pair `pairs` hands over its first or second stage.  Four in turn for each group: it comes
+// back to one only after the ring has let it reuse a slot, so after the publishing warp left it.
+__device__ __forceinline__ int group_barrier(uint32_t pairs, int second) { return 1 + (int)((pairs & 1u) * 4 + ((pairs >> 1) & 1u) * 2) + second; }
+
 template <int WB, bool BF16, int CTAS>
-__global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_constant__ CUtensorMap map_x, const TileParams p) {
+__global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const TileParams p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
-  const uint32_t bars = base + STAGES * STAGE_BYTES;
+  const uint32_t planes_at = base, stages_at = base + CHUNKS * WB * PLANE_BYTES, bars = stages_at + p.stages * p.stage_bytes;
   auto full_bar = [&](int s) { return bars + 8u * s; };                   // X landed and the weights are spread (in the leader)
-  auto empty_bar = [&](int s) { return bars + 8u * (STAGES + s); };
-  auto tfull_bar = [&](int a) { return bars + 8u * (2 * STAGES + a); };
-  auto tempty_bar = [&](int a) { return bars + 8u * (2 * STAGES + 2 + a); };
-  const uint32_t tmem_slot = bars + 8u * (2 * STAGES + 4);
+  auto empty_bar = [&](int s) { return bars + 8u * (MAX_STAGES + s); };
+  auto tfull_bar = [&](int a) { return bars + 8u * (2 * MAX_STAGES + a); };
+  auto tempty_bar = [&](int a) { return bars + 8u * (2 * MAX_STAGES + 2 + a); };
+  auto wfull_bar = [&](int c) { return bars + 8u * (2 * MAX_STAGES + 4 + c); };       // planes landed
+  auto wempty_bar = [&](int c) { return bars + 8u * (2 * MAX_STAGES + 6 + c); };      // and were read by all spreading warps
+  const uint32_t tmem_slot = bars + 8u * (2 * MAX_STAGES + 8);
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CTAS == 2 || p.split > 1 ? cluster_ctarank() : 0;
@@ -166,13 +177,15 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
   const int kbn = CTAS == 1 ? 2 * (int)((long long)kpairs * (rank + 1) / p.split) - kb0 : p.kblocks;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; s++) {
+    for (int s = 0; s < p.stages; s++) {
       mbar_init(full_bar(s), 1 + CTAS);   // the leader's TMA warp, the publishing warp of each block
       mbar_init(empty_bar(s), 1);
     }
     for (int a = 0; a < 2; a++) {
       mbar_init(tfull_bar(a), 1);
       mbar_init(tempty_bar(a), 4 * CTAS);
+      mbar_init(wfull_bar(a), 1);
+      mbar_init(wempty_bar(a), SPREAD_WARPS);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -203,11 +216,22 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
       uint32_t ph = 0;
       bool ok = true;
       const int rows = p.tn / CTAS;
+      uint32_t chunk = 0;       // over all tiles
       for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
         const int row = tile % p.tiles_x * p.tn + (int)half * rows;
-        for (int kb = 0; kb < kbn; kb++, s = (s + 1 == STAGES) ? 0 : s + 1, ph ^= (s == 0) ? 1u : 0u) {
+        const int wrow = (tile / p.tiles_x * CTAS + (int)half) * ROWS;
+        for (int kb = 0; kb < kbn; kb++, s = (s + 1 == p.stages) ? 0 : s + 1, ph ^= (s == 0) ? 1u : 0u) {
+          if (kb % CHUNK == 0) {
+            const uint32_t c = chunk % CHUNKS;
+            if (!mbar_wait(wempty_bar(c), ((chunk / CHUNKS) & 1u) ^ 1u)) { ok = false; break; }
+            mbar_expect_tx(wfull_bar(c), WB * PLANE_BYTES);
+            // rows behind N run into the next plane, and behind the last one they are zeros: their sums are not stored
+            for (int b = 0; b < WB; b++)
+              tma_load_2d(planes_at + (c * WB + b) * PLANE_BYTES, &map_w, 2 * (kb0 + kb), b * p.l.N + wrow, wfull_bar(c));
+            chunk++;
+          }
           if (!mbar_wait(empty_bar(s), ph ^ 1u)) { ok = false; break; }
-          const uint32_t dst = base + s * STAGE_BYTES + A_BYTES;
+          const uint32_t dst = stages_at + s * p.stage_bytes + A_BYTES;
           if (CTAS == 2) {
             if (rank == 0) mbar_expect_tx(full_bar(s), p.tn * BK);     // both blocks' bytes
             tma_load_2d_pair(dst, &map_x, (kb0 + kb) * 64, row, map_to_cta(full_bar(s), 0));
@@ -230,10 +254,10 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
         if (!mbar_wait(tempty_bar(acc), ((tl >> 1) & 1u) ^ 1u)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * 256;
-        for (int kb = 0; kb < kbn; kb++, s = (s + 1 == STAGES) ? 0 : s + 1, ph ^= (s == 0) ? 1u : 0u) {
+        for (int kb = 0; kb < kbn; kb++, s = (s + 1 == p.stages) ? 0 : s + 1, ph ^= (s == 0) ? 1u : 0u) {
           if (!wait_cluster(full_bar(s), ph)) { ok = false; break; }
           tc_fence_after();
-          const uint64_t adesc = make_smem_desc(base + s * STAGE_BYTES), bdesc = make_smem_desc(base + s * STAGE_BYTES + A_BYTES);
+          const uint64_t adesc = make_smem_desc(stages_at + s * p.stage_bytes), bdesc = make_smem_desc(stages_at + s * p.stage_bytes + A_BYTES);
 #pragma unroll
           for (int k = 0; k < 4; k++) mma_f16_kind<CTAS>(d_tmem, adesc + 2u * k, bdesc + 2u * k, p.idesc, (kb | k) != 0 ? 1u : 0u);
           commit<CTAS>(empty_bar(s));
@@ -246,67 +270,64 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
     // ---------------- publish spread stages ----------------
     const uint32_t full0 = CTAS == 2 ? map_to_cta(full_bar(0), 0) : map_to_cta(full_bar(0), rank);
     int s = 0;
-    uint32_t it = 0;
+    uint32_t pairs = 0;       // pairs of stages: the groups take them in turn
     for (int tile = first_tile; tile < num_tiles; tile += tile_step)
-      for (int kb = 0; kb < kbn; kb++, it++, s = (s + 1 == STAGES) ? 0 : s + 1) {
-        named_sync(1 + (int)((it & 1u) * 4 + ((it >> 1) & 3u)), GROUP_THREADS + 32);
+      for (int kb = 0; kb < kbn; kb++, pairs += (uint32_t)((kb & 1) == 0), s = (s + 1 == p.stages) ? 0 : s + 1) {
+        named_sync(group_barrier(pairs, kb & 1), GROUP_THREADS + 32);
         if (lane == 0) arrive_cluster(full0 + 8u * s);
       }
   } else if (warp >= 6) {
     // ---------------- spread the weights ----------------
-    const int grp = (warp - 6) >> 2;
+    const uint32_t grp = (uint32_t)(warp - 6) >> 2;
     const int r = ((warp - 6) & 3) * 32 + lane;
     const ZeroPoint<BF16> zero(p.l.zero);
-    const uint32_t row_at = base + (uint32_t)r * 128u, xr = (uint32_t)(r & 7);
-    int ftile = first_tile, fkb = grp;      // what is fetched next
-    const uint32_t* src = nullptr;
-    auto seek = [&]() {
-      const long long n = ((long long)(ftile / p.tiles_x) * CTAS + half) * ROWS + r;
-      src = p.l.W + min(n, (long long)p.l.N - 1) * p.l.kwords + 2 * kb0;      // rows behind N are not stored: they repeat the last
-    };
-    seek();
-    auto fetch = [&](uint2 (&w)[WB]) {
-      if (ftile >= num_tiles) return;
-#pragma unroll
-      for (int b = 0; b < WB; b++) w[b] = __ldg(reinterpret_cast<const uint2*>(src + b * p.l.plane_words + 2 * fkb));
-      fkb += 2;
-      if (fkb >= kbn) {
-        fkb = grp;
-        ftile += tile_step;
-        if (ftile < num_tiles) seek();
-      }
-    };
-    uint2 cur[WB] = {}, next[WB] = {};
-    if (kbn > 0) fetch(cur);
-    int s = grp;
-    uint32_t ph = 0, it = 0;
+    const uint32_t row_at = stages_at + (uint32_t)r * 128u, xr = (uint32_t)(r & 7);
+    const uint32_t words_at = planes_at + (uint32_t)r * 64u, wr = (uint32_t)(r >> 1) & 3u;      // 64-byte swizzle
+    int s = 0;
+    uint32_t ph = 0, pairs = 0, chunk = 0;
     bool ok = true;
     for (int tile = first_tile; tile < num_tiles; tile += tile_step)
-      for (int kb = grp; kb < kbn; kb += 2, it++) {
-        fetch(next);
-        // after a wait that ran out the warp keeps meeting the named barriers, so that everyone reaches the end
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(s), ph ^ 1u));
-        if (ok) {
-          const uint32_t dst = row_at + s * STAGE_BYTES;
+      for (int kb = 0; kb < kbn; kb += 2, pairs++) {
+        const uint32_t c = chunk % CHUNKS;
+        const bool mine = (pairs & 1u) == grp;
+        if (ok && (mine || kb % CHUNK == 0)) ok = __all_sync(0xffffffffu, mbar_wait(wfull_bar(c), (chunk / CHUNKS) & 1u));
+        uint4 words[WB];
+        if (ok && mine) {
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            uint32_t w[WB], o[16];
-#pragma unroll
-            for (int b = 0; b < WB; b++) w[b] = h ? cur[b].y : cur[b].x;
-            spread_in_order<WB, BF16>(w, zero, o);
-#pragma unroll
-            for (int c = 0; c < 4; c++) st_v4(dst + (((uint32_t)(4 * h + c) ^ xr) << 4), o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+          for (int b = 0; b < WB; b++) {
+            const uint32_t at = words_at + (c * WB + b) * PLANE_BYTES + ((((uint32_t)(kb % CHUNK) >> 1) ^ wr) << 4);
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(words[b].x), "=r"(words[b].y), "=r"(words[b].z), "=r"(words[b].w) : "r"(at));
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        if (ok) named_arrive(1 + grp * 4 + (int)(it & 3u), GROUP_THREADS + 32);
-        else named_sync(1 + grp * 4 + (int)(it & 3u), GROUP_THREADS + 32);      // no ring holds it back: in step with the others
+        if (kb % CHUNK == CHUNK - 2 || kb + 2 >= kbn) {       // this warp reads no more of the chunk
+          __syncwarp();
+          if (lane == 0) mbar_arrive(wempty_bar(c));
+          chunk++;
+        }
 #pragma unroll
-        for (int b = 0; b < WB; b++) cur[b] = next[b];
-        s += 2;
-        if (s >= STAGES) {
-          s -= STAGES;
-          ph ^= 1u;
+        for (int half_pair = 0; half_pair < 2; half_pair++) {
+          if (mine) {
+            // after a wait that ran out the warp keeps meeting the named barriers, so that everyone reaches the end
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(s), ph ^ 1u));
+            if (ok) {
+              const uint32_t dst = row_at + s * p.stage_bytes;
+#pragma unroll
+              for (int h = 0; h < 2; h++) {
+                uint32_t w[WB], o[16];
+#pragma unroll
+                for (int b = 0; b < WB; b++) w[b] = half_pair ? (h ? words[b].w : words[b].z) : (h ? words[b].y : words[b].x);
+                spread_in_order<WB, BF16>(w, zero, o);
+#pragma unroll
+                for (int q = 0; q < 4; q++) st_v4(dst + (((uint32_t)(4 * h + q) ^ xr) << 4), o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              named_arrive(group_barrier(pairs, half_pair), GROUP_THREADS + 32);
+            } else {
+              named_sync(group_barrier(pairs, half_pair), GROUP_THREADS + 32);      // no ring holds it back: in step with the others
+            }
+          }
+          s = s + 1 == p.stages ? 0 : s + 1;
+          ph ^= s == 0 ? 1u : 0u;
         }
       }
     if (!ok && lane == 0) give_up(4);
@@ -367,7 +388,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
         for (int j = 0; j < 32; j++) {
           const int col = c + j, owner = col / slice;
           // [rank that wrote][row of X within the slice][weight row]
-          const uint32_t at = base + (((uint32_t)rank * slice + (col - owner * slice)) * ROWS + quarter * 32 + lane) * 4u;
+          const uint32_t at = stages_at + (((uint32_t)rank * slice + (col - owner * slice)) * ROWS + quarter * 32 + lane) * 4u;
           asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(map_to_cta(at, owner)), "r"(v[j]) : "memory");
         }
       }
@@ -386,7 +407,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
         for (int j = 0; j < 4; j++) {
           f[j] = 0.0f;
           for (int k = 0; k < p.split; k++)
-            f[j] += *reinterpret_cast<const float*>(smem_raw + (base - raw) + (((uint32_t)k * slice + c + j) * ROWS + quarter * 32 + lane) * 4u);
+            f[j] += *reinterpret_cast<const float*>(smem_raw + (stages_at - raw) + (((uint32_t)k * slice + c + j) * ROWS + quarter * 32 + lane) * 4u);
         }
 #pragma unroll
         for (int j = 0; j < 4; j++)
@@ -435,7 +456,7 @@ Plan pick_plan(int M, int N, int kblocks, int sms) {
 }
 
 template <int WB, bool BF16, int CTAS>
-apnn_status launch(cudaStream_t s, const CUtensorMap& map, const TileParams& p, int blocks) {
+apnn_status launch(cudaStream_t s, const CUtensorMap& map, const CUtensorMap& map_w, const TileParams& p, int blocks) {
   const void* kernel = reinterpret_cast<const void*>(linear_tile_kernel<WB, BF16, CTAS>);
   cudaError_t e = ensure_max_smem(kernel, SMEM_BYTES);
   if (e != cudaSuccess) return cuda_fail(e, "linear_tile_kernel shared memory");
@@ -454,16 +475,16 @@ apnn_status launch(cudaStream_t s, const CUtensorMap& map, const TileParams& p, 
     cfg.numAttrs++;
   }
   cfg.attrs = attr;
-  e = cudaLaunchKernelEx(&cfg, linear_tile_kernel<WB, BF16, CTAS>, map, p);
+  e = cudaLaunchKernelEx(&cfg, linear_tile_kernel<WB, BF16, CTAS>, map, map_w, p);
   return e == cudaSuccess ? APNN_OK : cuda_fail(e, "linear_tile_kernel");
 }
 template <bool BF16, int CTAS>
-apnn_status launch_bits(cudaStream_t s, const CUtensorMap& map, const TileParams& p, int blocks) {
+apnn_status launch_bits(cudaStream_t s, const CUtensorMap& map, const CUtensorMap& map_w, const TileParams& p, int blocks) {
   switch (p.l.wbits) {
-    case 1: return launch<1, BF16, CTAS>(s, map, p, blocks);
-    case 2: return launch<2, BF16, CTAS>(s, map, p, blocks);
-    case 3: return launch<3, BF16, CTAS>(s, map, p, blocks);
-    default: return launch<4, BF16, CTAS>(s, map, p, blocks);
+    case 1: return launch<1, BF16, CTAS>(s, map, map_w, p, blocks);
+    case 2: return launch<2, BF16, CTAS>(s, map, map_w, p, blocks);
+    case 3: return launch<3, BF16, CTAS>(s, map, map_w, p, blocks);
+    default: return launch<4, BF16, CTAS>(s, map, map_w, p, blocks);
   }
 }
 
@@ -489,11 +510,20 @@ apnn_status linear_tile(cudaStream_t s, const LinearParams& l, bool bf16) {
   if (fn(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<uint16_t*>(l.X), dims, strides, box, estr,
          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return cuda_fail(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
+  CUtensorMap map_w;      // the planes one below the other, 64-byte rows of a chunk
+  const cuuint64_t wdims[2] = {(cuuint64_t)l.kwords, (cuuint64_t)l.N * l.wbits}, wstrides[1] = {(cuuint64_t)l.kwords * 4};
+  const cuuint32_t wbox[2] = {CHUNK * 2, ROWS};
+  if (fn(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<uint32_t*>(l.W), wdims, wstrides, wbox, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return cuda_fail(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
+  p.stage_bytes = A_BYTES + plan.tn / plan.ctas * BK;
+  p.stages = (SMEM_BYTES - 2048 - CHUNKS * l.wbits * PLANE_BYTES) / p.stage_bytes;
+  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
   const long long tiles = (long long)p.tiles_x * p.tiles_w;
   const int slots = sms / plan.ctas;
   const int blocks = plan.split > 1 ? (int)tiles * plan.split : (int)(tiles < slots ? tiles : slots) * plan.ctas;
-  if (plan.ctas == 2) return bf16 ? launch_bits<true, 2>(s, map, p, blocks) : launch_bits<false, 2>(s, map, p, blocks);
-  return bf16 ? launch_bits<true, 1>(s, map, p, blocks) : launch_bits<false, 1>(s, map, p, blocks);
+  if (plan.ctas == 2) return bf16 ? launch_bits<true, 2>(s, map, map_w, p, blocks) : launch_bits<false, 2>(s, map, map_w, p, blocks);
+  return bf16 ? launch_bits<true, 1>(s, map, map_w, p, blocks) : launch_bits<false, 1>(s, map, map_w, p, blocks);
 }
 
 }  // namespace apnn
