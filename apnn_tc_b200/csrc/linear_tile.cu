@@ -7,7 +7,8 @@
 // cycles as a stage's MMAs: 0.74 against 0.43 ms at 4096 x 16384 x 4096, 4 bits).  The weights never exist as 16-bit floats in
 // memory: eight warps spread the planes to level - zero (spread.cuh) and write the swizzled operand tile themselves, two groups
 // of four warps on alternate pairs of stages of 64 elements of K; a warp that loads nothing meets each group on a named barrier and
-// publishes the stage.  Roles: warp 0 TMA, 1 MMA, 2-5 epilogue, 6-13 spread, 14 publish; every wait is bounded.
+// publishes the stage.  Roles: warp 0 TMA of X, 1 MMA, 2-5 epilogue, 6-13 spread, 14 publish, 15 TMA
+// of the planes; every wait is bounded.
 //
 // What bounds a stage of 64 elements: shared memory, 32 KiB in and out for the weight tile and 256 bytes for each row of X a block
 // holds, at 128 bytes a clock -- 512 clk for the pair's 256 x 256 tile, as long as its MMAs.  Spreading takes about 250.
@@ -30,7 +31,7 @@ constexpr int CHUNK = 8;                        // stages of 64 elements that on
 constexpr int PLANE_BYTES = ROWS * CHUNK * 8;   // of one plane
 constexpr int CHUNKS = 2;
 constexpr int SPREAD_WARPS = 8, GROUP_THREADS = 128;
-constexpr int THREADS = 32 * (6 + SPREAD_WARPS + 1);
+constexpr int THREADS = 32 * (6 + SPREAD_WARPS + 2);
 constexpr int SMEM_BYTES = 232448;              // all an SM has: alignment, barriers, planes, stages
 constexpr int MAX_SPLIT = 8;
 
@@ -47,29 +48,16 @@ struct TileParams {
 __device__ __forceinline__ void arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// The same released to this block only: the publishing of a spread stage.  What it announces is read by the tensor core of the SM that
+// wrote it, behind each writer's fence to the async proxy; no thread of the other block loads it, so nothing has to be made visible
+// there (a release at cluster scope took 1000 clk a stage, twice the stage's MMAs).
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 __device__ __forceinline__ void named_arrive(int id, int count) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory"); }
 __device__ __forceinline__ void named_sync(int id, int count) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory"); }
 __device__ __forceinline__ void st_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity) {      // acquires what the peer's threads wrote
-  unsigned long long t0 = 0;
-  for (uint32_t spin = 0;; spin++) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.b32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (done) return true;
-    if ((spin & 255u) == 255u) {
-      const unsigned long long now = global_timer_ns();
-      if (t0 == 0) t0 = now;
-      else if (now - t0 > WAIT_LIMIT_NS) return false;
-    }
-  }
 }
 template <int CTAS>
 __device__ __forceinline__ void mma_f16_kind(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -216,20 +204,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
       uint32_t ph = 0;
       bool ok = true;
       const int rows = p.tn / CTAS;
-      uint32_t chunk = 0;       // over all tiles
       for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
         const int row = tile % p.tiles_x * p.tn + (int)half * rows;
-        const int wrow = (tile / p.tiles_x * CTAS + (int)half) * ROWS;
         for (int kb = 0; kb < kbn; kb++, s = (s + 1 == p.stages) ? 0 : s + 1, ph ^= (s == 0) ? 1u : 0u) {
-          if (kb % CHUNK == 0) {
-            const uint32_t c = chunk % CHUNKS;
-            if (!mbar_wait(wempty_bar(c), ((chunk / CHUNKS) & 1u) ^ 1u)) { ok = false; break; }
-            mbar_expect_tx(wfull_bar(c), WB * PLANE_BYTES);
-            // rows behind N run into the next plane, and behind the last one they are zeros: their sums are not stored
-            for (int b = 0; b < WB; b++)
-              tma_load_2d(planes_at + (c * WB + b) * PLANE_BYTES, &map_w, 2 * (kb0 + kb), b * p.l.N + wrow, wfull_bar(c));
-            chunk++;
-          }
           if (!mbar_wait(empty_bar(s), ph ^ 1u)) { ok = false; break; }
           const uint32_t dst = stages_at + s * p.stage_bytes + A_BYTES;
           if (CTAS == 2) {
@@ -255,7 +232,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * 256;
         for (int kb = 0; kb < kbn; kb++, s = (s + 1 == p.stages) ? 0 : s + 1, ph ^= (s == 0) ? 1u : 0u) {
-          if (!wait_cluster(full_bar(s), ph)) { ok = false; break; }
+          if (!mbar_wait(full_bar(s), ph)) { ok = false; break; }
           tc_fence_after();
           const uint64_t adesc = make_smem_desc(stages_at + s * p.stage_bytes), bdesc = make_smem_desc(stages_at + s * p.stage_bytes + A_BYTES);
 #pragma unroll
@@ -266,6 +243,24 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
       }
       if (!ok) give_up(2);
     }
+  } else if (warp == 7 + SPREAD_WARPS) {
+    // ---------------- planes by TMA, a chunk ahead of the spreading ----------------
+    if (lane == 0) {
+      uint32_t chunk = 0;       // over all tiles
+      bool ok = true;
+      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
+        const int row = (tile / p.tiles_x * CTAS + (int)half) * ROWS;
+        for (int kb = 0; kb < kbn; kb += CHUNK, chunk++) {
+          const uint32_t c = chunk % CHUNKS;
+          if (!mbar_wait(wempty_bar(c), ((chunk / CHUNKS) & 1u) ^ 1u)) { ok = false; break; }
+          mbar_expect_tx(wfull_bar(c), WB * PLANE_BYTES);
+          // rows behind N run into the next plane, and behind the last one they are zeros: their sums are not stored
+          for (int b = 0; b < WB; b++)
+            tma_load_2d(planes_at + (c * WB + b) * PLANE_BYTES, &map_w, 2 * (kb0 + kb), b * p.l.N + row, wfull_bar(c));
+        }
+      }
+      if (!ok) give_up(6);
+    }
   } else if (warp == 6 + SPREAD_WARPS) {
     // ---------------- publish spread stages ----------------
     const uint32_t full0 = CTAS == 2 ? map_to_cta(full_bar(0), 0) : map_to_cta(full_bar(0), rank);
@@ -274,7 +269,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
     for (int tile = first_tile; tile < num_tiles; tile += tile_step)
       for (int kb = 0; kb < kbn; kb++, pairs += (uint32_t)((kb & 1) == 0), s = (s + 1 == p.stages) ? 0 : s + 1) {
         named_sync(group_barrier(pairs, kb & 1), GROUP_THREADS + 32);
-        if (lane == 0) arrive_cluster(full0 + 8u * s);
+        if (lane == 0) arrive_remote(full0 + 8u * s);
       }
   } else if (warp >= 6) {
     // ---------------- spread the weights ----------------
