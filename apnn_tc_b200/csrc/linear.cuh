@@ -20,12 +20,19 @@ struct LinearParams {
   int split;       // few rows: blocks of a cluster, which share K
 };
 
+// 1 / (1 + exp(-x)) to a few units of 2^-23: one exponential and one reciprocal instruction
+__device__ __forceinline__ float logistic(float x) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return r;
+}
 __device__ __forceinline__ float activate(float v, int act) {
   switch (act) {
     case APNN_ACT_RELU: return v > 0.0f ? v : (v == v ? 0.0f : v);
-    case APNN_ACT_SILU: return v / (1.0f + expf(-v));
+    case APNN_ACT_SILU: return v * logistic(v);
     case APNN_ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678f));
-    case APNN_ACT_GELU_TANH: return 0.5f * v * (1.0f + tanhf(0.79788456f * (v + 0.044715f * v * v * v)));
+    case APNN_ACT_GELU_TANH: return v * logistic(1.5957691f * (v + 0.044715f * v * v * v));      // (1 + tanh u) / 2 = logistic(2 u)
     default: return v;
   }
 }

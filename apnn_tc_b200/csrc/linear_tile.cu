@@ -59,29 +59,45 @@ __device__ __forceinline__ void named_sync(int id, int count) { asm volatile("ba
 __device__ __forceinline__ void st_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+// The four MMAs of a stage and the commit that frees it.  The whole warp runs this with uniform operands and one lane issues, so that
+// descriptors stay in uniform registers: issued from a one-lane branch a stage took 600 clk whatever its width, more than the
+// MMAs of a 256-wide tile.
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t lead;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(lead));
+  return lead;
+}
+#define APNN_STAGE_MMAS(G)                                                                             \
+  "{\n\t.reg .pred q, p, t;\n\t.reg .b64 a, b;\n\t.reg .b32 al, bl;\n\t"                                 \
+  "setp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"                           \
+  "mov.b64 a, {%1, %6};\n\tmov.b64 b, {%2, %6};\n\t"                                                     \
+  "@q tcgen05.mma.cta_group::" G ".kind::f16 [%0], a, b, %3, p;\n\t"                                     \
+  "add.u32 al, %1, 2;\n\tadd.u32 bl, %2, 2;\n\tmov.b64 a, {al, %6};\n\tmov.b64 b, {bl, %6};\n\t"         \
+  "@q tcgen05.mma.cta_group::" G ".kind::f16 [%0], a, b, %3, t;\n\t"                                     \
+  "add.u32 al, %1, 4;\n\tadd.u32 bl, %2, 4;\n\tmov.b64 a, {al, %6};\n\tmov.b64 b, {bl, %6};\n\t"         \
+  "@q tcgen05.mma.cta_group::" G ".kind::f16 [%0], a, b, %3, t;\n\t"                                     \
+  "add.u32 al, %1, 6;\n\tadd.u32 bl, %2, 6;\n\tmov.b64 a, {al, %6};\n\tmov.b64 b, {bl, %6};\n\t"         \
+  "@q tcgen05.mma.cta_group::" G ".kind::f16 [%0], a, b, %3, t;\n\t}"
 template <int CTAS>
-__device__ __forceinline__ void mma_f16_kind(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-  if (CTAS == 2)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
+__device__ __forceinline__ void stage_mmas(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
+  constexpr uint32_t HI = (1024u >> 4) | (1u << 14) | (2u << 29);      // descriptor: 8-row groups 1024 bytes apart, version, 128-byte swizzle
+  if (CTAS == 2) asm volatile(APNN_STAGE_MMAS("2") ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(lead), "r"(HI) : "memory");
+  else asm volatile(APNN_STAGE_MMAS("1") ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(lead), "r"(HI) : "memory");
 }
 template <int CTAS>
-__device__ __forceinline__ void commit(uint32_t bar) {      // pair: the barrier at this offset in both blocks
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t lead) {      // pair: the barrier at this offset in both blocks
   if (CTAS == 2)
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar), "h"((uint16_t)3), "r"(lead) : "memory");
   else
-    tc_commit(bar);
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
 }
 
 // 32 columns of the epilogue: v[j] is the sum of weight row n with row m0 + j of X.
@@ -222,26 +238,28 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
     }
   } else if (warp == 1) {
     // ---------------- MMA ----------------
-    if (lane == 0 && half == 0) {
+    if (half == 0) {
+      const uint32_t lead = elect_lane();
       int s = 0;
       uint32_t ph = 0, tl = 0;
       bool ok = true;
       for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, tl++) {
         const uint32_t acc = tl & 1u;
-        if (!mbar_wait(tempty_bar(acc), ((tl >> 1) & 1u) ^ 1u)) { ok = false; break; }
+        if (!__all_sync(0xffffffffu, mbar_wait(tempty_bar(acc), ((tl >> 1) & 1u) ^ 1u))) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * 256;
-        for (int kb = 0; kb < kbn; kb++, s = (s + 1 == p.stages) ? 0 : s + 1, ph ^= (s == 0) ? 1u : 0u) {
-          if (!mbar_wait(full_bar(s), ph)) { ok = false; break; }
+        for (int kb = 0; kb < kbn; kb++) {
+          if (!__all_sync(0xffffffffu, mbar_wait(full_bar(s), ph))) { ok = false; break; }
           tc_fence_after();
-          const uint64_t adesc = make_smem_desc(stages_at + s * p.stage_bytes), bdesc = make_smem_desc(stages_at + s * p.stage_bytes + A_BYTES);
-#pragma unroll
-          for (int k = 0; k < 4; k++) mma_f16_kind<CTAS>(d_tmem, adesc + 2u * k, bdesc + 2u * k, p.idesc, (kb | k) != 0 ? 1u : 0u);
-          commit<CTAS>(empty_bar(s));
+          const uint32_t a_lo = ((stages_at + s * p.stage_bytes) >> 4) | (1u << 16);
+          stage_mmas<CTAS>(d_tmem, a_lo, a_lo + (A_BYTES >> 4), p.idesc, kb != 0 ? 1u : 0u, lead);
+          commit<CTAS>(empty_bar(s), lead);
+          s = s + 1 == p.stages ? 0 : s + 1;
+          ph ^= s == 0 ? 1u : 0u;
         }
-        if (ok) commit<CTAS>(tfull_bar(acc));
+        if (ok) commit<CTAS>(tfull_bar(acc), lead);
       }
-      if (!ok) give_up(2);
+      if (!ok && lane == 0) give_up(2);
     }
   } else if (warp == 7 + SPREAD_WARPS) {
     // ---------------- planes by TMA, a chunk ahead of the spreading ----------------
