@@ -299,27 +299,32 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
     int s = 0;
     uint32_t ph = 0, pairs = 0, chunk = 0;
     bool ok = true;
-    for (int tile = first_tile; tile < num_tiles; tile += tile_step)
-      for (int kb = 0; kb < kbn; kb += 2, pairs++) {
+    auto advance = [&](int n) {      // n <= 2 < stages
+      s += n;
+      if (s >= p.stages) {
+        s -= p.stages;
+        ph ^= 1u;
+      }
+    };
+    for (int tile = first_tile; tile < num_tiles; tile += tile_step) {
+      // This group's pairs of the tile: every other one, two of a whole chunk.  (A loop over all pairs that skips the other
+      // group's spread them all the same: the compiler works ahead of the branch.)
+      const int first = (int)((pairs & 1u) ^ grp) * 2;
+      for (int kc = 0; kc < kbn; kc += CHUNK, chunk++) {
         const uint32_t c = chunk % CHUNKS;
-        const bool mine = (pairs & 1u) == grp;
-        if (ok && (mine || kb % CHUNK == 0)) ok = __all_sync(0xffffffffu, mbar_wait(wfull_bar(c), (chunk / CHUNKS) & 1u));
-        uint4 words[WB];
-        if (ok && mine) {
+        const int end = min(kc + CHUNK, kbn);
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(wfull_bar(c), (chunk / CHUNKS) & 1u));
+        if (first) advance(2);
+        for (int kb = kc + first; kb < end; kb += 4) {
+          uint4 words[WB];
 #pragma unroll
           for (int b = 0; b < WB; b++) {
-            const uint32_t at = words_at + (c * WB + b) * PLANE_BYTES + ((((uint32_t)(kb % CHUNK) >> 1) ^ wr) << 4);
+            const uint32_t at = words_at + (c * WB + b) * PLANE_BYTES + ((((uint32_t)(kb - kc) >> 1) ^ wr) << 4);
             asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(words[b].x), "=r"(words[b].y), "=r"(words[b].z), "=r"(words[b].w) : "r"(at));
           }
-        }
-        if (kb % CHUNK == CHUNK - 2 || kb + 2 >= kbn) {       // this warp reads no more of the chunk
-          __syncwarp();
-          if (lane == 0) mbar_arrive(wempty_bar(c));
-          chunk++;
-        }
+          const uint32_t pair = pairs + ((uint32_t)kb >> 1);
 #pragma unroll
-        for (int half_pair = 0; half_pair < 2; half_pair++) {
-          if (mine) {
+          for (int half_pair = 0; half_pair < 2; half_pair++) {
             // after a wait that ran out the warp keeps meeting the named barriers, so that everyone reaches the end
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(s), ph ^ 1u));
             if (ok) {
@@ -334,15 +339,19 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
                 for (int q = 0; q < 4; q++) st_v4(dst + (((uint32_t)(4 * h + q) ^ xr) << 4), o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
               }
               asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              named_arrive(group_barrier(pairs, half_pair), GROUP_THREADS + 32);
+              named_arrive(group_barrier(pair, half_pair), GROUP_THREADS + 32);
             } else {
-              named_sync(group_barrier(pairs, half_pair), GROUP_THREADS + 32);      // no ring holds it back: in step with the others
+              named_sync(group_barrier(pair, half_pair), GROUP_THREADS + 32);      // no ring holds it back: in step with the others
             }
+            advance(1);
           }
-          s = s + 1 == p.stages ? 0 : s + 1;
-          ph ^= s == 0 ? 1u : 0u;
+          if (kb + 2 < end) advance(2);
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(wempty_bar(c));
       }
+      pairs += (uint32_t)(kbn >> 1);
+    }
     if (!ok && lane == 0) give_up(4);
   } else if (CTAS == 2 || p.split == 1) {
     // ---------------- epilogue ----------------
