@@ -11,7 +11,7 @@ namespace {
 using namespace tc5;
 
 // ---------------------------------------------------------------------------------------------- few rows
-// At most 16 rows of X: the weights are read once and bound it, so nothing of them goes through shared memory.  A warp takes 16
+// At most 8 rows of X: the weights are read once and bound it, so nothing of them goes through shared memory.  A warp takes 16
 // weight rows, the M operand of mma.sync m16n8k16; the rows of X are its N.  A lane (g, t) reads 16 bytes of each plane of rows
 // g and g + 8, 128 elements of K, the four lanes of a row 64 contiguous bytes, a 512-element block ahead.  Which elements of K
 // meet in one instruction is free as long as both operands agree, so the fields of a word are taken as they lie, bits b and
@@ -20,7 +20,7 @@ using namespace tc5;
 // X would not fit; their sums meet in distributed shared memory, added in the order of the ranks.
 constexpr int FEW_WARPS = 8;
 constexpr int FEW_TILE = 16 * FEW_WARPS;      // weight rows of a block
-constexpr int FEW_ROWS = 16;                  // rows of X
+constexpr int FEW_ROWS = 8;                   // rows of X; from nine on linear_tile is as fast (4096 x 4096, 4 bits: 11.4 us against 12.0 with two column tiles here)
 constexpr int FEW_SPLIT = 8;                  // largest cluster
 constexpr int FEW_X_BYTES = 96 * 1024;        // two blocks to an SM
 
@@ -66,11 +66,11 @@ __device__ __forceinline__ uint2 few_x_load(const uint16_t* src, int left) {
   return v;
 }
 
-template <int WB, bool BF16, int NT>
+template <int WB, bool BF16>
 __global__ void __launch_bounds__(32 * FEW_WARPS, 2) linear_few_rows_kernel(const LinearParams p) {
   using F = Fields<WB>;
   extern __shared__ __align__(64) uint4 x_s[];
-  __shared__ float part_s[FEW_TILE][8 * NT + 1];
+  __shared__ float part_s[FEW_TILE][FEW_ROWS + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int rank = blockIdx.x % p.split;
@@ -81,11 +81,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) linear_few_rows_kernel(cons
   grid_launch_dependents();
   if (p.status_flag && blockIdx.x == 0 && threadIdx.x == 0) *p.status_flag = 0;
   const ZeroPoint<BF16> zero(p.zero);
-  float acc[NT][4];
-#pragma unroll
-  for (int i = 0; i < NT; i++)
-#pragma unroll
-    for (int c = 0; c < 4; c++) acc[i][c] = 0.0f;
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 
   // This lane's chunk of the planes for block kb.  Beyond the edges it reads what is there: sums of rows behind N are not
   // stored, and X is zero behind K.
@@ -133,9 +129,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) linear_few_rows_kernel(cons
   __syncthreads();
 
   // lanes behind the last row of X repeat it: their columns are not stored
-  const uint4* x_row[NT];
-#pragma unroll
-  for (int i = 0; i < NT; i++) x_row[i] = x_s + few_x_at(min(i * 8 + g, p.M - 1), blocks, 0, 0, t, 0);
+  const uint4* x_row = x_s + few_x_at(min(g, p.M - 1), blocks, 0, 0, t, 0);
   auto contract = [&](int kb, const uint4 (&w)[2][WB]) {
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -147,18 +141,16 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) linear_few_rows_kernel(cons
       }
       gather_fields<WB>(p0, f0);
       gather_fields<WB>(p1, f1);
-      uint32_t y[NT][16];
+      uint32_t y[16];
 #pragma unroll
-      for (int i = 0; i < NT; i++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          // x_row stands at piece t ^ (m & 1) of its group of four; piece c lies c exchanged bits from there
-          const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(x_row[i] + (kb * 4 + j) * 16) ^ (uintptr_t)(c * 16));
-          y[i][4 * c] = v.x;
-          y[i][4 * c + 1] = v.y;
-          y[i][4 * c + 2] = v.z;
-          y[i][4 * c + 3] = v.w;
-        }
+      for (int c = 0; c < 4; c++) {
+        // x_row stands at piece t ^ (m & 1) of its group of four; piece c lies c exchanged bits from there
+        const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(x_row + (kb * 4 + j) * 16) ^ (uintptr_t)(c * 16));
+        y[4 * c] = v.x;
+        y[4 * c + 1] = v.y;
+        y[4 * c + 2] = v.z;
+        y[4 * c + 3] = v.w;
+      }
 #pragma unroll
       for (int q = 0; q < F::WORDS; q++)
 #pragma unroll
@@ -166,22 +158,11 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) linear_few_rows_kernel(cons
           const int b0 = F::WIDTH * f + q, b1 = F::WIDTH * (f + 1) + q;
           const uint32_t a0 = level_pair<F::WIDTH, BF16>(f0[q], f, zero), a1 = level_pair<F::WIDTH, BF16>(f1[q], f, zero);
           const uint32_t a2 = level_pair<F::WIDTH, BF16>(f0[q], f + 1, zero), a3 = level_pair<F::WIDTH, BF16>(f1[q], f + 1, zero);
-#pragma unroll
-          for (int i = 0; i < NT; i++) mma_16<BF16>(acc[i], a0, a1, a2, a3, y[i][b0], y[i][b1]);
+          mma_16<BF16>(acc, a0, a1, a2, a3, y[b0], y[b1]);
         }
     }
   };
-  if (NT == 2 && WB > 2) {     // no registers for a second set: the next block waits in L2
-    for (int kb = 0; kb < blocks; kb++) {
-      if (kb > 0) load_weights(kb, w0);
-      const int word = min((kb0 + min(kb + 1, blocks - 1)) * 16 + t * 4, p.kwords - 4);
-#pragma unroll
-      for (int r = 0; r < 2; r++)
-#pragma unroll
-        for (int b = 0; b < WB; b++) asm volatile("prefetch.global.L2 [%0];" ::"l"(base[r] + b * p.plane_words + word));
-      contract(kb, w0);
-    }
-  } else for (int kb = 0; kb < blocks; kb += 2) {
+  for (int kb = 0; kb < blocks; kb += 2) {
     load_weights(kb + 1, w1);
     contract(kb, w0);
     if (kb + 1 == blocks) break;
@@ -189,9 +170,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) linear_few_rows_kernel(cons
     contract(kb + 1, w1);
   }
 #pragma unroll
-  for (int i = 0; i < NT; i++)
-#pragma unroll
-    for (int c = 0; c < 4; c++) part_s[warp * 16 + g + (c >> 1) * 8][i * 8 + 2 * t + (c & 1)] = acc[i][c];
+  for (int c = 0; c < 4; c++) part_s[warp * 16 + g + (c >> 1) * 8][2 * t + (c & 1)] = acc[c];
   const int rows = FEW_TILE / p.split;      // of the block's, finished by this rank
   if (p.split > 1) cluster_sync_all();
   else __syncthreads();
@@ -202,7 +181,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) linear_few_rows_kernel(cons
     if (n >= p.N) continue;
     float sum = 0.0f;
     if (p.split > 1) {
-      for (int k = 0; k < p.split; k++) sum += ld_cluster(map_to_cta(mine + (row * (8 * NT + 1) + m) * 4, k));
+      for (int k = 0; k < p.split; k++) sum += ld_cluster(map_to_cta(mine + (row * (FEW_ROWS + 1) + m) * 4, k));
     } else {
       sum = part_s[row][m];
     }
@@ -211,9 +190,9 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) linear_few_rows_kernel(cons
   if (p.split > 1) cluster_sync_all();      // no rank leaves while another reads its sums
 }
 
-template <bool BF16, int NT>
+template <bool BF16>
 void (*few_rows_kernel(int wbits))(LinearParams) {
-  return wbits == 1 ? linear_few_rows_kernel<1, BF16, NT> : wbits == 2 ? linear_few_rows_kernel<2, BF16, NT> : wbits == 3 ? linear_few_rows_kernel<3, BF16, NT> : linear_few_rows_kernel<4, BF16, NT>;
+  return wbits == 1 ? linear_few_rows_kernel<1, BF16> : wbits == 2 ? linear_few_rows_kernel<2, BF16> : wbits == 3 ? linear_few_rows_kernel<3, BF16> : linear_few_rows_kernel<4, BF16>;
 }
 
 }  // namespace
@@ -273,9 +252,7 @@ extern "C" apnn_status apnn_linear_planes(void* stream, int wbits, const void* W
     }
     if (x_bytes(split) <= FEW_X_BYTES) {
       p.split = split;
-      const bool bf16 = d->x_type == APNN_TYPE_BF16;
-      void (*const kernel)(LinearParams) = M <= 8 ? (bf16 ? few_rows_kernel<true, 1>(wbits) : few_rows_kernel<false, 1>(wbits))
-                                                  : (bf16 ? few_rows_kernel<true, 2>(wbits) : few_rows_kernel<false, 2>(wbits));
+      void (*const kernel)(LinearParams) = d->x_type == APNN_TYPE_BF16 ? few_rows_kernel<true>(wbits) : few_rows_kernel<false>(wbits);
       cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(kernel), FEW_X_BYTES);
       if (e != cudaSuccess) return cuda_fail(e, "linear_few_rows_kernel shared memory");
       cfg.gridDim = dim3((unsigned)(tiles * split), 1, 1);

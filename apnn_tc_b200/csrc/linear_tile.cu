@@ -7,8 +7,8 @@
 // cycles as a stage's MMAs: 0.74 against 0.43 ms at 4096 x 16384 x 4096, 4 bits).  The weights never exist as 16-bit floats in
 // memory: eight warps spread the planes to level - zero (spread.cuh) and write the swizzled operand tile themselves, two groups
 // of four warps on alternate pairs of stages of 64 elements of K; a warp that loads nothing meets each group on a named barrier and
-// publishes the stage.  Roles: warp 0 TMA of X, 1 MMA, 2-5 epilogue, 6-13 spread, 14 publish, 15 TMA
-// of the planes; every wait is bounded.
+// publishes the stage.  Roles: warp 0 TMA of X, 1 MMA, 2-9 epilogue (two to a quarter of the TMEM
+// lanes), 10-17 spread, 18 publish, 19 TMA of the planes; every wait is bounded.
 //
 // What bounds a stage of 64 elements: shared memory, 32 KiB in and out for the weight tile and 256 bytes for each row of X a block
 // holds, at 128 bytes a clock -- 512 clk for the pair's 256 x 256 tile, as long as its MMAs.  Spreading takes about 250.
@@ -30,8 +30,10 @@ constexpr int A_BYTES = ROWS * BK;
 constexpr int CHUNK = 8;                        // stages of 64 elements that one load of the planes covers
 constexpr int PLANE_BYTES = ROWS * CHUNK * 8;   // of one plane
 constexpr int CHUNKS = 2;
-constexpr int SPREAD_WARPS = 8, GROUP_THREADS = 128;
-constexpr int THREADS = 32 * (6 + SPREAD_WARPS + 2);
+constexpr int EPI_WARPS = 8, SPREAD_WARPS = 8, GROUP_THREADS = 128;
+constexpr int FIRST_SPREAD = 2 + EPI_WARPS, PUBLISH = FIRST_SPREAD + SPREAD_WARPS, PLANES = PUBLISH + 1;      // warps
+constexpr int THREADS = 32 * (PLANES + 1);
+constexpr int COLUMNS = 16;                     // of an accumulator that an epilogue warp takes at a time
 constexpr int SMEM_BYTES = 232448;              // all an SM has: alignment, barriers, planes, stages
 constexpr int MAX_SPLIT = 8;
 
@@ -42,6 +44,7 @@ struct TileParams {
   int kblocks;              // of 64 elements: even
   int split;                // blocks of a cluster that share K (1: none)
   int stages, stage_bytes;
+  int wide;                 // 16-bit output whose pairs of columns are words
   uint32_t idesc;
 };
 
@@ -100,55 +103,80 @@ __device__ __forceinline__ void commit(uint32_t bar, uint32_t lead) {      // pa
         "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(lead) : "memory");
 }
 
-// 32 columns of the epilogue: v[j] is the sum of weight row n with row m0 + j of X.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// 16 columns of the epilogue: v[j] is the sum of weight row n (a lane each; live: there is one) with row m0 + j of X.  wide: the
+// output may be stored in pairs of columns.
 template <bool BF16>
-__device__ __forceinline__ void finish_columns(const LinearParams& p, float (&v)[32], long long m0, long long n, bool live, float scale, float bias) {
-  const int count = (int)min(32ll, (long long)p.M - m0);
-  if (!live || count <= 0) return;
+__device__ __forceinline__ void finish_columns(const LinearParams& p, float (&v)[COLUMNS], long long m0, long long n, bool live, bool wide, float scale, float bias) {
+  const int count = (int)min((long long)COLUMNS, (long long)p.M - m0);
+  if (count <= 0) return;      // the whole warp
 #pragma unroll
-  for (int j = 0; j < 32; j++) v[j] = fmaf(v[j], scale, bias);
+  for (int j = 0; j < COLUMNS; j++) v[j] = fmaf(v[j], scale, bias);
   switch (p.act) {
     case APNN_ACT_RELU:
 #pragma unroll
-      for (int j = 0; j < 32; j++) v[j] = activate(v[j], APNN_ACT_RELU);
+      for (int j = 0; j < COLUMNS; j++) v[j] = activate(v[j], APNN_ACT_RELU);
       break;
     case APNN_ACT_SILU:
 #pragma unroll
-      for (int j = 0; j < 32; j++) v[j] = activate(v[j], APNN_ACT_SILU);
+      for (int j = 0; j < COLUMNS; j++) v[j] = activate(v[j], APNN_ACT_SILU);
       break;
     case APNN_ACT_GELU:
 #pragma unroll
-      for (int j = 0; j < 32; j++) v[j] = activate(v[j], APNN_ACT_GELU);
+      for (int j = 0; j < COLUMNS; j++) v[j] = activate(v[j], APNN_ACT_GELU);
       break;
     case APNN_ACT_GELU_TANH:
 #pragma unroll
-      for (int j = 0; j < 32; j++) v[j] = activate(v[j], APNN_ACT_GELU_TANH);
+      for (int j = 0; j < COLUMNS; j++) v[j] = activate(v[j], APNN_ACT_GELU_TANH);
       break;
     default: break;
   }
   if (p.out_f32) {
-    const float* r = static_cast<const float*>(p.residual) + m0 * p.ldr + n;
+    if (p.residual && live) {
+      const float* r = static_cast<const float*>(p.residual) + m0 * p.ldr + n;
+#pragma unroll
+      for (int j = 0; j < COLUMNS; j++, r += p.ldr)
+        if (j < count) v[j] += *r;
+    }
+    if (!live) return;
     float* o = static_cast<float*>(p.out) + m0 * p.ldo + n;
-    if (p.residual) {
 #pragma unroll
-      for (int j = 0; j < 32; j++)
-        if (j < count) v[j] += r[j * p.ldr];
-    }
-#pragma unroll
-    for (int j = 0; j < 32; j++)
-      if (j < count) o[j * p.ldo] = v[j];
-  } else {
-    const uint16_t* r = static_cast<const uint16_t*>(p.residual) + m0 * p.ldr + n;
-    uint16_t* o = static_cast<uint16_t*>(p.out) + m0 * p.ldo + n;
-    if (p.residual) {
-#pragma unroll
-      for (int j = 0; j < 32; j++)
-        if (j < count) v[j] += unpack2<BF16>(r[j * p.ldr]).x;
-    }
-#pragma unroll
-    for (int j = 0; j < 32; j++)
-      if (j < count) o[j * p.ldo] = (uint16_t)pack2<BF16>(v[j], 0.0f);
+    for (int j = 0; j < COLUMNS; j++, o += p.ldo)
+      if (j < count) *o = v[j];
+    return;
   }
+  if (p.residual && live) {
+    const uint16_t* r = static_cast<const uint16_t*>(p.residual) + m0 * p.ldr + n;
+    uint16_t x[COLUMNS];      // all on their way together: the stores below may be to the same addresses
+#pragma unroll
+    for (int j = 0; j < COLUMNS; j++, r += p.ldr) x[j] = j < count ? *r : (uint16_t)0;
+#pragma unroll
+    for (int j = 0; j < COLUMNS; j++) v[j] += unpack2<BF16>(x[j]).x;
+  }
+  uint16_t* o = static_cast<uint16_t*>(p.out) + m0 * p.ldo + n;
+  if (wide) {
+    // neighbouring lanes exchange a value of two rows, so that each stores two columns of one row
+    const bool odd = threadIdx.x & 1;
+    o += odd ? p.ldo - 1 : 0;
+#pragma unroll
+    for (int j = 0; j < COLUMNS; j += 2, o += 2 * p.ldo) {
+      const float other = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
+      const uint32_t word = odd ? pack2<BF16>(other, v[j + 1]) : pack2<BF16>(v[j], other);
+      if (live && j + (odd ? 1 : 0) < count) *reinterpret_cast<uint32_t*>(o) = word;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < COLUMNS; j++, o += p.ldo)
+    if (live && j < count) *o = (uint16_t)pack2<BF16>(v[j], 0.0f);
 }
 
 // The named barrier on which the group of pair `pairs` hands over its first or second stage.  Four in turn for each group: it comes
@@ -187,7 +215,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
     }
     for (int a = 0; a < 2; a++) {
       mbar_init(tfull_bar(a), 1);
-      mbar_init(tempty_bar(a), 4 * CTAS);
+      mbar_init(tempty_bar(a), EPI_WARPS * CTAS);
       mbar_init(wfull_bar(a), 1);
       mbar_init(wempty_bar(a), SPREAD_WARPS);
     }
@@ -261,7 +289,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
       }
       if (!ok && lane == 0) give_up(2);
     }
-  } else if (warp == 7 + SPREAD_WARPS) {
+  } else if (warp == PLANES) {
     // ---------------- planes by TMA, a chunk ahead of the spreading ----------------
     if (lane == 0) {
       uint32_t chunk = 0;       // over all tiles
@@ -279,7 +307,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
       }
       if (!ok) give_up(6);
     }
-  } else if (warp == 6 + SPREAD_WARPS) {
+  } else if (warp == PUBLISH) {
     // ---------------- publish spread stages ----------------
     const uint32_t full0 = CTAS == 2 ? map_to_cta(full_bar(0), 0) : map_to_cta(full_bar(0), rank);
     int s = 0;
@@ -289,10 +317,10 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
         named_sync(group_barrier(pairs, kb & 1), GROUP_THREADS + 32);
         if (lane == 0) arrive_remote(full0 + 8u * s);
       }
-  } else if (warp >= 6) {
+  } else if (warp >= FIRST_SPREAD) {
     // ---------------- spread the weights ----------------
-    const uint32_t grp = (uint32_t)(warp - 6) >> 2;
-    const int r = ((warp - 6) & 3) * 32 + lane;
+    const uint32_t grp = (uint32_t)(warp - FIRST_SPREAD) >> 2;
+    const int r = ((warp - FIRST_SPREAD) & 3) * 32 + lane;
     const ZeroPoint<BF16> zero(p.l.zero);
     const uint32_t row_at = stages_at + (uint32_t)r * 128u, xr = (uint32_t)(r & 7);
     const uint32_t words_at = planes_at + (uint32_t)r * 64u, wr = (uint32_t)(r >> 1) & 3u;      // 64-byte swizzle
@@ -355,28 +383,29 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
     if (!ok && lane == 0) give_up(4);
   } else if (CTAS == 2 || p.split == 1) {
     // ---------------- epilogue ----------------
-    const int quarter = warp & 3;
+    const int quarter = warp & 3, turn = (warp - 2) >> 2;
     uint32_t tl = 0;
     bool ok = true;
     for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step, tl++) {
       const uint32_t acc = tl & 1u;
       const long long n = ((long long)(tile / p.tiles_x) * CTAS + half) * ROWS + quarter * 32 + lane;
       const bool live = n < p.l.N;
+      const bool wide = p.wide && n - lane + 32 <= p.l.N;      // all of the warp's columns
       const float scale = live ? __ldg(p.l.scale + n) : 0.0f, bias = live && p.l.bias ? __ldg(p.l.bias + n) : 0.0f;
       if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), (tl >> 1) & 1u))) { ok = false; break; }
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * 256;
       const long long m0 = (long long)(tile % p.tiles_x) * p.tn;
 #pragma unroll 1
-      for (int c = 0; c < p.tn; c += 32) {
-        uint32_t v[32];
+      for (int c = turn * COLUMNS; c < p.tn; c += 2 * COLUMNS) {
+        uint32_t v[COLUMNS];
         __syncwarp();
-        tmem_ld32(taddr + c, v);
+        tmem_ld16(taddr + c, v);
         tmem_ld_wait();
-        float f[32];
+        float f[COLUMNS];
 #pragma unroll
-        for (int j = 0; j < 32; j++) f[j] = __uint_as_float(v[j]);
-        finish_columns<BF16>(p.l, f, m0 + c, n, live, scale, bias);
+        for (int j = 0; j < COLUMNS; j++) f[j] = __uint_as_float(v[j]);
+        finish_columns<BF16>(p.l, f, m0 + c, n, live, wide, scale, bias);
       }
       tc_fence_before();
       __syncwarp();
@@ -390,8 +419,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
 
   if (CTAS == 1 && p.split > 1) {
     // ---------------- the cluster's sums of one tile meet: every block's in the order of the ranks ----------------
-    const bool reader = warp >= 2 && warp < 6;
-    const int quarter = warp & 3, slice = p.tn / p.split;      // rows of X that a rank finishes
+    const bool reader = warp >= 2 && warp < 2 + EPI_WARPS;
+    const int quarter = warp & 3, turn = (warp - 2) >> 2, slice = p.tn / p.split;      // rows of X that a rank finishes
     bool ok = true;
     __syncwarp();
     if (reader) ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(0), 0));
@@ -401,13 +430,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
     if (reader && ok) {
       const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
-      for (int c = 0; c < p.tn; c += 32) {
-        uint32_t v[32];
+      for (int c = turn * COLUMNS; c < p.tn; c += 2 * COLUMNS) {
+        uint32_t v[COLUMNS];
         __syncwarp();
-        tmem_ld32(taddr + c, v);
+        tmem_ld16(taddr + c, v);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 32; j++) {
+        for (int j = 0; j < COLUMNS; j++) {
           const int col = c + j, owner = col / slice;
           // [rank that wrote][row of X within the slice][weight row]
           const uint32_t at = stages_at + (((uint32_t)rank * slice + (col - owner * slice)) * ROWS + quarter * 32 + lane) * 4u;
@@ -423,7 +452,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
       const float scale = live ? __ldg(p.l.scale + n) : 0.0f, bias = live && p.l.bias ? __ldg(p.l.bias + n) : 0.0f;
       const long long m0 = (long long)(tile % p.tiles_x) * p.tn + (long long)rank * slice;
 #pragma unroll 1
-      for (int c = 0; c < slice; c += 4) {
+      for (int c = turn * 4; c < slice; c += 8) {
         float f[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -455,8 +484,10 @@ struct Plan {
   int ctas, tn, split;
 };
 
-// The plan of the shortest estimated time, in clocks: waves of tiles times the stages of one, each as long as the slowest of the MMAs,
-// shared memory and spreading, and what a block spends before its first stage and behind its last.
+// The plan of the shortest estimated time.  A wave of tiles takes its stages or its epilogue, whichever is longer, and the last
+// epilogue shows; a split adds the exchange.  The figures (us) are fitted to 24 shapes on every plan (16 to 4096 rows, 1000 to 32003
+// weights, K from 128 to 8192), most within a tenth: e.g. 333 x 2337 x 2296 14.9 on 64-wide tiles, 18.7 on the pair's 256; 128 x 4096 x 4096
+// 17.9 with 128-wide tiles and K in four, 23.5 without.
 Plan pick_plan(int M, int N, int kblocks, int sms) {
   Plan best = {1, 32, 1};
   double least = 1e30;
@@ -465,10 +496,16 @@ Plan pick_plan(int M, int N, int kblocks, int sms) {
       for (int split = 1; split <= (ctas == 2 ? 1 : MAX_SPLIT) && 2 * split <= kblocks; split *= 2) {
         if (tn / split < 4) continue;
         const long long tiles = (long long)((M + tn - 1) / tn) * ((N + ROWS * ctas - 1) / (ROWS * ctas));
-        const int slots = sms / (ctas * split);
-        const double stage = 2.0 * tn > 256.0 + 2.0 * tn / ctas ? 2.0 * tn : 256.0 + 2.0 * tn / ctas;
-        const double stages = (double)((kblocks / 2 + split - 1) / split * 2);
-        const double time = (double)((tiles + slots - 1) / slots) * (stages * (stage > 300 ? stage : 300) + (split > 1 ? 3000.0 + 20.0 * tn : 0.0)) + 4000.0 + 15.0 * tn;
+        // a cluster finds its blocks within one group of SMs: the driver knows how many fit
+        const int slots = split > 1 ? cluster_capacity(reinterpret_cast<const void*>(linear_tile_kernel<4, true, 1>), THREADS, SMEM_BYTES, split) : sms / ctas;
+        if (slots < 1) continue;
+        const double stage = ctas == 1 ? (tn == 32 ? 0.255 : tn == 64 ? 0.265 : tn == 128 ? 0.295 : 0.43) : (tn == 64 ? 0.265 : tn == 128 ? 0.285 : 0.375);
+        const double epilogue = (ctas == 1 ? 0.8 : 1.4) + 0.012 * tn;
+        const double stages = stage * (double)((kblocks / 2 + split - 1) / split * 2);
+        const double exchange = split > 1 ? 1.5 + 0.1 * (tn / split) + 0.015 * tn : 0.0;
+        // a split block ends with its tile: the next wave's begins anew
+        const double wave = split > 1 ? stages + exchange + epilogue + 3.0 : stages > epilogue ? stages : epilogue;
+        const double time = (double)((tiles + slots - 1) / slots) * wave + (split > 1 ? 1.0 : 4.0 + epilogue);
         if (time < least) {
           least = time;
           best = {ctas, tn, split};
@@ -516,6 +553,7 @@ apnn_status linear_tile(cudaStream_t s, const LinearParams& l, bool bf16) {
   TileParams p = {};
   p.l = l;
   p.kblocks = l.kwords / 2;
+  p.wide = !l.out_f32 && l.ldo % 2 == 0 && (reinterpret_cast<uintptr_t>(l.out) & 3u) == 0;
   const int sms = device_sm_count();
   const Plan plan = pick_plan(l.M, l.N, p.kblocks, sms);
   p.tn = plan.tn;
