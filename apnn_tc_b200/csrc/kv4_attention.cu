@@ -1,101 +1,13 @@
 // Attention over the 4-bit cache.
-#include <cmath>
 #include <type_traits>
 
-#include "kv4.cuh"
-#include "tc5_common.cuh"
+#include "kv4_attention.cuh"
 
 namespace apnn {
 namespace {
 
 using namespace tc5;
 
-struct AttentionParams {
-  Kv4View cache;
-  Kv4Batch batch;
-  const uint16_t* q;
-  uint16_t* out;
-  float* lse;
-  long long q_stride, out_stride;
-  int q_heads, group, causal, window;
-  float scale;
-  int* status_flag;
-};
-
-// One warp per row and query head, lanes over the head's elements.
-template <bool BF16, int D>
-__global__ void __launch_bounds__(128) kv4_attention_rows_kernel(const AttentionParams p) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int t = (int)(item / p.q_heads), h = (int)(item % p.q_heads);
-  grid_dependency_wait();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.status_flag = 0;
-  if (t >= p.batch.rows) return;
-  const int b = sequence_of(p.batch.cu_q, p.batch.sequences, t, lane);
-  if (b < 0) return;
-  const int first = __ldg(p.batch.cu_q + b), len = __ldg(p.batch.kv_len + b);
-  const int i = t - first;
-  if (i >= p.batch.max_q) return;
-  const int pos = len - (__ldg(p.batch.cu_q + b + 1) - first) + i;
-  int end = len, begin = 0;
-  if (p.causal) {
-    end = min(end, pos + 1);
-    if (p.window > 0) begin = max(0, pos + 1 - p.window);
-  }
-  end = (int)min((long long)end, (long long)p.batch.table_width << p.cache.page_shift);
-  float q[E], o[E];
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    const uint32_t w = p.q[t * p.q_stride + (long long)h * D + lane * E + e];
-    q[e] = unpack2<BF16>(w).x;
-    o[e] = 0.0f;
-  }
-  float top = -INFINITY, sum = 0.0f;
-  const long long codes = (long long)p.cache.page_size * (D / 2);
-  for (int j = begin; j < end; j++) {
-    const uint8_t* page = page_of(p.cache, p.batch, b, j);
-    if (page == nullptr) continue;
-    const uint8_t* head = page + (h / p.group) * p.cache.head_bytes;
-    const int slot = j & (p.cache.page_size - 1);
-    const float2 kp = unpack2<BF16>(*reinterpret_cast<const uint32_t*>(head + 2 * codes + slot * 4ll));
-    const float2 vp = unpack2<BF16>(*reinterpret_cast<const uint32_t*>(head + 2 * codes + (p.cache.page_size + slot) * 4ll));
-    float s = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      const int d = lane * E + e;
-      const uint32_t n = (head[slot * (long long)(D / 2) + d / 2] >> (4 * (d & 1))) & 15u;
-      s += q[e] * fmaf(kp.x, (float)n, kp.y);
-    }
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
-    s *= p.scale;
-    const float m = fmaxf(top, s);
-    const float keep = top == -INFINITY ? 0.0f : expf(top - m), w = expf(s - m);
-    sum = sum * keep + w;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      const int d = lane * E + e;
-      const uint32_t n = (head[codes + slot * (long long)(D / 2) + d / 2] >> (4 * (d & 1))) & 15u;
-      o[e] = o[e] * keep + w * fmaf(vp.x, (float)n, vp.y);
-    }
-    top = m;
-  }
-#pragma unroll
-  for (int e = 0; e < E; e++)
-    p.out[t * p.out_stride + (long long)h * D + lane * E + e] = (uint16_t)pack2<BF16>(sum == 0.0f ? 0.0f : o[e] / sum, 0.0f);
-  if (p.lse && lane == 0) p.lse[(long long)t * p.q_heads + h] = sum == 0.0f ? -INFINITY : top + logf(sum);
-}
-
-
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // D(16x8, fp32) += A(16x16, fp16) * B(16x8, fp16)
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -119,16 +31,6 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t* r) {
   if (WORDS == 1) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r[0]) : "r"(a));
   if (WORDS == 2) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(a));
   if (WORDS == 4) asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
-}
-
-// Four elements of an output row from their sums: row r of the sequence's rows for key head h.
-template <bool BF16, int D, typename S>
-__device__ __forceinline__ void finish_row(const AttentionParams& p, const S& s, int h, int r, int d, float M, float L, float4 v) {
-  const int i = r / p.group, head = h * p.group + (r - i * p.group);
-  const float inv = L == 0.0f ? 0.0f : 1.0f / L;      // no key: 0; NaN stays NaN
-  const long long t = s.first + i;
-  *reinterpret_cast<uint2*>(p.out + t * p.out_stride + (long long)head * D + d) = make_uint2(pack2<BF16>(v.x * inv, v.y * inv), pack2<BF16>(v.z * inv, v.w * inv));
-  if (d == 0 && p.lse != nullptr) p.lse[t * p.q_heads + head] = L == 0.0f ? -INFINITY : M * LN2 + logf(L);
 }
 
 // ---------------------------------------------------------------------------------------------- single and few tokens
@@ -179,64 +81,9 @@ struct Flow {
 // in different banks (D = 64; two by two at D = 128), while eight lanes that read key rows still take whole 128-byte lines.
 __device__ __forceinline__ int flow_key(int r) { return r ^ ((r >> 1) & 1) ^ ((r >> 2) & 1); }
 
-// Two fp32 in one instruction.
-struct Pair { unsigned long long v; };
-__device__ __forceinline__ Pair pair(float x, float y) {
-  Pair p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(x), "f"(y));
-  return p;
-}
-__device__ __forceinline__ float2 unpair(Pair p) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
-  return f;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-  Pair d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-  Pair d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return d;
-}
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
                : "memory");
-}
-
-// One sequence of the call: which rows, which keys any of them sees.
-struct Span {
-  int first, n;        // rows first .. first + n - 1
-  int pos0;            // position of the first
-  int len;             // keys there are
-  int begin, end;      // keys that some row sees lie in [begin, end)
-  int tile0, tiles;    // tiles of `TILE` keys over them; one (empty) tile where there is no key, none without rows
-};
-template <int TILE>
-__device__ __forceinline__ Span span_of(const AttentionParams& p, int b) {
-  Span s;
-  s.first = __ldg(p.batch.cu_q + b);
-  const int all = __ldg(p.batch.cu_q + b + 1) - s.first;
-  s.n = s.first < 0 ? 0 : min(min(all, p.batch.max_q), p.batch.rows - s.first);
-  const int kv = __ldg(p.batch.kv_len + b);
-  s.pos0 = kv - all;
-  s.len = (int)min((long long)kv, (long long)p.batch.table_width << p.cache.page_shift);
-  s.begin = 0;
-  s.end = s.len;
-  if (p.causal) {
-    s.end = min(s.end, s.pos0 + s.n);
-    if (p.window > 0) s.begin = max(0, s.pos0 + 1 - p.window);
-  }
-  s.tile0 = s.begin / TILE;
-  s.tiles = s.n <= 0 ? 0 : s.end > s.begin ? (s.end + TILE - 1) / TILE - s.tile0 : 1;
-  return s;
 }
 
 struct FlowParams {
@@ -905,7 +752,7 @@ size_t apnn_kv4_attention_workspace_bytes(const apnn_kv4_cache* cache, const apn
   Kv4Batch geo = {};
   if (kv4_view(cache, &view) != APNN_OK || kv4_batch(batch, 1, &geo) != APNN_OK || q_heads <= 0 || q_heads % cache->heads != 0) return 0;
   const int group = q_heads / cache->heads;
-  if ((long long)batch->max_q * group > largest_rows(cache->head_dim)) return 256;
+  if ((long long)batch->max_q * group > largest_rows(cache->head_dim)) return kv4_prompt_workspace_bytes(cache, batch, group);
   return flow_plan(cache, batch, group).bytes;
 }
 
@@ -946,18 +793,7 @@ apnn_status apnn_kv4_attention(void* stream, const apnn_kv4_cache* cache, const 
         {launch_flow_rows<true, 64>, launch_flow_rows<true, 128>, launch_flow_rows<true, 256>}};
     return launch[cache->type == APNN_TYPE_BF16][cache->head_dim / 128](s, f, fp);
   }
-  void (*const kernels[2][3])(AttentionParams) = {
-      {kv4_attention_rows_kernel<false, 64>, kv4_attention_rows_kernel<false, 128>, kv4_attention_rows_kernel<false, 256>},
-      {kv4_attention_rows_kernel<true, 64>, kv4_attention_rows_kernel<true, 128>, kv4_attention_rows_kernel<true, 256>}};
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(((long long)a->rows * a->q_heads + 3) / 4), 1, 1);
-  cfg.blockDim = dim3(128, 1, 1);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  cfg.numAttrs = pdl_attribute(attr);
-  cfg.attrs = attr;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernels[cache->type == APNN_TYPE_BF16][cache->head_dim / 128], p);
-  return e == cudaSuccess ? APNN_OK : cuda_fail(e, "kv4_attention_rows_kernel");
+  return kv4_prompt(s, cache, batch, p, workspace);
 }
 
 apnn_status apnn_kv4_attention_check(void* stream, const void* workspace) {
