@@ -16,6 +16,8 @@
 // Bounds per 128 x 128 tile and 128 elements: 1024 clk of MMAs, 1024 of exponentials, about 950 issue slots of softmax and 200 of
 // spreading (one K / V tile serves both row tiles).
 // Few units and many keys: the keys are split over blocks and kv4_prompt_join_kernel adds the parts in order.
+#include <type_traits>
+
 #include "kv4_attention.cuh"
 
 namespace apnn {
@@ -90,6 +92,12 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+      "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -100,7 +108,9 @@ __device__ __forceinline__ uint32_t lds(uint32_t at) {
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at));
   return v;
 }
-__device__ __forceinline__ void lds_pairs(uint32_t at, Pair& a, Pair& b) { asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a.v), "=l"(b.v) : "r"(at)); }
+struct __align__(16) PairPair {      // of two keys: steps, mids
+  Pair step, mid;
+};
 __device__ __forceinline__ uint32_t hadd2(uint32_t a, uint32_t b) {
   const __half2 v = __hadd2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -203,30 +213,29 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
     const int page_size = p.cache.page_size;
     const uint8_t* head = p.cache.data + h * p.cache.head_bytes;
     constexpr int CHUNKS = D / 32;    // 16-byte pieces of a row of levels
-    uint4 words[CHUNKS];
-    uint32_t par = 0;
-    long long at = -1;                // the row's page and slot as an offset, -1 where there is none
-    int slot = 0;
-    auto locate = [&](int i) {
+    // A tile ahead: the row's levels and parameters, of the keys and of the values; two ahead: where it lies (an offset to its slot in
+    // the page's key levels, -1 where there is no row)
+    uint4 words[2][CHUNKS];
+    uint32_t par[2] = {0u, 0u};
+    auto locate = [&](int i) -> long long {
       const int j = (tile0 + i) * TILE + key;
-      at = -1;
-      if (i < tiles && j < key_end) {      // key_end <= table_width * page_size
-        const int id = __ldg(trow + (j >> p.cache.page_shift));
-        if ((uint32_t)id < (uint32_t)p.cache.pages) at = id * p.cache.page_stride;
-      }
-      slot = j & (page_size - 1);
+      if (i >= tiles || j >= key_end) return -1;      // key_end <= table_width * page_size
+      const int id = __ldg(trow + (j >> p.cache.page_shift));
+      return (uint32_t)id < (uint32_t)p.cache.pages ? id * p.cache.page_stride : -1;
     };
-    auto fetch = [&](int which) {
+    auto fetch = [&](int which, int i, long long at) {
+      const int slot = ((tile0 + i) * TILE + key) & (page_size - 1);
       const uint8_t* src = head + max(at, 0ll) + (long long)page_size * (D / 2) * which + (long long)slot * (D / 2);
 #pragma unroll
-      for (int c = 0; c < CHUNKS; c++) words[c] = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
-      par = at >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(head + at + (long long)page_size * D + (which * page_size + slot) * 4ll)) : 0u;
+      for (int c = 0; c < CHUNKS; c++)
+        words[which][c] = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+      par[which] = at >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(head + at + (long long)page_size * D + (which * page_size + slot) * 4ll)) : 0u;
     };
-    auto store = [&](uint32_t dst) {
+    auto store = [&](int which, uint32_t dst) {
       const uint32_t row = dst + (uint32_t)key * 128u, x = (uint32_t)(key & 7);
 #pragma unroll
       for (int c = 0; c < CHUNKS; c++) {
-        const uint32_t w[4] = {words[c].x, words[c].y, words[c].z, words[c].w};
+        const uint32_t w[4] = {words[which][c].x, words[which][c].y, words[which][c].z, words[which][c].w};
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           uint32_t o[4];
@@ -236,31 +245,33 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
       }
     };
     bool ok = true;
-    locate(0);
-    fetch(0);
+    long long at = locate(0), at1 = locate(1);
+    fetch(0, 0, at);
+    fetch(1, 0, at);
     for (int j = 0; j < tiles && ok; j++) {
       const int s = j % P::DEPTH;
       const uint32_t ph = (uint32_t)(j / P::DEPTH) & 1u;
       const uint32_t slot_at = base + P::PAR_AT + (uint32_t)(j % SLOTS) * P::SLOT + (uint32_t)(key >> 1) * 16u + (uint32_t)(key & 1) * 4u;
+      const long long at2 = locate(j + 2);
       if (!__all_sync(0xffffffffu, mbar_wait(k_empty(s), ph ^ 1u))) { ok = false; break; }
-      store(base + P::K_AT + s * P::OPERAND);
+      store(0, base + P::K_AT + s * P::OPERAND);
       {
-        const float2 f = unpack2<BF16>(par);
+        const float2 f = unpack2<BF16>(par[0]);
         sts32(slot_at, __float_as_uint(f.x));
         sts32(slot_at + 8, __float_as_uint(fmaf(8.0f, f.x, f.y)));      // the value of level 8
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(k_full(s));
-      fetch(1);
-      const bool live = at >= 0;
+      fetch(0, j + 1, at1);
       if (!__all_sync(0xffffffffu, mbar_wait(v_empty(s), ph ^ 1u))) { ok = false; break; }
-      store(base + P::V_AT + s * P::OPERAND);
+      store(1, base + P::V_AT + s * P::OPERAND);
       {
-        const float2 f = unpack2<BF16>(par);
+        const bool live = at >= 0;
+        const float2 f = unpack2<BF16>(par[1]);
         sts32(slot_at + 1024, __float_as_uint(f.x));
         sts32(slot_at + 1024 + 8, __float_as_uint(fmaf(8.0f, f.x, f.y)));
-        const uint32_t bits = live ? __float_as_uint(fabsf(f.x)) : 0u;
+        const uint32_t bits = __float_as_uint(fabsf(f.x));
         const uint32_t lives = __ballot_sync(0xffffffffu, live);
         const uint32_t most = __reduce_max_sync(0xffffffffu, live && bits < 0x7f800000u && (tile0 + j) * TILE + key >= key_begin ? bits : 0u);
         if (lane == 0) {
@@ -275,8 +286,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
         mbar_arrive(v_full(s));
         mbar_arrive(par_full(j % SLOTS));
       }
-      locate(j + 1);
-      fetch(0);
+      fetch(1, j + 1, at1);
+      at = at1;
+      at1 = at2;
     }
     if (!ok && lane == 0) give_up(1);
   } else if (warp < 12) {
@@ -337,6 +349,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
         bool ok = true;
         for (int j = 0; j < tiles && ok; j++) {
           const uint32_t slot = base + P::PAR_AT + (uint32_t)(j % SLOTS) * P::SLOT;
+          const PairPair* pars = reinterpret_cast<const PairPair*>(smem_raw + (slot - raw));      // keys, then values
           const int key = (tile0 + j) * TILE;
           ok = __all_sync(0xffffffffu, mbar_wait(par_full(j % SLOTS), (uint32_t)(j / SLOTS) & 1u) && mbar_wait(s_full(qt), (uint32_t)j & 1u));
           if (!ok) break;
@@ -355,8 +368,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
           float top = -INFINITY;
 #pragma unroll
           for (int c = 0; c < TILE; c += 2) {
-            Pair step, mid;
-            lds_pairs(slot + c * 8, step, mid);
+            const Pair step = pars[c / 2].step, mid = pars[c / 2].mid;
             const float2 v = unpair(fma2(mul2(pair(sc[c], sc[c + 1]), step), qf2, mul2(mid, ql2)));
             sc[c] = v.x;
             sc[c + 1] = v.y;
@@ -364,7 +376,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
           if (!whole) {
 #pragma unroll
             for (int c = 0; c < TILE; c++)
-              if (!((seen[c >> 5] >> (c & 31)) & 1u)) sc[c] = -INFINITY;
+              sc[c] = (seen[c >> 5] >> (c & 31)) & 1u ? sc[c] : -INFINITY;
           }
 #pragma unroll
           for (int c = 0; c < TILE; c += 2) top = fmaxf(top, fmaxf(sc[c], sc[c + 1]));
@@ -398,31 +410,35 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
             }
           }
           const Pair below2 = pair(below, below), lift2 = pair(lift, lift);
+          auto weigh = [&](auto tag) {      // apart for tiles without a masked key: no branch stands between the elements
+            constexpr bool WHOLE = decltype(tag)::value;
 #pragma unroll
-          for (int c = 0; c < 2; c++) {
-            uint32_t w[32];
+            for (int c = 0; c < 4; c++) {
+              uint32_t w[16];
 #pragma unroll
-            for (int e = 0; e < 32; e++) {
-              const int k = 64 * c + 2 * e;
-              Pair step, mid;
-              lds_pairs(slot + 1024 + k * 8, step, mid);
-              const float2 z = unpair(add2(pair(sc[k], sc[k + 1]), below2));
-              const Pair ex = pair(ex2(z.x), ex2(z.y));
-              l = add2(l, ex);
-              float2 f = unpair(mul2(ex, mul2(step, lift2)));
-              if (whole) {
-                vsum = fma2(ex, mid, vsum);
-              } else {      // a masked place may hold NaN
-                const bool on0 = (seen[k >> 5] >> (k & 31)) & 1u, on1 = (seen[k >> 5] >> ((k + 1) & 31)) & 1u;
-                const float2 md = unpair(mid);
-                f.x = on0 ? f.x : 0.0f;
-                f.y = on1 ? f.y : 0.0f;
-                vsum = fma2(ex, pair(on0 ? md.x : 0.0f, on1 ? md.y : 0.0f), vsum);
+              for (int e = 0; e < 16; e++) {
+                const int k = 32 * c + 2 * e;
+                const Pair step = pars[64 + k / 2].step, mid = pars[64 + k / 2].mid;
+                const float2 z = unpair(add2(pair(sc[k], sc[k + 1]), below2));
+                const Pair ex = pair(ex2(z.x), ex2(z.y));
+                l = add2(l, ex);
+                float2 f = unpair(mul2(ex, mul2(step, lift2)));
+                if (WHOLE) {
+                  vsum = fma2(ex, mid, vsum);
+                } else {      // a masked place may hold NaN
+                  const bool on0 = (seen[c] >> (2 * e)) & 1u, on1 = (seen[c] >> (2 * e + 1)) & 1u;
+                  const float2 md = unpair(mid);
+                  f.x = on0 ? f.x : 0.0f;
+                  f.y = on1 ? f.y : 0.0f;
+                  vsum = fma2(ex, pair(on0 ? md.x : 0.0f, on1 ? md.y : 0.0f), vsum);
+                }
+                w[e] = pack2<false>(f.x, f.y);
               }
-              w[e] = pack2<false>(f.x, f.y);
+              tmem_st16(s_at + 16 * c, w);      // columns of scores that were read
             }
-            tmem_st32(s_at + 32 * c, w);      // columns of scores that were read
-          }
+          };
+          if (whole) weigh(std::true_type());
+          else weigh(std::false_type());
           tmem_st_done();
           tc_fence_before();
           __syncwarp();
