@@ -92,11 +92,11 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+// (no memory clobber: loads of parameters may pass it; the wait below orders it)
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
-      "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
+      "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
 }
 __device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -245,6 +245,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
       }
     };
     bool ok = true;
+    int R = -112;
     long long at = locate(0), at1 = locate(1);
     fetch(0, 0, at);
     fetch(1, 0, at);
@@ -269,16 +270,21 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
       {
         const bool live = at >= 0;
         const float2 f = unpack2<BF16>(par[1]);
-        sts32(slot_at + 1024, __float_as_uint(f.x));
         sts32(slot_at + 1024 + 8, __float_as_uint(fmaf(8.0f, f.x, f.y)));
         const uint32_t bits = __float_as_uint(fabsf(f.x));
         const uint32_t lives = __ballot_sync(0xffffffffu, live);
         const uint32_t most = __reduce_max_sync(0xffffffffu, live && bits < 0x7f800000u && (tile0 + j) * TILE + key >= key_begin ? bits : 0u);
+        // 2^R is above every value step met so far, within fp32's range: the largest of the four warps' keys
+        const uint32_t head_at = base + P::PAR_AT + (uint32_t)(j % SLOTS) * P::SLOT + 2048u;
         if (lane == 0) {
-          const uint32_t head_at = base + P::PAR_AT + (uint32_t)(j % SLOTS) * P::SLOT + 2048u;
           sts32(head_at + warp * 4, lives);
           sts32(head_at + 16 + warp * 4, most);
         }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const uint32_t all = max(max(lds(head_at + 16), lds(head_at + 20)), max(lds(head_at + 24), lds(head_at + 28)));
+        R = max(R, min((int)(all >> 23) - 126, 127));
+        if (key == 0) sts32(head_at + 32, (uint32_t)R);
+        sts32(slot_at + 1024, __float_as_uint(f.x * power2(6 - R)));
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -341,11 +347,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;          // this warp's quarter of the TMEM lanes
         const uint32_t s_at = tmem + lanes + (uint32_t)qt * TILE, o_at = tmem + lanes + P::O_COLUMN + (uint32_t)qt * D;
         const Pair qf2 = pair(qf, qf), ql2 = pair(ql, ql);
-        Pair l = pair(0.0f, 0.0f), vsum = pair(0.0f, 0.0f);
+        Pair l[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)}, vsum[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};      // two chains each
         float below = 0.0f, rise_at = -INFINITY;                    // minus the reference point (0: none yet), and 8 above it
-        int R = -112;
-        uint32_t step_bits = 0;
-        float lift = power2(6 + 112);
+        int R = -112;      // the values' steps come times 2^(6 - R)
         bool ok = true;
         for (int j = 0; j < tiles && ok; j++) {
           const uint32_t slot = base + P::PAR_AT + (uint32_t)(j % SLOTS) * P::SLOT;
@@ -357,15 +361,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
           float sc[TILE];
 #pragma unroll
           for (int c = 0; c < 4; c++) tmem_ld32(s_at + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&sc[32 * c]));
-          uint32_t seen[4], steps = 0;
+          uint32_t seen[4];
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
-            seen[c] = lds(slot + 2048 + 4 * c) & bit_range(begin - key - 32 * c, end - key - 32 * c);
-            steps = max(steps, lds(slot + 2064 + 4 * c));
-          }
+          for (int c = 0; c < 4; c++) seen[c] = lds(slot + 2048 + 4 * c) & bit_range(begin - key - 32 * c, end - key - 32 * c);
+          const int rise = (int)lds(slot + 2080);
           const bool whole = __all_sync(0xffffffffu, (seen[0] & seen[1] & seen[2] & seen[3]) == 0xffffffffu);
           tmem_ld_wait();
-          float top = -INFINITY;
+          float top;
 #pragma unroll
           for (int c = 0; c < TILE; c += 2) {
             const Pair step = pars[c / 2].step, mid = pars[c / 2].mid;
@@ -378,21 +380,29 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
             for (int c = 0; c < TILE; c++)
               sc[c] = (seen[c >> 5] >> (c & 31)) & 1u ? sc[c] : -INFINITY;
           }
+          {
+            float most[8];
 #pragma unroll
-          for (int c = 0; c < TILE; c += 2) top = fmaxf(top, fmaxf(sc[c], sc[c + 1]));
-          if (__any_sync(0xffffffffu, top > rise_at || steps > step_bits)) {
+            for (int c = 0; c < 8; c++) most[c] = fmaxf(sc[c], sc[c + 8]);
+#pragma unroll
+            for (int c = 16; c < TILE; c += 8)
+#pragma unroll
+              for (int e = 0; e < 8; e++) most[e] = fmaxf(most[e], sc[c + e]);
+            top = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), fmaxf(fmaxf(most[4], most[5]), fmaxf(most[6], most[7])));
+          }
+          if (__any_sync(0xffffffffu, top > rise_at || rise != R)) {
             const float m = rise_at == -INFINITY ? -INFINITY : -below;
-            const int rise = max(R, min((int)(steps >> 23) - 126, 127));
             const float shrink = power2(max(R - rise, -127));      // 2^-127 as 0
             R = rise;
-            step_bits = (uint32_t)(127 + R) << 23;
-            lift = power2(6 - R);
             top = fmaxf(top, m);
             const float keep = m == top ? 1.0f : ex2(m - top);
             below = top == -INFINITY ? 0.0f : -top;
             rise_at = top + 8.0f;
-            l = mul2(l, pair(keep, keep));
-            vsum = mul2(vsum, pair(keep, keep));
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+              l[c] = mul2(l[c], pair(keep, keep));
+              vsum[c] = mul2(vsum[c], pair(keep, keep));
+            }
             if (j > 0) {
               ok = __all_sync(0xffffffffu, mbar_wait(o_done(qt), (uint32_t)(j - 1) & 1u));
               if (!ok) break;
@@ -409,7 +419,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
               }
             }
           }
-          const Pair below2 = pair(below, below), lift2 = pair(lift, lift);
+          const Pair below2 = pair(below, below);
           auto weigh = [&](auto tag) {      // apart for tiles without a masked key: no branch stands between the elements
             constexpr bool WHOLE = decltype(tag)::value;
 #pragma unroll
@@ -421,16 +431,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
                 const Pair step = pars[64 + k / 2].step, mid = pars[64 + k / 2].mid;
                 const float2 z = unpair(add2(pair(sc[k], sc[k + 1]), below2));
                 const Pair ex = pair(ex2(z.x), ex2(z.y));
-                l = add2(l, ex);
-                float2 f = unpair(mul2(ex, mul2(step, lift2)));
+                l[e & 1] = add2(l[e & 1], ex);
+                float2 f = unpair(mul2(ex, step));
                 if (WHOLE) {
-                  vsum = fma2(ex, mid, vsum);
+                  vsum[e & 1] = fma2(ex, mid, vsum[e & 1]);
                 } else {      // a masked place may hold NaN
                   const bool on0 = (seen[c] >> (2 * e)) & 1u, on1 = (seen[c] >> (2 * e + 1)) & 1u;
                   const float2 md = unpair(mid);
                   f.x = on0 ? f.x : 0.0f;
                   f.y = on1 ? f.y : 0.0f;
-                  vsum = fma2(ex, pair(on0 ? md.x : 0.0f, on1 ? md.y : 0.0f), vsum);
+                  vsum[e & 1] = fma2(ex, pair(on0 ? md.x : 0.0f, on1 ? md.y : 0.0f), vsum[e & 1]);
                 }
                 w[e] = pack2<false>(f.x, f.y);
               }
@@ -447,7 +457,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
         // ---- the row's output
         float total, mids;
         {
-          const float2 a = unpair(l), c = unpair(vsum);
+          const float2 a = unpair(add2(l[0], l[1])), c = unpair(add2(vsum[0], vsum[1]));
           total = a.x + a.y;
           mids = c.x + c.y;
         }
