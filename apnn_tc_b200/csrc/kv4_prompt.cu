@@ -59,22 +59,34 @@ __device__ __forceinline__ uint32_t elect_lane() {
       : "=r"(lead));
   return lead;
 }
-// A and B from shared memory; descriptors as low words, the high words are constants of the layouts
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
+// Four MMAs of 16 elements of K each; descriptors as low words, the high words are constants of the layouts.  A and B from shared
+// memory (rows of 64 elements: 32 bytes further each time), or A from TMEM (8 columns further) and B sixteen keys further.
+__device__ __forceinline__ void mma_ss4(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
   asm volatile(
-      "{\n\t.reg .pred q, p;\n\t.reg .b64 a, b;\n\t"
-      "setp.ne.b32 q, %6, 0;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "{\n\t.reg .pred q, p, t;\n\t.reg .b64 a, b;\n\t.reg .b32 al, bl;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
       "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(lead)
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t"
+      "add.u32 al, %1, 2;\n\tadd.u32 bl, %2, 2;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, t;\n\t"
+      "add.u32 al, %1, 4;\n\tadd.u32 bl, %2, 4;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, t;\n\t"
+      "add.u32 al, %1, 6;\n\tadd.u32 bl, %2, 6;\n\tmov.b64 a, {al, %3};\n\tmov.b64 b, {bl, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, t;\n\t}" ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(lead)
       : "memory");
 }
-// A from TMEM
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
+__device__ __forceinline__ void mma_ts4(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
   asm volatile(
-      "{\n\t.reg .pred q, p;\n\t.reg .b64 b;\n\t"
-      "setp.ne.b32 q, %6, 0;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "{\n\t.reg .pred q, p, t;\n\t.reg .b64 b;\n\t.reg .b32 al, bl;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
       "mov.b64 b, {%2, %3};\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d), "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(lead)
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t"
+      "add.u32 al, %1, 8;\n\tadd.u32 bl, %2, 128;\n\tmov.b64 b, {bl, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [al], b, %4, t;\n\t"
+      "add.u32 al, %1, 16;\n\tadd.u32 bl, %2, 256;\n\tmov.b64 b, {bl, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [al], b, %4, t;\n\t"
+      "add.u32 al, %1, 24;\n\tadd.u32 bl, %2, 384;\n\tmov.b64 b, {bl, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [al], b, %4, t;\n\t}" ::"r"(d), "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(lead)
       : "memory");
 }
 __device__ __forceinline__ void commit_to(uint32_t bar, uint32_t lead) {
@@ -359,21 +371,25 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
           if (!ok) break;
           tc_fence_after();
           float sc[TILE];
-#pragma unroll
-          for (int c = 0; c < 4; c++) tmem_ld32(s_at + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&sc[32 * c]));
+          tmem_ld32(s_at, *reinterpret_cast<uint32_t(*)[32]>(&sc[0]));
           uint32_t seen[4];
 #pragma unroll
           for (int c = 0; c < 4; c++) seen[c] = lds(slot + 2048 + 4 * c) & bit_range(begin - key - 32 * c, end - key - 32 * c);
           const int rise = (int)lds(slot + 2080);
           const bool whole = __all_sync(0xffffffffu, (seen[0] & seen[1] & seen[2] & seen[3]) == 0xffffffffu);
-          tmem_ld_wait();
           float top;
 #pragma unroll
-          for (int c = 0; c < TILE; c += 2) {
-            const Pair step = pars[c / 2].step, mid = pars[c / 2].mid;
-            const float2 v = unpair(fma2(mul2(pair(sc[c], sc[c + 1]), step), qf2, mul2(mid, ql2)));
-            sc[c] = v.x;
-            sc[c + 1] = v.y;
+          for (int c = 0; c < 4; c++) {      // the next 32 columns are on their way while these are scaled
+            tmem_ld_wait();
+            if (c < 3) tmem_ld32(s_at + 32 * (c + 1), *reinterpret_cast<uint32_t(*)[32]>(&sc[32 * (c + 1)]));
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const int k = 32 * c + e;
+              const Pair step = pars[k / 2].step, mid = pars[k / 2].mid;
+              const float2 v = unpair(fma2(mul2(pair(sc[k], sc[k + 1]), step), qf2, mul2(mid, ql2)));
+              sc[k] = v.x;
+              sc[k + 1] = v.y;
+            }
           }
           if (!whole) {
 #pragma unroll
@@ -519,10 +535,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
       auto issue_qk = [&](int qt, int s) {
         const uint32_t a0 = ((base + qt * P::OPERAND) >> 4) | (1u << 16), b0 = ((base + P::K_AT + s * P::OPERAND) >> 4) | (1u << 16);
 #pragma unroll
-        for (int k = 0; k < D / 16; k++) {
-          const uint32_t step = (uint32_t)(k >> 2) * (16384u >> 4) + (uint32_t)(k & 3) * 2u;
-          mma_ss(tmem + qt * TILE, a0 + step, b0 + step, HI, QK, k != 0 ? 1u : 0u, lead);
-        }
+        for (int k = 0; k < D / 64; k++) mma_ss4(tmem + qt * TILE, a0 + k * (16384u >> 4), b0 + k * (16384u >> 4), HI, QK, k != 0 ? 1u : 0u, lead);
         commit_to(s_full(qt), lead);
       };
       bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0) && mbar_wait(k_full(0), 0));
@@ -540,8 +553,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
           // V: columns of 64 elements 16 KiB apart (the leading offset), eight keys 1024 bytes
           const uint32_t b0 = ((base + P::V_AT + s * P::OPERAND) >> 4) | ((16384u >> 4) << 16);
 #pragma unroll
-          for (int k = 0; k < TILE / 16; k++)
-            mma_ts(tmem + P::O_COLUMN + qt * D, tmem + qt * TILE + 8 * k, b0 + k * (2048u >> 4), HI, WV, (j | k) != 0 ? 1u : 0u, lead);
+          for (int k = 0; k < TILE / 64; k++)
+            mma_ts4(tmem + P::O_COLUMN + qt * D, tmem + qt * TILE + 32 * k, b0 + k * (8192u >> 4), HI, WV, (j | k) != 0 ? 1u : 0u, lead);
           commit_to(o_done(qt), lead);
           if (qt == tiles_q - 1) commit_to(v_empty(s), lead);
           if (j + 1 < tiles) {
