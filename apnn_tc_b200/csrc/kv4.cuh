@@ -47,19 +47,26 @@ __device__ __forceinline__ float round16(float x) {
   return BF16 ? __bfloat162float(__float2bfloat16_rn(x)) : __half2float(__float2half_rn(x));
 }
 
-// The sequence of row t (a whole warp asks): the last b with cu_q[b] <= t, found 32 entries at a time; -1 behind the last row.
+// The sequence of row t (a whole warp asks): the last b with cu_q[b] <= t, -1 behind the last row.  128 entries a round, all of
+// a round's loads and the row count's at once, so up to 128 sequences cost one load's latency.
 __device__ __forceinline__ int sequence_of(const int* cu_q, int sequences, int t, int lane) {
-  if (t >= __ldg(cu_q + sequences)) return -1;
+  const int end = __ldg(cu_q + sequences);
   int lo = 0, n = sequences;   // the answer lies in [lo, lo + n)
-  while (n > 1) {
-    const int step = (n + 31) >> 5;
-    const int at = lo + lane * step;
-    const bool reached = lane * step < n && __ldg(cu_q + at) <= t;
-    const int hit = 31 - __clz(__ballot_sync(0xffffffffu, reached) | 1u);
+  do {
+    const int step = (n + 127) >> 7;
+    int at[4], hits = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int k = (lane + 32 * i) * step;
+      at[i] = k < n ? __ldg(cu_q + lo + k) : 0x7fffffff;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) hits += __popc(__ballot_sync(0xffffffffu, at[i] <= t));
+    const int hit = max(hits - 1, 0);
     lo += hit * step;
     n = min(step, n - hit * step);
-  }
-  return lo;
+  } while (n > 1);
+  return t >= end ? -1 : lo;
 }
 
 // Byte address of head 0 of the page that holds `pos` of sequence b, or null where there is none.

@@ -472,7 +472,7 @@ typedef struct apnn_kv4_append_args {
   const void *q_norm, *k_norm; /* [D] in the cache's type, or null */
   double eps;
   int32_t interleaved;    /* 1: pairs are adjacent elements */
-  const float *rotary;    /* [rotary_rows][rotary_dim]: rotary_dim/2 cosines, then as many sines */
+  const float *rotary;    /* [rotary_rows][rotary_dim]: rotary_dim/2 cosines, then as many sines; 16-byte aligned */
   int32_t rotary_rows;
 } apnn_kv4_append_args;
 #define APNN_KV4_APPEND_ARGS_INIT {(uint32_t)sizeof(apnn_kv4_append_args)}
