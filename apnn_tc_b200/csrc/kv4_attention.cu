@@ -48,15 +48,16 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t* r) {
 //   sum_j p_j v_jd = 2^(R - 6) (sum_j w_j n_jd - 8 sum_j w_j) + sum_j p_j (low_j + 8 step_j)
 // takes the same rounded w in both sums, so the rounding meets levels centred at 8, not 0..15 (half the error of fp16
 // results).  Value words of two keys are put side by side by PRMT to give pairs along the keys.
-// HBM bounds it: (D + 8) bytes per key and head.
+// HBM is the floor, (D + 8) bytes per key and head; the steady state runs at 1.36 times that, bound by instruction issue (585
+// for 32 keys of a warp), and some 17 us go to the start, the meeting of the warps and the joining kernel (64 sequences of up to
+// 16384 keys, 212 MB: 66 us, 3.2 TB/s; one of 65536, 71 MB: 28 us).
 constexpr int FLOW_WARPS = 4;
 constexpr int FLOW_KEYS = 32;                       // per warp and tile
 constexpr int FLOW_TILE = FLOW_WARPS * FLOW_KEYS;   // 128
 constexpr int FLOW_STAGES = 3;
-#ifndef SEGC
-#define SEGC 2
-#endif
-constexpr int FLOW_SEGMENT = SEGC;   // what beginning and ending a (sequence, head) costs, in tiles, when work is shared out
+// What beginning and ending a (sequence, head) costs, in tiles, when work is shared out (64 ragged sequences of 8 heads: 72 us
+// at 1, 66 at 2, 68 at 4).
+constexpr int FLOW_SEGMENT = 2;
 constexpr int UNSPLIT_KEYS = 512;   // tables of at most this many positions: no split, no second launch
 
 template <int D, int NQ>
@@ -311,13 +312,12 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
     const int last_begin = p.causal && p.window > 0 ? max(0, s.pos0 + s.n - p.window) : 0;
     const int first_end = p.causal ? min(s.len, s.pos0 + 1) : s.len;
 
-    float o[F::WV][4][NQ][4], ones[NQ][4];
+    float o[F::WV][4][NQ][4];
     Pair l[NQ], vsum[NQ];
 #pragma unroll
     for (int q = 0; q < NQ; q++)
 #pragma unroll
       for (int c = 0; c < 4; c++) {
-        ones[q][c] = 0.0f;
 #pragma unroll
         for (int w = 0; w < F::WV; w++)
 #pragma unroll
@@ -447,7 +447,6 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
           kept[c] = keep;
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            ones[c >> 1][(c & 1) + 2 * e] *= k;
 #pragma unroll
             for (int w = 0; w < F::WV; w++)
 #pragma unroll
@@ -461,7 +460,14 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
           below[q] = pair(top[2 * q] == -INFINITY ? 0.0f : -top[2 * q], top[2 * q + 1] == -INFINITY ? 0.0f : -top[2 * q + 1]);
         }
       }
-      // ---- weights, and their products with the values
+      // ---- weights, and their products with the values.  Levels are centred at 8 tile by tile: sums of what is all positive
+      // grow far above the result, and the tensor cores truncate (3000 keys, fp16: 4.2e-4 off with one subtraction at the end, so
+      // 2.8e-4, which the roundings of the weights and of the result make up)
+      float eights[NQ][4];
+#pragma unroll
+      for (int q = 0; q < NQ; q++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) eights[q][c] = 0.0f;
       uint32_t wt[2][NQ][2];
 #pragma unroll
       for (int r = 0; r < 4; r++) {
@@ -492,7 +498,7 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
           lds_words<F::WV>(at + F::V_AT + (mt * 16 + (k >> 1) * 8) * F::ROW + (fv ^ (k & 1)) * F::ROW + 4 * F::WV * g, vw[k]);
         }
 #pragma unroll
-        for (int q = 0; q < NQ; q++) mma_f16(ones[q], 0x00010001u, 0x00010001u, 0x00010001u, 0x00010001u, wt[mt][q][0], wt[mt][q][1]);
+        for (int q = 0; q < NQ; q++) mma_f16(eights[q], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, wt[mt][q][0], wt[mt][q][1]);
 #pragma unroll
         for (int w = 0; w < F::WV; w++) {
 #pragma unroll
@@ -508,6 +514,20 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
               mma_f16(o[w][j][q], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, wt[mt][q][0], wt[mt][q][1]);
           }
         }
+      }
+#pragma unroll
+      for (int q = 0; q < NQ; q++) {
+        const Pair down = pair(-eights[q][0], -eights[q][1]), down16 = mul2(down, pair(16.0f, 16.0f));
+#pragma unroll
+        for (int w = 0; w < F::WV; w++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) {      // the second row of a word's pair stands 16 times too high
+            const float2 a = unpair(add2(pair(o[w][j][q][0], o[w][j][q][1]), down)), b = unpair(add2(pair(o[w][j][q][2], o[w][j][q][3]), down16));
+            o[w][j][q][0] = a.x;
+            o[w][j][q][1] = a.y;
+            o[w][j][q][2] = b.x;
+            o[w][j][q][3] = b.y;
+          }
       }
     };
 
@@ -549,14 +569,13 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
           lc += __shfl_xor_sync(0xffffffffu, lc, d);
           vc += __shfl_xor_sync(0xffffffffu, vc, d);
         }
-        const float eight = 8.0f * ones[c >> 1][c & 1];
 #pragma unroll
         for (int w = 0; w < F::WV; w++)
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             float2 v;      // elements 2 j and 2 j + 1 of the word; the second stands 16 times too high
-            v.x = fmaf((o[w][j][c >> 1][c & 1] - eight) * unit, lower, vc);
-            v.y = fmaf((o[w][j][c >> 1][(c & 1) + 2] * 0.0625f - eight) * unit, lower, vc);
+            v.x = fmaf(o[w][j][c >> 1][c & 1] * unit, lower, vc);
+            v.y = fmaf(o[w][j][c >> 1][(c & 1) + 2] * (0.0625f * unit), lower, vc);
             *reinterpret_cast<float2*>(mine + r * (D + 4) + 8 * (F::WV * g + w) + 2 * j) = v;
           }
         if (g == 0) *reinterpret_cast<float2*>(mine + r * (D + 4) + D) = make_float2(reference(c), lc);
