@@ -79,7 +79,7 @@ def linear_planes(x: torch.Tensor, planes: torch.Tensor, scale: torch.Tensor, *,
     bias_ptr = None if bias is None else _vector(index, "bias", bias, N)
     made = out is None
     if made:
-        out = x.new_empty((M, N)) if out_dtype is None or out_dtype is x_dtype else x.new_empty((M, N), dtype=out_dtype)
+        out = x.new_empty(M, N) if out_dtype is None or out_dtype is x_dtype else x.new_empty(M, N, dtype=out_dtype)
     elif out_dtype is not None and out.dtype is not out_dtype:
         raise ValueError("out and out_dtype disagree")
     out_dtype = out.dtype
@@ -153,6 +153,7 @@ class KVCache4:
         self.pages, self.heads, self.page_size, self.head_dim = pages, heads, page_size, head_dim
         stride = data.stride(0) * 4 if pages > 1 else heads * words * 4
         self._index = data.get_device()
+        self._like = torch.empty(0, dtype=dtype, device=data.device)      # what kv4_read's outputs are made from
         self._c = _cabi.Kv4Cache(type=_TYPES[dtype], data=data.data_ptr(), page_stride=stride, pages=pages, heads=heads,
                                  page_size=page_size, head_dim=head_dim)
         self._ptr = ctypes.addressof(self._c)
@@ -210,6 +211,12 @@ def _same(cache: KVCache4, batch: KVBatch) -> int:
     return cache._index
 
 
+def _gain(index: int, name: str, t: torch.Tensor, cache: KVCache4) -> int:
+    if t.dtype is not cache.dtype or t.dim() != 1 or t.numel() != cache.head_dim or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous [{cache.head_dim}] of {cache.dtype}")
+    return _on(index, name, t)
+
+
 def kv4_append(cache: KVCache4, batch: KVBatch, k: torch.Tensor, v: torch.Tensor, *, q: Optional[torch.Tensor] = None,
                q_out: Optional[torch.Tensor] = None, q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
                eps: float = 1e-6, rotary: Optional[torch.Tensor] = None, interleaved: bool = False) -> Optional[torch.Tensor]:
@@ -227,7 +234,7 @@ def kv4_append(cache: KVCache4, batch: KVBatch, k: torch.Tensor, v: torch.Tensor
     if q is not None:
         q_rows, q_heads, q_stride = _rows("q", q, cache)
         if q_out is None:
-            q_out, q_out_stride = q.new_empty((q_rows, q_heads, cache.head_dim)), q_heads * cache.head_dim
+            q_out, q_out_stride = q.new_empty(q_rows, q_heads, cache.head_dim), q_heads * cache.head_dim
         else:
             out_rows, out_heads, q_out_stride = _rows("q_out", q_out, cache)
             if out_rows != q_rows or out_heads != q_heads:
@@ -237,14 +244,8 @@ def kv4_append(cache: KVCache4, batch: KVBatch, k: torch.Tensor, v: torch.Tensor
         raise ValueError("q_out and q_norm need q")
     if v_rows != rows or (q is not None and q_rows != rows):
         raise ValueError("q, k and v disagree on the rows")
-    norms = []
-    for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if t is None:
-            norms.append(0)
-            continue
-        if t.dtype is not cache.dtype or t.dim() != 1 or t.numel() != cache.head_dim or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous [{cache.head_dim}] of {cache.dtype}")
-        norms.append(_on(index, name, t))
+    q_norm_ptr = 0 if q_norm is None else _gain(index, "q_norm", q_norm, cache)
+    k_norm_ptr = 0 if k_norm is None else _gain(index, "k_norm", k_norm, cache)
     rotary_ptr = rotary_rows = rotary_dim = 0
     if rotary is not None:
         if rotary.dtype is not torch.float32 or rotary.dim() != 2 or not rotary.is_contiguous() or rotary.numel() == 0:
@@ -253,7 +254,7 @@ def kv4_append(cache: KVCache4, batch: KVBatch, k: torch.Tensor, v: torch.Tensor
         rotary_ptr = _on(index, "rotary", rotary)
     if rows > 0:
         args = _APPEND(rows, _on(index, "k", k), _on(index, "v", v), k_stride, v_stride, q_ptr, q_out_ptr, q_stride, q_out_stride,
-                       q_heads, rotary_dim, norms[0], norms[1], eps, 1 if interleaved and rotary is not None else 0, rotary_ptr, rotary_rows)
+                       q_heads, rotary_dim, q_norm_ptr, k_norm_ptr, eps, 1 if interleaved and rotary is not None else 0, rotary_ptr, rotary_rows)
         _launch(index, "apnn_kv4_append", _cabi.lib().apnn_kv4_append, cache._ptr, batch._ptr, args)
     return q_out
 
@@ -272,11 +273,12 @@ def kv4_read(cache: KVCache4, batch: KVBatch, rows: Optional[int] = None, *, k_o
         rows = given.shape[0]
     index = _same(cache, batch)
     shape = (rows, cache.heads, cache.head_dim)
-    for name, t in (("k_out", k_out), ("v_out", v_out)):
-        if t is not None and (t.dtype is not cache.dtype or tuple(t.shape) != shape or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous [{rows}, {cache.heads}, {cache.head_dim}] of {cache.dtype}")
+    if given is not None:
+        for name, t in (("k_out", k_out), ("v_out", v_out)):
+            if t is not None and (t.dtype is not cache.dtype or tuple(t.shape) != shape or not t.is_contiguous()):
+                raise ValueError(f"{name} must be a contiguous [{rows}, {cache.heads}, {cache.head_dim}] of {cache.dtype}")
     if k_out is None:
-        k_out = cache.data.new_empty(shape, dtype=cache.dtype)
+        k_out = cache._like.new_empty(*shape)
     if v_out is None:
         v_out = torch.empty_like(k_out)
     if rows > 0:
@@ -303,7 +305,7 @@ def kv4_attention(cache: KVCache4, batch: KVBatch, q: torch.Tensor, *, scale: Op
     rows, q_heads, q_stride = _rows("q", q, cache)
     if out is None:
         out_stride = q_heads * cache.head_dim
-        out = torch.empty_like(q) if q_stride == out_stride else q.new_empty((rows, q_heads, cache.head_dim))
+        out = torch.empty_like(q) if q_stride == out_stride else q.new_empty(rows, q_heads, cache.head_dim)
     else:
         out_rows, out_heads, out_stride = _rows("out", out, cache)
         if out_rows != rows or out_heads != q_heads:
