@@ -36,6 +36,11 @@ constexpr int THREADS = 32 * (PLANES + 1);
 constexpr int COLUMNS = 16;                     // of an accumulator that an epilogue warp takes at a time
 constexpr int SMEM_BYTES = 232448;              // all an SM has: alignment, barriers, planes, stages
 constexpr int MAX_SPLIT = 8;
+// TMEM columns between the two accumulators; a block alone keeps its weight tiles behind them, 32 columns for a stage
+template <int CTAS>
+constexpr int ACC_COLUMNS = CTAS == 2 ? 256 : 128;
+constexpr int TILES_AT = 256, STAGE_COLUMNS = 32;
+static_assert(TILES_AT + MAX_STAGES * STAGE_COLUMNS <= 512, "TMEM");
 
 struct TileParams {
   LinearParams l;
@@ -90,6 +95,28 @@ __device__ __forceinline__ void stage_mmas(uint32_t d_tmem, uint32_t a_lo, uint3
   constexpr uint32_t HI = (1024u >> 4) | (1u << 14) | (2u << 29);      // descriptor: 8-row groups 1024 bytes apart, version, 128-byte swizzle
   if (CTAS == 2) asm volatile(APNN_STAGE_MMAS("2") ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(lead), "r"(HI) : "memory");
   else asm volatile(APNN_STAGE_MMAS("1") ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(lead), "r"(HI) : "memory");
+}
+// The same with the weights in TMEM, 16 elements of K in 8 columns.
+__device__ __forceinline__ void stage_mmas_tmem(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate, uint32_t lead) {
+  constexpr uint32_t HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+  asm volatile(
+      "{\n\t.reg .pred q, p, t;\n\t.reg .b64 b;\n\t.reg .b32 al, bl;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      "mov.b64 b, {%2, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t"
+      "add.u32 al, %1, 8;\n\tadd.u32 bl, %2, 2;\n\tmov.b64 b, {bl, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [al], b, %3, t;\n\t"
+      "add.u32 al, %1, 16;\n\tadd.u32 bl, %2, 4;\n\tmov.b64 b, {bl, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [al], b, %3, t;\n\t"
+      "add.u32 al, %1, 24;\n\tadd.u32 bl, %2, 6;\n\tmov.b64 b, {bl, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [al], b, %3, t;\n\t}" ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(lead), "r"(HI)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+      "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 template <int CTAS>
 __device__ __forceinline__ void commit(uint32_t bar, uint32_t lead) {      // pair: the barrier at this offset in both blocks
@@ -252,7 +279,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
         const int row = tile % p.tiles_x * p.tn + (int)half * rows;
         for (int kb = 0; kb < kbn; kb++, s = (s + 1 == p.stages) ? 0 : s + 1, ph ^= (s == 0) ? 1u : 0u) {
           if (!mbar_wait(empty_bar(s), ph ^ 1u)) { ok = false; break; }
-          const uint32_t dst = stages_at + s * p.stage_bytes + A_BYTES;
+          const uint32_t dst = stages_at + s * p.stage_bytes + (CTAS == 2 ? A_BYTES : 0);
           if (CTAS == 2) {
             if (rank == 0) mbar_expect_tx(full_bar(s), p.tn * BK);     // both blocks' bytes
             tma_load_2d_pair(dst, &map_x, (kb0 + kb) * 64, row, map_to_cta(full_bar(s), 0));
@@ -275,12 +302,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
         const uint32_t acc = tl & 1u;
         if (!__all_sync(0xffffffffu, mbar_wait(tempty_bar(acc), ((tl >> 1) & 1u) ^ 1u))) { ok = false; break; }
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * 256;
+        const uint32_t d_tmem = tmem_base + acc * ACC_COLUMNS<CTAS>;
         for (int kb = 0; kb < kbn; kb++) {
           if (!__all_sync(0xffffffffu, mbar_wait(full_bar(s), ph))) { ok = false; break; }
           tc_fence_after();
-          const uint32_t a_lo = ((stages_at + s * p.stage_bytes) >> 4) | (1u << 16);
-          stage_mmas<CTAS>(d_tmem, a_lo, a_lo + (A_BYTES >> 4), p.idesc, kb != 0 ? 1u : 0u, lead);
+          const uint32_t lo = ((stages_at + s * p.stage_bytes) >> 4) | (1u << 16);
+          if (CTAS == 2) stage_mmas<CTAS>(d_tmem, lo, lo + (A_BYTES >> 4), p.idesc, kb != 0 ? 1u : 0u, lead);
+          else stage_mmas_tmem(d_tmem, tmem_base + TILES_AT + s * STAGE_COLUMNS, lo, p.idesc, kb != 0 ? 1u : 0u, lead);
           commit<CTAS>(empty_bar(s), lead);
           s = s + 1 == p.stages ? 0 : s + 1;
           ph ^= s == 0 ? 1u : 0u;
@@ -320,7 +348,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
   } else if (warp >= FIRST_SPREAD) {
     // ---------------- spread the weights ----------------
     const uint32_t grp = (uint32_t)(warp - FIRST_SPREAD) >> 2;
-    const int r = ((warp - FIRST_SPREAD) & 3) * 32 + lane;
+    const int r = (warp & 3) * 32 + lane;      // a warp reaches a quarter of the TMEM lanes
     const ZeroPoint<BF16> zero(p.l.zero);
     const uint32_t row_at = stages_at + (uint32_t)r * 128u, xr = (uint32_t)(r & 7);
     const uint32_t words_at = planes_at + (uint32_t)r * 64u, wr = (uint32_t)(r >> 1) & 3u;      // 64-byte swizzle
@@ -356,17 +384,25 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
             // after a wait that ran out the warp keeps meeting the named barriers, so that everyone reaches the end
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(s), ph ^ 1u));
             if (ok) {
-              const uint32_t dst = row_at + s * p.stage_bytes;
+              const uint32_t dst = row_at + s * p.stage_bytes, columns = tmem_base + ((uint32_t)(warp & 3) << 21) + TILES_AT + s * STAGE_COLUMNS;
+              if (CTAS == 1) tc_fence_after();
 #pragma unroll
               for (int h = 0; h < 2; h++) {
                 uint32_t w[WB], o[16];
 #pragma unroll
                 for (int b = 0; b < WB; b++) w[b] = half_pair ? (h ? words[b].w : words[b].z) : (h ? words[b].y : words[b].x);
                 spread_in_order<WB, BF16>(w, zero, o);
+                if (CTAS == 1) tmem_st16(columns + 16 * h, o);
+                else
 #pragma unroll
-                for (int q = 0; q < 4; q++) st_v4(dst + (((uint32_t)(4 * h + q) ^ xr) << 4), o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+                  for (int q = 0; q < 4; q++) st_v4(dst + (((uint32_t)(4 * h + q) ^ xr) << 4), o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
               }
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              if (CTAS == 1) {
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+              } else {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              }
               named_arrive(group_barrier(pair, half_pair), GROUP_THREADS + 32);
             } else {
               named_sync(group_barrier(pair, half_pair), GROUP_THREADS + 32);      // no ring holds it back: in step with the others
@@ -394,7 +430,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
       const float scale = live ? __ldg(p.l.scale + n) : 0.0f, bias = live && p.l.bias ? __ldg(p.l.bias + n) : 0.0f;
       if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), (tl >> 1) & 1u))) { ok = false; break; }
       tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * 256;
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * ACC_COLUMNS<CTAS>;
       const long long m0 = (long long)(tile % p.tiles_x) * p.tn;
 #pragma unroll 1
       for (int c = turn * COLUMNS; c < p.tn; c += 2 * COLUMNS) {
@@ -492,7 +528,7 @@ Plan pick_plan(int M, int N, int kblocks, int sms) {
   Plan best = {1, 32, 1};
   double least = 1e30;
   for (int ctas = 1; ctas <= 2; ctas++)
-    for (int tn = ctas == 2 ? 64 : 32; tn <= 256; tn *= 2)
+    for (int tn = ctas == 2 ? 64 : 32; tn <= 128 * ctas; tn *= 2)
       for (int split = 1; split <= (ctas == 2 ? 1 : MAX_SPLIT) && 2 * split <= kblocks; split *= 2) {
         if (tn / split < 4) continue;
         const long long tiles = (long long)((M + tn - 1) / tn) * ((N + ROWS * ctas - 1) / (ROWS * ctas));
@@ -576,7 +612,7 @@ apnn_status linear_tile(cudaStream_t s, const LinearParams& l, bool bf16) {
   if (fn(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<uint32_t*>(l.W), wdims, wstrides, wbox, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
          CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return cuda_fail(cudaErrorInvalidValue, "cuTensorMapEncodeTiled");
-  p.stage_bytes = A_BYTES + plan.tn / plan.ctas * BK;
+  p.stage_bytes = (plan.ctas == 2 ? A_BYTES : 0) + plan.tn / plan.ctas * BK;
   p.stages = (SMEM_BYTES - 2048 - CHUNKS * l.wbits * PLANE_BYTES) / p.stage_bytes;
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
   const long long tiles = (long long)p.tiles_x * p.tiles_w;
