@@ -5,13 +5,16 @@
 // stores 32 neighbouring columns of one row of the output.  X comes by TMA (128-byte swizzle, zeros beyond its edges), and so do the
 // planes, 512 elements of K of every row at a time into a ring of two (loads of 8 bytes from 128 rows took as many L1
 // cycles as a stage's MMAs: 0.74 against 0.43 ms at 4096 x 16384 x 4096, 4 bits).  The weights never exist as 16-bit floats in
-// memory: eight warps spread the planes to level - zero (spread.cuh) and write the swizzled operand tile themselves, two groups
-// of four warps on alternate pairs of stages of 64 elements of K; a warp that loads nothing meets each group on a named barrier and
-// publishes the stage.  Roles: warp 0 TMA of X, 1 MMA, 2-9 epilogue (two to a quarter of the TMEM
-// lanes), 10-17 spread, 18 publish, 19 TMA of the planes; every wait is bounded.
+// memory: groups of four warps spread the planes to level - zero (spread.cuh) and write the operand tile themselves, two stages of 64
+// elements of K at a time, the groups in turn; a block alone keeps these tiles in TMEM, a pair swizzled in shared memory (its
+// accumulators fill TMEM).  A warp that loads nothing meets each group on a named barrier and publishes the stages.  Roles: warp 0 TMA
+// of X, 1 MMA, 2-9 epilogue (two to a quarter of the TMEM lanes), from 10 on spread, then publish and TMA of the planes; every wait
+// is bounded.
 //
-// What bounds a stage of 64 elements: shared memory, 32 KiB in and out for the weight tile and 256 bytes for each row of X a block
-// holds, at 128 bytes a clock -- 512 clk for the pair's 256 x 256 tile, as long as its MMAs.  Spreading takes about 250.
+// What bounds a stage: of the pair's 256 x 256 tile, shared memory, 32 KiB in and out for the weight tile and 256 bytes for each row
+// of X a block holds, at 128 bytes a clock, 512 clk and as long as its MMAs (4096 x 16384 x 4096, 4 bits: 352 us, 1.56 PFLOP/s).  Of a
+// block alone about 0.2 us whatever its width: 240 clk of the integer pipe at 4 bits, and 215 clk for the one warp that waits for a
+// stage, issues its MMAs and commits them (16 x 16384 x 4096, 2 bits: 16 us; with the tiles in shared memory 18.8).
 //
 // Few tiles and a long K: the blocks of a cluster share a tile's K, and each finishes a slice of the tile's rows of X from the others'
 // sums in its shared memory, added in the order of the ranks.
@@ -30,9 +33,15 @@ constexpr int A_BYTES = ROWS * BK;
 constexpr int CHUNK = 8;                        // stages of 64 elements that one load of the planes covers
 constexpr int PLANE_BYTES = ROWS * CHUNK * 8;   // of one plane
 constexpr int CHUNKS = 2;
-constexpr int EPI_WARPS = 8, SPREAD_WARPS = 8, GROUP_THREADS = 128;
-constexpr int FIRST_SPREAD = 2 + EPI_WARPS, PUBLISH = FIRST_SPREAD + SPREAD_WARPS, PLANES = PUBLISH + 1;      // warps
-constexpr int THREADS = 32 * (PLANES + 1);
+constexpr int EPI_WARPS = 8, FIRST_SPREAD = 2 + EPI_WARPS, GROUP_THREADS = 128;
+// Groups of spreading warps.  A group that has spread a pair of stages waits for the slots of its next pair, 2 GROUPS stages on: with
+// no fewer slots in the ring the use before the one it waits for is over by then, so the parity names one use only.  (128 x 4096 x 4096, 4
+// bits, a block alone: 18.3 us with two groups, 17.6 with three, 18.1 with four.)
+template <int CTAS>
+struct Roles {
+  static constexpr int GROUPS = CTAS == 2 ? 2 : 3, SPREAD_WARPS = 4 * GROUPS;
+  static constexpr int PUBLISH = FIRST_SPREAD + SPREAD_WARPS, PLANES = PUBLISH + 1, THREADS = 32 * (PLANES + 1);
+};
 constexpr int COLUMNS = 16;                     // of an accumulator that an epilogue warp takes at a time
 constexpr int SMEM_BYTES = 232448;              // all an SM has: alignment, barriers, planes, stages
 constexpr int MAX_SPLIT = 8;
@@ -139,6 +148,30 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "memory");
 }
 
+// One lane's copy of a box into shared memory, announced on `bar` (announce: with its bytes), by a whole warp with uniform operands
+// for the same reason: from a one-lane branch a copy took 350 clk to issue, more than spreading a stage.
+template <int CTAS>
+__device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar, uint32_t lead) {
+  if (CTAS == 2)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar), "r"(lead)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(dst), "l"(map), "r"(x),
+        "r"(y), "r"(bar), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes), "r"(lead)
+      : "memory");
+}
+
 // 16 columns of the epilogue: v[j] is the sum of weight row n (a lane each; live: there is one) with row m0 + j of X.  wide: the
 // output may be stored in pairs of columns.
 template <bool BF16>
@@ -206,12 +239,16 @@ __device__ __forceinline__ void finish_columns(const LinearParams& p, float (&v)
     if (live && j < count) *o = (uint16_t)pack2<BF16>(v[j], 0.0f);
 }
 
-// The named barrier on which the group of pair `pairs` hands over its first or second stage.  Four in turn for each group: it comes
-// back to one only after the ring has let it reuse a slot, so after the publishing warp left it.
-__device__ __forceinline__ int group_barrier(uint32_t pairs, int second) { return 1 + (int)((pairs & 1u) * 4 + ((pairs >> 1) & 1u) * 2) + second; }
+// The named barrier on which a group hands over its pair of stages.  Two in turn for each group: it comes back to one only after the
+// ring has let it reuse a slot, so after the publishing warp left it (4 GROUPS stages are more than a ring has).
+template <int GROUPS>
+__device__ __forceinline__ int group_barrier(uint32_t pair) { return 1 + (int)(pair % GROUPS * 2 + (pair / GROUPS & 1u)); }
+static_assert(4 * Roles<1>::GROUPS >= MAX_STAGES && 4 * Roles<2>::GROUPS >= MAX_STAGES && 2 * Roles<1>::GROUPS < 16, "named barriers");
 
 template <int WB, bool BF16, int CTAS>
-__global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const TileParams p) {
+__global__ void __launch_bounds__(Roles<CTAS>::THREADS, 1)
+    linear_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const TileParams p) {
+  constexpr int GROUPS = Roles<CTAS>::GROUPS, SPREAD_WARPS = Roles<CTAS>::SPREAD_WARPS, PUBLISH = Roles<CTAS>::PUBLISH, PLANES = Roles<CTAS>::PLANES;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -270,27 +307,23 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
 
   if (warp == 0) {
     // ---------------- X by TMA ----------------
-    if (lane == 0) {
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      const int rows = p.tn / CTAS;
-      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
-        const int row = tile % p.tiles_x * p.tn + (int)half * rows;
-        for (int kb = 0; kb < kbn; kb++, s = (s + 1 == p.stages) ? 0 : s + 1, ph ^= (s == 0) ? 1u : 0u) {
-          if (!mbar_wait(empty_bar(s), ph ^ 1u)) { ok = false; break; }
-          const uint32_t dst = stages_at + s * p.stage_bytes + (CTAS == 2 ? A_BYTES : 0);
-          if (CTAS == 2) {
-            if (rank == 0) mbar_expect_tx(full_bar(s), p.tn * BK);     // both blocks' bytes
-            tma_load_2d_pair(dst, &map_x, (kb0 + kb) * 64, row, map_to_cta(full_bar(s), 0));
-          } else {
-            mbar_expect_tx(full_bar(s), p.tn * BK);
-            tma_load_2d(dst, &map_x, (kb0 + kb) * 64, row, full_bar(s));
-          }
-        }
+    const uint32_t lead = elect_lane();
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    const int rows = p.tn / CTAS;
+    for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
+      const int row = tile % p.tiles_x * p.tn + (int)half * rows;
+      for (int kb = 0; kb < kbn; kb++) {
+        if (!__all_sync(0xffffffffu, mbar_wait(empty_bar(s), ph ^ 1u))) { ok = false; break; }
+        const uint32_t dst = stages_at + s * p.stage_bytes + (CTAS == 2 ? A_BYTES : 0);
+        if (CTAS == 1 || rank == 0) expect_bytes(full_bar(s), p.tn * BK, lead);     // pair: both blocks' bytes
+        copy_box<CTAS>(dst, &map_x, (kb0 + kb) * 64, row, CTAS == 2 ? map_to_cta(full_bar(s), 0) : full_bar(s), lead);
+        s = s + 1 == p.stages ? 0 : s + 1;
+        ph ^= s == 0 ? 1u : 0u;
       }
-      if (!ok) give_up(1);
     }
+    if (!ok && lane == 0) give_up(1);
   } else if (warp == 1) {
     // ---------------- MMA ----------------
     if (half == 0) {
@@ -319,31 +352,33 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
     }
   } else if (warp == PLANES) {
     // ---------------- planes by TMA, a chunk ahead of the spreading ----------------
-    if (lane == 0) {
-      uint32_t chunk = 0;       // over all tiles
-      bool ok = true;
-      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
-        const int row = (tile / p.tiles_x * CTAS + (int)half) * ROWS;
-        for (int kb = 0; kb < kbn; kb += CHUNK, chunk++) {
-          const uint32_t c = chunk % CHUNKS;
-          if (!mbar_wait(wempty_bar(c), ((chunk / CHUNKS) & 1u) ^ 1u)) { ok = false; break; }
-          mbar_expect_tx(wfull_bar(c), WB * PLANE_BYTES);
-          // rows behind N run into the next plane, and behind the last one they are zeros: their sums are not stored
-          for (int b = 0; b < WB; b++)
-            tma_load_2d(planes_at + (c * WB + b) * PLANE_BYTES, &map_w, 2 * (kb0 + kb), b * p.l.N + row, wfull_bar(c));
-        }
+    const uint32_t lead = elect_lane();
+    uint32_t chunk = 0;       // over all tiles
+    bool ok = true;
+    for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
+      const int row = (tile / p.tiles_x * CTAS + (int)half) * ROWS;
+      for (int kb = 0; kb < kbn; kb += CHUNK, chunk++) {
+        const uint32_t c = chunk % CHUNKS;
+        if (!__all_sync(0xffffffffu, mbar_wait(wempty_bar(c), ((chunk / CHUNKS) & 1u) ^ 1u))) { ok = false; break; }
+        expect_bytes(wfull_bar(c), WB * PLANE_BYTES, lead);
+        // rows behind N run into the next plane, and behind the last one they are zeros: their sums are not stored
+#pragma unroll
+        for (int b = 0; b < WB; b++)
+          copy_box<1>(planes_at + (c * WB + b) * PLANE_BYTES, &map_w, 2 * (kb0 + kb), b * p.l.N + row, wfull_bar(c), lead);
       }
-      if (!ok) give_up(6);
     }
+    if (!ok && lane == 0) give_up(6);
   } else if (warp == PUBLISH) {
     // ---------------- publish spread stages ----------------
     const uint32_t full0 = CTAS == 2 ? map_to_cta(full_bar(0), 0) : map_to_cta(full_bar(0), rank);
     int s = 0;
-    uint32_t pairs = 0;       // pairs of stages: the groups take them in turn
+    uint32_t pair = 0;        // of stages: the groups take them in turn
     for (int tile = first_tile; tile < num_tiles; tile += tile_step)
-      for (int kb = 0; kb < kbn; kb++, pairs += (uint32_t)((kb & 1) == 0), s = (s + 1 == p.stages) ? 0 : s + 1) {
-        named_sync(group_barrier(pairs, kb & 1), GROUP_THREADS + 32);
-        if (lane == 0) arrive_remote(full0 + 8u * s);
+      for (int kb = 0; kb < kbn; kb += 2, pair++) {
+        named_sync(group_barrier<GROUPS>(pair), GROUP_THREADS + 32);
+#pragma unroll
+        for (int i = 0; i < 2; i++, s = (s + 1 == p.stages) ? 0 : s + 1)
+          if (lane == 0) arrive_remote(full0 + 8u * s);
       }
   } else if (warp >= FIRST_SPREAD) {
     // ---------------- spread the weights ----------------
@@ -352,69 +387,64 @@ __global__ void __launch_bounds__(THREADS, 1) linear_tile_kernel(const __grid_co
     const ZeroPoint<BF16> zero(p.l.zero);
     const uint32_t row_at = stages_at + (uint32_t)r * 128u, xr = (uint32_t)(r & 7);
     const uint32_t words_at = planes_at + (uint32_t)r * 64u, wr = (uint32_t)(r >> 1) & 3u;      // 64-byte swizzle
-    int s = 0;
-    uint32_t ph = 0, pairs = 0, chunk = 0;
-    bool ok = true;
-    auto advance = [&](int n) {      // n <= 2 < stages
-      s += n;
-      if (s >= p.stages) {
-        s -= p.stages;
-        ph ^= 1u;
-      }
+    struct Slot { int s; uint32_t ph; } at = {0, 0};      // of the chunk's first stage
+    auto after = [&](Slot x, int n) {
+      for (x.s += n; x.s >= p.stages; x.s -= p.stages) x.ph ^= 1u;
+      return x;
     };
+    uint32_t pair = 0, chunk = 0;      // of the chunk's first pair
+    bool ok = true;
     for (int tile = first_tile; tile < num_tiles; tile += tile_step) {
-      // This group's pairs of the tile: every other one, two of a whole chunk.  (A loop over all pairs that skips the other
-      // group's spread them all the same: the compiler works ahead of the branch.)
-      const int first = (int)((pairs & 1u) ^ grp) * 2;
       for (int kc = 0; kc < kbn; kc += CHUNK, chunk++) {
         const uint32_t c = chunk % CHUNKS;
-        const int end = min(kc + CHUNK, kbn);
+        const int count = min(CHUNK, kbn - kc) / 2;
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(wfull_bar(c), (chunk / CHUNKS) & 1u));
-        if (first) advance(2);
-        for (int kb = kc + first; kb < end; kb += 4) {
+        // This group's pairs of the chunk.  (A loop over all pairs that skips the others' spread them all the same: the compiler
+        // works ahead of the branch.)
+        for (int i = (int)((grp + GROUPS - pair % GROUPS) % GROUPS); i < count; i += GROUPS) {
           uint4 words[WB];
 #pragma unroll
           for (int b = 0; b < WB; b++) {
-            const uint32_t at = words_at + (c * WB + b) * PLANE_BYTES + ((((uint32_t)(kb - kc) >> 1) ^ wr) << 4);
-            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(words[b].x), "=r"(words[b].y), "=r"(words[b].z), "=r"(words[b].w) : "r"(at));
+            const uint32_t from = words_at + (c * WB + b) * PLANE_BYTES + (((uint32_t)i ^ wr) << 4);
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(words[b].x), "=r"(words[b].y), "=r"(words[b].z), "=r"(words[b].w) : "r"(from));
           }
-          const uint32_t pair = pairs + ((uint32_t)kb >> 1);
+          const Slot one = after(at, 2 * i), two = after(one, 1);
+          // the second stage's slot is freed after the first's.  After a wait that ran out the warp keeps meeting the named
+          // barriers, so that everyone reaches the end
+          if (ok) ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(two.s), two.ph ^ 1u));
+          if (ok) {
+            if (CTAS == 1) tc_fence_after();
 #pragma unroll
-          for (int half_pair = 0; half_pair < 2; half_pair++) {
-            // after a wait that ran out the warp keeps meeting the named barriers, so that everyone reaches the end
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(empty_bar(s), ph ^ 1u));
-            if (ok) {
-              const uint32_t dst = row_at + s * p.stage_bytes, columns = tmem_base + ((uint32_t)(warp & 3) << 21) + TILES_AT + s * STAGE_COLUMNS;
-              if (CTAS == 1) tc_fence_after();
+            for (int h = 0; h < 4; h++) {
+              const int s = h < 2 ? one.s : two.s;
+              uint32_t w[WB], o[16];
 #pragma unroll
-              for (int h = 0; h < 2; h++) {
-                uint32_t w[WB], o[16];
-#pragma unroll
-                for (int b = 0; b < WB; b++) w[b] = half_pair ? (h ? words[b].w : words[b].z) : (h ? words[b].y : words[b].x);
-                spread_in_order<WB, BF16>(w, zero, o);
-                if (CTAS == 1) tmem_st16(columns + 16 * h, o);
-                else
-#pragma unroll
-                  for (int q = 0; q < 4; q++) st_v4(dst + (((uint32_t)(4 * h + q) ^ xr) << 4), o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
-              }
+              for (int b = 0; b < WB; b++) w[b] = h == 0 ? words[b].x : h == 1 ? words[b].y : h == 2 ? words[b].z : words[b].w;
+              spread_in_order<WB, BF16>(w, zero, o);
               if (CTAS == 1) {
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                tc_fence_before();
+                tmem_st16(tmem_base + ((uint32_t)(warp & 3) << 21) + TILES_AT + s * STAGE_COLUMNS + 16 * (h & 1), o);
               } else {
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                  st_v4(row_at + s * p.stage_bytes + (((uint32_t)(4 * (h & 1) + q) ^ xr) << 4), o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
               }
-              named_arrive(group_barrier(pair, half_pair), GROUP_THREADS + 32);
-            } else {
-              named_sync(group_barrier(pair, half_pair), GROUP_THREADS + 32);      // no ring holds it back: in step with the others
             }
-            advance(1);
+            if (CTAS == 1) {
+              asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+              tc_fence_before();
+            } else {
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
+            named_arrive(group_barrier<GROUPS>(pair + (uint32_t)i), GROUP_THREADS + 32);
+          } else {
+            named_sync(group_barrier<GROUPS>(pair + (uint32_t)i), GROUP_THREADS + 32);      // no ring holds it back: in step with the others
           }
-          if (kb + 2 < end) advance(2);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(wempty_bar(c));
+        at = after(at, 2 * count);
+        pair += (uint32_t)count;
       }
-      pairs += (uint32_t)(kbn >> 1);
     }
     if (!ok && lane == 0) give_up(4);
   } else if (CTAS == 2 || p.split == 1) {
@@ -533,9 +563,9 @@ Plan pick_plan(int M, int N, int kblocks, int sms) {
         if (tn / split < 4) continue;
         const long long tiles = (long long)((M + tn - 1) / tn) * ((N + ROWS * ctas - 1) / (ROWS * ctas));
         // a cluster finds its blocks within one group of SMs: the driver knows how many fit
-        const int slots = split > 1 ? cluster_capacity(reinterpret_cast<const void*>(linear_tile_kernel<4, true, 1>), THREADS, SMEM_BYTES, split) : sms / ctas;
+        const int slots = split > 1 ? cluster_capacity(reinterpret_cast<const void*>(linear_tile_kernel<4, true, 1>), Roles<1>::THREADS, SMEM_BYTES, split) : sms / ctas;
         if (slots < 1) continue;
-        const double stage = ctas == 1 ? (tn == 32 ? 0.255 : tn == 64 ? 0.265 : tn == 128 ? 0.295 : 0.43) : (tn == 64 ? 0.265 : tn == 128 ? 0.285 : 0.375);
+        const double stage = ctas == 1 ? (tn <= 64 ? 0.2 : 0.215) : (tn == 64 ? 0.265 : tn == 128 ? 0.285 : 0.375);
         const double epilogue = (ctas == 1 ? 0.8 : 1.4) + 0.012 * tn;
         const double stages = stage * (double)((kblocks / 2 + split - 1) / split * 2);
         const double exchange = split > 1 ? 1.5 + 0.1 * (tn / split) + 0.015 * tn : 0.0;
@@ -557,7 +587,7 @@ apnn_status launch(cudaStream_t s, const CUtensorMap& map, const CUtensorMap& ma
   if (e != cudaSuccess) return cuda_fail(e, "linear_tile_kernel shared memory");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks, 1, 1);
-  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.blockDim = dim3(Roles<CTAS>::THREADS, 1, 1);
   cfg.dynamicSmemBytes = SMEM_BYTES;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -615,6 +645,7 @@ apnn_status linear_tile(cudaStream_t s, const LinearParams& l, bool bf16) {
   p.stage_bytes = (plan.ctas == 2 ? A_BYTES : 0) + plan.tn / plan.ctas * BK;
   p.stages = (SMEM_BYTES - 2048 - CHUNKS * l.wbits * PLANE_BYTES) / p.stage_bytes;
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+  if (p.stages < 2 * (plan.ctas == 2 ? Roles<2>::GROUPS : Roles<1>::GROUPS)) return APNN_ERR_UNSUPPORTED;      // not reached: 5 and 8 at least
   const long long tiles = (long long)p.tiles_x * p.tiles_w;
   const int slots = sms / plan.ctas;
   const int blocks = plan.split > 1 ? (int)tiles * plan.split : (int)(tiles < slots ? tiles : slots) * plan.ctas;
