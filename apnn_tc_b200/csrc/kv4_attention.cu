@@ -759,6 +759,13 @@ apnn_status launch_flow_rows(cudaStream_t stream, const FlowPlan& f, const FlowP
   return APNN_ERR_UNSUPPORTED;     // not reached: such rows take the other kernel
 }
 
+// What 32-bit positions and shares hold: tables of up to 2^30 positions, and tiles of all sequences and heads below 2^31.
+constexpr int MOST_POSITIONS = 1 << 30;
+bool too_long(const apnn_kv4_cache* c, const apnn_kv4_batch* b) {
+  const long long keys = (long long)b->table_width * c->page_size;
+  return keys > MOST_POSITIONS || (long long)b->sequences * c->heads * ((keys + FLOW_TILE - 1) / FLOW_TILE + FLOW_SEGMENT) > 0x7fffffffll;
+}
+
 }  // namespace
 }  // namespace apnn
 
@@ -769,7 +776,9 @@ extern "C" {
 size_t apnn_kv4_attention_workspace_bytes(const apnn_kv4_cache* cache, const apnn_kv4_batch* batch, int q_heads) {
   Kv4View view = {};
   Kv4Batch geo = {};
-  if (kv4_view(cache, &view) != APNN_OK || kv4_batch(batch, 1, &geo) != APNN_OK || q_heads <= 0 || q_heads % cache->heads != 0) return 0;
+  if (kv4_view(cache, &view) != APNN_OK || kv4_batch(batch, 1, &geo) != APNN_OK || q_heads <= 0 || q_heads % cache->heads != 0 ||
+      too_long(cache, batch))
+    return 0;
   const int group = q_heads / cache->heads;
   if ((long long)batch->max_q * group > largest_rows(cache->head_dim)) return kv4_prompt_workspace_bytes(cache, batch, group);
   return flow_plan(cache, batch, group).bytes;
@@ -783,6 +792,7 @@ apnn_status apnn_kv4_attention(void* stream, const apnn_kv4_cache* cache, const 
   if (st == APNN_OK) st = kv4_batch(batch, a->rows, &p.batch);
   if (st != APNN_OK) return st;
   if (a->q_heads <= 0 || a->q_heads % cache->heads != 0) return APNN_ERR_INVALID_ARG;
+  if (too_long(cache, batch)) return APNN_ERR_UNSUPPORTED;
   if ((a->causal != 0 && a->causal != 1) || a->window < 0 || (a->window > 0 && !a->causal)) return APNN_ERR_INVALID_ARG;
   if (!std::isfinite(a->scale)) return APNN_ERR_INVALID_ARG;
   const long long row = (long long)a->q_heads * cache->head_dim;
@@ -799,7 +809,7 @@ apnn_status apnn_kv4_attention(void* stream, const apnn_kv4_cache* cache, const 
   p.q_heads = a->q_heads;
   p.group = a->q_heads / cache->heads;
   p.causal = a->causal;
-  p.window = a->window;
+  p.window = a->window < MOST_POSITIONS ? a->window : MOST_POSITIONS;      // as far as any row sees
   p.scale = a->scale;
   p.status_flag = static_cast<int*>(workspace);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

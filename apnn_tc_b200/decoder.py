@@ -321,7 +321,10 @@ def kv4_attention(cache: KVCache4, batch: KVBatch, q: torch.Tensor, *, scale: Op
     if window and not causal:
         raise ValueError("a window needs causal")
     q_ptr = _on(index, "q", q)
-    if workspace is None:
+    if workspace is not None:
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+    else:
         workspace = torch.empty(max(1, kv4_attention_workspace_bytes(cache, batch, q_heads)), dtype=torch.uint8, device=q.device)
     if rows > 0:
         args = _ATTENTION(rows, q_ptr, _on(index, "out", out), lse_ptr, q_stride, out_stride, q_heads, 1 if causal else 0, window,

@@ -488,6 +488,7 @@ apnn_status apnn_kv4_read(void *stream, const apnn_kv4_cache *cache, const apnn_
  *   Out = softmax(scale * q k^T) v;   lse = ln sum exp(scale * q k^T);   a row that sees no key: Out 0, lse -infinity.
  * Products of levels are exact, softmax statistics and sums are held in 32 bits, the weights of the values in fp16
  * relative to the row's maximum; one rounding at the store.  Results do not depend on timing (no atomics on values).
+ * At most 2^30 positions in a table row and 2^31 tiles of 128 of them over all sequences and heads (else APNN_ERR_UNSUPPORTED).
  * workspace: apnn_kv4_attention_workspace_bytes of device memory, 16-byte aligned, for one call at a time. */
 typedef struct apnn_kv4_attention_args {
   uint32_t struct_size;

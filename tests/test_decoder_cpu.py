@@ -30,6 +30,7 @@ def linear(wbits=4, W=P, X=P, Out=P, M=4, N=64, K=128, flag=None, **kw):
     (INVALID, dict(zero=-0.5)), (INVALID, dict(zero=15.5)), (INVALID, dict(zero=float("nan"))), (INVALID, dict(ldx=120)),
     (INVALID, dict(ldo=63)), (INVALID, dict(residual=P, ldr=63)),
     (UNSUPPORTED, dict(wbits=0)), (UNSUPPORTED, dict(wbits=5)), (UNSUPPORTED, dict(wbits=8)),
+    (UNSUPPORTED, dict(N=1 << 30, ldo=1 << 30)),
     (ALIGNMENT, dict(W=P + 4)), (ALIGNMENT, dict(X=P + 2)), (ALIGNMENT, dict(ldx=132)), (ALIGNMENT, dict(Out=P + 1)),
     (ALIGNMENT, dict(out_type=2, Out=P + 2)), (ALIGNMENT, dict(scale=P + 2)), (ALIGNMENT, dict(flag=P + 1)),
 ])
@@ -90,6 +91,7 @@ def test_descriptors_of_another_size_are_refused():
     (INVALID, dict(rotary_dim=32)), (INVALID, dict(rotary=P, rotary_rows=0, rotary_dim=32)), (INVALID, dict(rotary=P, rotary_rows=4, rotary_dim=80)),
     (UNSUPPORTED, dict(rotary=P, rotary_rows=4, rotary_dim=24)), (INVALID, dict(eps=-1.0)), (INVALID, dict(eps=float("nan"))),
     (INVALID, dict(interleaved=2)), (ALIGNMENT, dict(k=P + 2)), (ALIGNMENT, dict(v_stride=132)), (ALIGNMENT, dict(k_norm=P + 8)),
+    (ALIGNMENT, dict(rotary=P + 8, rotary_rows=4, rotary_dim=32)),
 ])
 def test_append_refuses(status, kw):
     d = dict(rows=2, k=P, v=P, k_stride=128, v_stride=128, eps=1e-6)
@@ -108,6 +110,16 @@ def test_attention_refuses(status, kw):
     d.update(kw)
     c, b, a = cache(), batch(), _cabi.Kv4AttentionArgs(**d)
     assert _cabi.lib().apnn_kv4_attention(None, ctypes.addressof(c), ctypes.addressof(b), ctypes.addressof(a), P, 1 << 40) == status
+
+
+@pytest.mark.parametrize("kw", [dict(table_width=(1 << 30) // 8 + 1), dict(sequences=1 << 12, table_width=1 << 24)])
+def test_attention_refuses_what_32_bits_do_not_count(kw):
+    """Tables of more than 2^30 positions, or more than 2^31 tiles of 128 positions over all sequences and heads (pages of 16, 2 heads)."""
+    c, b = cache(page_size=8 if len(kw) == 1 else 16, page_stride=1 << 12), batch(table_stride=1 << 30, **kw)
+    a = _cabi.Kv4AttentionArgs(rows=2, q=P, out=P, q_stride=256, out_stride=256, q_heads=4, causal=1, scale=0.1)
+    L = _cabi.lib()
+    assert L.apnn_kv4_attention(None, ctypes.addressof(c), ctypes.addressof(b), ctypes.addressof(a), P, 1 << 40) == UNSUPPORTED
+    assert L.apnn_kv4_attention_workspace_bytes(ctypes.addressof(c), ctypes.addressof(b), 4) == 0
 
 
 def test_attention_needs_its_workspace():

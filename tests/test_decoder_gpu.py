@@ -287,6 +287,15 @@ def test_append_odd_rows(cuda_device, dtype):
     check_append(Setup(1, [12], [20], 2, 128, 16, dtype), 4, True, 64, False, k=k, v=v, rows=18)
 
 
+@pytest.mark.parametrize("Hq,heads,D,most,B,norm,rot", [(1, 1, 64, 5, 2500, True, 64), (3, 2, 128, 40, 260, False, 64), (1, 1, 64, 4, 30000, False, 0), (4, 3, 256, 900, 9, True, 256)])
+def test_append_rows_that_share_a_block(cuda_device, Hq, heads, D, most, B, norm, rot):
+    """So many rows that a block takes several, up to 32, across the borders of sequences and past the last one."""
+    rng = np.random.default_rng(B)
+    lens_q = rng.integers(0, most + 1, size=B)
+    s = Setup(B, lens_q, lens_q + rng.integers(0, 12, size=B), heads, D, 16, BF, spare_rows=70)
+    check_append(s, Hq, norm, rot, False, rows=most + 12)
+
+
 def test_append_bad_pages_and_positions(cuda_device):
     """Page numbers outside the cache, lengths shorter than the rows, lengths behind the table: those rows are not written."""
     s = Setup(4, [6, 9, 4], [40, 5, 60], 2, 64, 16, BF, wide=3)
@@ -348,6 +357,12 @@ def test_attention_few_tokens(cuda_device, D, page, dtype, window):
 @pytest.mark.parametrize("window", [0, 50])
 def test_attention_prompts(cuda_device, D, page, dtype, window):
     check_attention(Setup(D + 1, [70, 1, 131], [70, 100, 260], 2, D, page, dtype, spare_rows=1), 4, window=window)
+
+
+@pytest.mark.parametrize("q", [2, 5, 40])
+def test_attention_widest_window(cuda_device, q):
+    """A window of 2^31 - 1 is none, also where rows stand before position 0."""
+    check_attention(Setup(q, [q, 1, q], [q - 2, 70, 130], 2, 64, 16, BF), 4, window=2 ** 31 - 1)
 
 
 @pytest.mark.parametrize("q", [1, 3, 40])
