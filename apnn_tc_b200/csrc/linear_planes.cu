@@ -17,10 +17,13 @@ using namespace tc5;
 // meet in one instruction is free as long as both operands agree, so the fields of a word are taken as they lie, bits b and
 // b + 16 side by side: elements 31 - b and 15 - b.  The block pairs its part of X the same way in shared memory, once for its
 // eight warps.  K is split over the blocks of a cluster where the weight rows alone are too few warps for the device, and where
-// X would not fit; their sums meet in distributed shared memory, added in the order of the ranks.
+// X would not fit; their sums meet in distributed shared memory, added in the order of the ranks.  What bounds it is the spreading,
+// some 25 elements a clock and SM at 4 bits (32768 x 16384: 78 us, 3.4 TB/s of planes; 61 at 2 bits, 51 at 1), and below a
+// few thousand rows the launch and one chain of loads (4096 x 4096, 4 bits: 6-7 us).
 constexpr int FEW_WARPS = 8;
 constexpr int FEW_TILE = 16 * FEW_WARPS;      // weight rows of a block
-constexpr int FEW_ROWS = 8;                   // rows of X; from nine on linear_tile is as fast (4096 x 4096, 4 bits: 11.4 us against 12.0 with two column tiles here)
+// Rows of X: from nine on linear_tile is as fast (4096 x 4096, 4 bits: 10.9 us against 12.0 with two column tiles here).
+constexpr int FEW_ROWS = 8;
 constexpr int FEW_SPLIT = 8;                  // largest cluster
 constexpr int FEW_X_BYTES = 96 * 1024;        // two blocks to an SM
 
