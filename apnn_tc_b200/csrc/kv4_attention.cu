@@ -64,7 +64,7 @@ template <int D, int NQ>
 struct Flow {
   static constexpr int WK = D / 32;    // words of a key row per lane (four lanes hold a row)
   static constexpr int WV = D / 64;    // words of a value row per lane (eight lanes)
-  static constexpr int ROW = D / 2;
+  static constexpr int ROW = D / 2, ROW_LOG = D == 64 ? 5 : D == 128 ? 6 : 7;
   static constexpr int V_AT = FLOW_KEYS * ROW, KP_AT = 2 * V_AT, VP_AT = KP_AT + FLOW_KEYS * 4;
   static constexpr int STAGE = VP_AT + FLOW_KEYS * 4;
   static constexpr int RING = FLOW_STAGES * STAGE;
@@ -73,7 +73,7 @@ struct Flow {
   static constexpr int PER_WARP = RING > MERGE ? RING : MERGE;
   static constexpr bool Q_IN_REGS = NQ * WK <= 4;
   static constexpr int Q_BYTES = Q_IN_REGS ? 0 : 2 * WK * NQ * 32 * 8;
-  static constexpr int SMEM = FLOW_WARPS * PER_WARP + Q_BYTES + ROWS * 8 + 512;
+  static constexpr int SMEM = FLOW_WARPS * PER_WARP + Q_BYTES + ROWS * 8 + 128;
   static constexpr int BLOCKS = NQ == 1 ? (D == 256 ? 2 : 4) : NQ == 2 ? (D == 256 ? 2 : 3) : 2;   // per SM
   static constexpr int SLOT = ROWS * (D + 2);            // floats of a partial result
 };
@@ -82,9 +82,11 @@ struct Flow {
 // in different banks (D = 64; two by two at D = 128), while eight lanes that read key rows still take whole 128-byte lines.
 __device__ __forceinline__ int flow_key(int r) { return r ^ ((r >> 1) & 1) ^ ((r >> 2) & 1); }
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ const uint8_t* shuffle_ptr(const uint8_t* p, int lane) {
+  return reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), lane));
 }
 
 struct FlowParams {
@@ -107,13 +109,7 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
   uint2* q_s = reinterpret_cast<uint2*>(smem + FLOW_WARPS * F::PER_WARP);
   float2* qf_s = reinterpret_cast<float2*>(smem + FLOW_WARPS * F::PER_WARP + F::Q_BYTES);   // per row: factor of the products, of the lows
   int* scan_s = reinterpret_cast<int*>(smem + FLOW_WARPS * F::PER_WARP + F::Q_BYTES + F::ROWS * 8);
-  // per warp and stage: a barrier that the copies complete on, and which of the four groups of eight keys there are
-  const uint32_t bars = smem_u32(scan_s) + 128 + warp * (FLOW_STAGES * 8);
-  volatile uint32_t* live_s = reinterpret_cast<volatile uint32_t*>(scan_s + 64) + warp * FLOW_STAGES;
   const int heads = p.cache.heads, sequences = p.batch.sequences;
-  if (lane < FLOW_STAGES) mbar_init(bars + 8 * lane, 1);
-  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  __syncthreads();
   grid_dependency_wait();
   grid_launch_dependents();   // the joining kernel waits for this whole grid anyway
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.status_flag = 0;
@@ -168,9 +164,6 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
     u0 = blockIdx.x;
     u1 = sequences * heads;
   }
-  int stage = 0, fill = 0;      // ring slot to read, to fill; both have passed the same number of tiles between segments
-  uint32_t phase = 0;           // of the slot to read
-  bool ok = true;
 
   for (int u = u0; u < u1;) {
     int t0 = 0, nt, bh_unit = 0;
@@ -197,43 +190,73 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
     }
     const int rows = s.n * p.group;     // at most 8 NQ
 
-    // ---- copies of this warp's 32-key pieces of the segment: per run of keys in one page its key levels, value levels and
-    // the parameters of both, a lane each
+    // ---- copies of this warp's 32-key pieces of the segment, 16 bytes a lane: key levels, value levels and the parameters of
+    // both lie in runs of 8 to 32 keys of one page.  Four lanes look up the page of a run, a tile ahead.  (Bulk copies of a run by a
+    // lane each: they leave a warp one at a time, 1000 clk for a tile's four, half as long as its attention.)
     const int key0 = (s.tile0 + t0) * FLOW_TILE + warp * FLOW_KEYS;
-    const int run = lane >> 2, part = lane & 3, run_keys = 1 << fp.run_shift;
-    const int unit_bytes = part < 2 ? F::ROW : 4;
-    const uint8_t* part_base = p.cache.data + h * p.cache.head_bytes + (long long)p.cache.page_size * (part < 2 ? part * F::ROW : D + (part - 2) * 4);
-    const uint32_t part_dst = ring + (part == 0 ? 0 : part == 1 ? F::V_AT : part == 2 ? F::KP_AT : F::VP_AT) + run * run_keys * unit_bytes;
+    const int run_shift = fp.run_shift, run_log = F::ROW_LOG + run_shift, v_off = p.cache.page_size * F::ROW;
+    const uint8_t* head_base = p.cache.data + h * p.cache.head_bytes;
     const int* trow = p.batch.table + (long long)b * p.batch.table_stride;
-    // the key this lane copies next, and where its copying ends (end <= table_width * page_size: within the table)
-    int at_key = key0 + run * run_keys;
-    const int stop = run < (FLOW_KEYS >> fp.run_shift) ? min(s.end, key0 + nt * FLOW_TILE) : 0;
-    const uint32_t all_live = 0xffffu >> (16 - 4 * (FLOW_KEYS >> fp.run_shift));
-    auto source = [&]() -> const uint8_t* {
+    const uint32_t all_live = 0xffffu >> (16 - 4 * (FLOW_KEYS >> run_shift));
+    const uint32_t lane_dst = ring + lane * 16;
+    // this lane's run of the next tile to look up, and where the looking ends (end <= table_width * page_size: within the table)
+    int at_key = key0 + ((lane >> 2) << run_shift);
+    const int stop = (lane >> 2) < (FLOW_KEYS >> run_shift) ? min(s.end, key0 + nt * FLOW_TILE) : 0;
+    auto source = [&]() -> const uint8_t* {      // the first key's levels; a page of more than 32 keys holds the tile in one run
       const uint8_t* src = nullptr;
       if (at_key < stop) {
         const int id = __ldg(trow + (at_key >> p.cache.page_shift));
-        if ((uint32_t)id < (uint32_t)p.cache.pages) src = part_base + id * p.cache.page_stride + (at_key & (p.cache.page_size - 1)) * unit_bytes;
+        if ((uint32_t)id < (uint32_t)p.cache.pages) src = head_base + id * p.cache.page_stride + (at_key & (p.cache.page_size - 1)) * F::ROW;
       }
       at_key += FLOW_TILE;
       return src;
     };
-    auto issue = [&](int i, const uint8_t* src) {
-      if (i >= nt || !ok) return;
-      const uint32_t live = __ballot_sync(0xffffffffu, src != nullptr);     // four bits for each run
-      if (lane == 0) {
-        live_s[fill] = live;
-        mbar_expect_tx(bars + 8 * fill, __popc(live) * (run_keys * (2 * F::ROW + 8) / 4));
+    // returns which runs there are, four bits for each
+    auto issue = [&](int i, const uint8_t* src) -> uint32_t {
+      uint32_t live = 0;
+      if (i < nt) {
+        live = __ballot_sync(0xffffffffu, src != nullptr);
+        const uint32_t dst = lane_dst + (i % FLOW_STAGES) * F::STAGE;
+        const int first = (key0 + i * FLOW_TILE) & (p.cache.page_size - 1);
+        // from a run's key levels to the keys' parameters (the page holds both parts' levels first)
+        const int params = 2 * v_off - (run_shift == 5 ? first * (F::ROW - 4) : 0);
+        if (run_shift == 5) {
+          const uint8_t* from = shuffle_ptr(src, 0);
+          if (live != 0) {
+            const uint8_t *k = from + lane * 16, *v = k + v_off;
+#pragma unroll
+            for (int c = 0; c < F::V_AT / 512; c++) {
+              copy16(dst + c * 512, k + c * 512);
+              copy16(dst + F::V_AT + c * 512, v + c * 512);
+            }
+            if (lane < 16) copy16(dst + F::KP_AT, from + params + (lane >> 3) * (4 * p.cache.page_size) + (lane & 7) * 16);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < F::V_AT / 512; c++) {
+            const int byte = c * 512 + lane * 16;
+            const uint8_t* from = shuffle_ptr(src, (byte >> run_log) * 4);
+            if (from != nullptr) {
+              from += byte & ((1 << run_log) - 1);
+              copy16(dst + c * 512, from);
+              copy16(dst + F::V_AT + c * 512, from + v_off);
+            }
+          }
+          const int byte = (lane & 7) * 16;
+          const uint8_t* from = shuffle_ptr(src, (byte >> (2 + run_shift)) * 4);
+          if (from != nullptr && lane < 16)
+            copy16(dst + F::KP_AT, from + params + (lane >> 3) * (4 * p.cache.page_size) + (byte & ((4 << run_shift) - 1)));
+        }
       }
-      __syncwarp();
-      if (src != nullptr) bulk_load(part_dst + fill * F::STAGE, src, run_keys * unit_bytes, bars + 8 * fill);
-      fill = fill + 1 == FLOW_STAGES ? 0 : fill + 1;
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      return live;
     };
     const uint8_t* src = source();
+    uint32_t live_of[FLOW_STAGES - 1];      // of the tiles on their way
 #pragma unroll
     for (int i = 0; i < FLOW_STAGES - 1; i++) {
       const uint8_t* next = source();
-      issue(i, src);
+      live_of[i] = issue(i, src);
       src = next;
     }
 
@@ -531,27 +554,24 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
       }
     };
 
-    for (int i = 0; i < nt && ok; i++) {
+    for (int i = 0; i < nt; i++) {
       const uint8_t* next = source();
-      if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, phase))) {
-        // never seen.  Give up; the copies still on their way get one more bounded wait each.
-        ok = false;
-        if (lane == 0) atomicExch(p.status_flag, 1);
-        for (int k = 1; k < FLOW_STAGES - 1 && i + k < nt; k++) mbar_wait(bars + 8 * ((stage + k) % FLOW_STAGES), phase ^ (stage + k >= FLOW_STAGES ? 1u : 0u));
-        break;
-      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(FLOW_STAGES - 2) : "memory");
+      __syncwarp();
+      const uint32_t live = live_of[0];
       const int key = key0 + i * FLOW_TILE;
       if (key < s.end && key + FLOW_KEYS > s.begin) {       // warp-uniform
-        const uint32_t at = ring + stage * F::STAGE, live = live_s[stage];
+        const uint32_t at = ring + (i % FLOW_STAGES) * F::STAGE;
         if (live == all_live && key >= last_begin && key + FLOW_KEYS <= first_end) attend(std::true_type(), key, at, live);
         else attend(std::false_type(), key, at, live);
       }
       __syncwarp();
-      issue(i + FLOW_STAGES - 1, src);
+#pragma unroll
+      for (int k = 0; k < FLOW_STAGES - 2; k++) live_of[k] = live_of[k + 1];
+      live_of[FLOW_STAGES - 2] = issue(i + FLOW_STAGES - 1, src);
       src = next;
-      stage = stage + 1 == FLOW_STAGES ? 0 : stage + 1;
-      if (stage == 0) phase ^= 1u;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
 
     // ---- the four warps' results meet in shared memory
@@ -620,7 +640,6 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
         if (d == 0) *reinterpret_cast<float2*>(slot + r * 2) = make_float2(M, L);
       }
     }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();     // the exchange area is the next segment's ring
     u = next_u;
     loc = 0;
