@@ -55,8 +55,8 @@ constexpr int FLOW_WARPS = 4;
 constexpr int FLOW_KEYS = 32;                       // per warp and tile
 constexpr int FLOW_TILE = FLOW_WARPS * FLOW_KEYS;   // 128
 constexpr int FLOW_STAGES = 3;
-// What beginning and ending a (sequence, head) costs, in tiles, when work is shared out (64 ragged sequences of 8 heads: 72 us
-// at 1, 66 at 2, 68 at 4).
+// What beginning and ending a (sequence, head) costs, in tiles, when work is shared out (64 ragged sequences of 8 heads: 69 us
+// at 1, 62 at 2, 63 at 3 and 4).
 constexpr int FLOW_SEGMENT = 2;
 constexpr int UNSPLIT_KEYS = 512;   // tables of at most this many positions: no split, no second launch
 
@@ -117,24 +117,33 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
   // ---- which units this block takes: an equal share of all, in order.  A (sequence, head) is FLOW_SEGMENT units of overhead,
   // then a unit for each tile.
   int u0, u1, b = 0, h = 0, loc = 0;
-  long long total = 0, sharing = 0;     // blocks that take part
+  int share = 0, longer = 0;     // units of a block; the first `longer` blocks have one more
   Span s;
   auto weight = [&](const Span& x) { return x.tiles == 0 ? 0 : (x.tiles + FLOW_SEGMENT) * heads; };
   if (fp.split) {
-    int sum = 0;
-    for (int i = threadIdx.x; i < sequences; i += 32 * FLOW_WARPS) sum += weight(span_of<FLOW_TILE>(p, i));
-    sum = __reduce_add_sync(0xffffffffu, sum);
-    if (lane == 0) scan_s[warp] = sum;
-    __syncthreads();
-    total = (long long)scan_s[0] + scan_s[1] + scan_s[2] + scan_s[3];
-    sharing = min(total, (long long)gridDim.x);     // no share is empty: the joining kernel counts on every block between two
-    if (blockIdx.x >= sharing) return;
-    u0 = (int)(total * blockIdx.x / sharing);
-    u1 = (int)(total * (blockIdx.x + 1) / sharing);
+    // false for a block without a share.  No share between two is empty: the joining kernel counts on it
+    auto take = [&](int total) {
+      const int sharing = min(total, (int)gridDim.x), block = (int)blockIdx.x;
+      if (block >= sharing) return false;
+      share = total / sharing;
+      longer = total - share * sharing;
+      u0 = share * block + min(block, longer);
+      u1 = u0 + share + (block < longer ? 1 : 0);
+      return true;
+    };
+    const bool at_once = sequences <= 32 * FLOW_WARPS;
+    if (!at_once) {
+      int sum = 0;
+      for (int i = threadIdx.x; i < sequences; i += 32 * FLOW_WARPS) sum += weight(span_of<FLOW_TILE>(p, i));
+      sum = __reduce_add_sync(0xffffffffu, sum);
+      if (lane == 0) scan_s[warp] = sum;
+      __syncthreads();
+      if (!take(scan_s[0] + scan_s[1] + scan_s[2] + scan_s[3])) return;
+    }
     // the sequence of unit u0, 128 sequences at a time
     int before = 0;
     for (int base = 0;; base += 32 * FLOW_WARPS) {
-      __syncthreads();
+      if (base > 0) __syncthreads();
       const int i = base + threadIdx.x;
       const int mine = i < sequences ? weight(span_of<FLOW_TILE>(p, i)) : 0;
       int inc = mine;
@@ -147,12 +156,13 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
       __syncthreads();
       int at = before;
       for (int w = 0; w < warp; w++) at += scan_s[4 + w];
+      before += scan_s[4] + scan_s[5] + scan_s[6] + scan_s[7];
+      if (at_once && !take(before)) return;
       if (u0 >= at + inc - mine && u0 < at + inc) {
         scan_s[8] = i;
         scan_s[9] = at + inc - mine;
       }
-      before += scan_s[4] + scan_s[5] + scan_s[6] + scan_s[7];
-      if (before > u0) break;     // uniform; total > u0, so a sequence is found
+      if (before > u0) break;     // uniform; the total is more than u0, so a sequence is found
     }
     __syncthreads();
     b = scan_s[8];
@@ -607,8 +617,9 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
     float* slot = complete ? nullptr : fp.slots + (2ll * blockIdx.x + (t0 == 0 ? 1 : 0)) * F::SLOT;
     if (threadIdx.x == 0 && fp.split && t0 == 0) {
       // the last unit of this (sequence, head) lies with the block whose share holds it
-      const long long last = (long long)bh_unit + FLOW_SEGMENT + s.tiles - 1;
-      fp.pieces[bh] = complete ? make_int2(0, 0) : make_int2((int)blockIdx.x, (int)(((last + 1) * sharing - 1) / total) - (int)blockIdx.x + 1);
+      const int last = bh_unit + FLOW_SEGMENT + s.tiles - 1, even = longer * (share + 1);
+      const int block = last < even ? last / (share + 1) : longer + (last - even) / share;
+      fp.pieces[bh] = complete ? make_int2(0, 0) : make_int2((int)blockIdx.x, block - (int)blockIdx.x + 1);
     }
     for (int e = threadIdx.x; e < rows * (D / 4); e += 32 * FLOW_WARPS) {
       const int r = e / (D / 4), d = (e % (D / 4)) * 4;
