@@ -451,6 +451,17 @@ def test_attention_long_and_ragged(cuda_device, dtype):
     check_attention(Setup(8, [40], [2500], 1, 64, 64, dtype), 2)
 
 
+@pytest.mark.parametrize("B,window", [(128, 0), (129, 0), (300, 40), (1000, 0)])
+def test_attention_many_sequences(cuda_device, B, window):
+    """Work shared out over more sequences than a block looks at in one go, some without rows, a few long ones among them."""
+    rng = np.random.default_rng(B)
+    lens_q = rng.integers(0, 3, size=B)
+    lens_kv = lens_q + rng.integers(0, 40, size=B)
+    lens_kv[::37] = rng.integers(500, 900, size=len(lens_kv[::37]))
+    lens_q[0], lens_q[-1] = 0, 2
+    check_attention(Setup(B, lens_q, np.maximum(lens_kv, 1), 2, 64, 64, BF, spare_rows=2), 4, window=window)
+
+
 def test_attention_more_rows_than_promised(cuda_device):
     """Rows of a sequence beyond max_q are left as they were."""
     for promised, q in ((1, 3), (2, 9), (40, 50)):
