@@ -248,6 +248,7 @@ static_assert(4 * Roles<1>::GROUPS >= MAX_STAGES && 4 * Roles<2>::GROUPS >= MAX_
 template <int WB, bool BF16, int CTAS>
 __global__ void __launch_bounds__(Roles<CTAS>::THREADS, 1)
     linear_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const TileParams p) {
+  constexpr int STEP = CTAS == 2 ? 1 : 2;      // stages that share their barriers: the full one of the first, the empty one of the last
   constexpr int GROUPS = Roles<CTAS>::GROUPS, SPREAD_WARPS = Roles<CTAS>::SPREAD_WARPS, PUBLISH = Roles<CTAS>::PUBLISH, PLANES = Roles<CTAS>::PLANES;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -314,12 +315,14 @@ __global__ void __launch_bounds__(Roles<CTAS>::THREADS, 1)
     const int rows = p.tn / CTAS;
     for (int tile = first_tile; tile < num_tiles && ok; tile += tile_step) {
       const int row = tile % p.tiles_x * p.tn + (int)half * rows;
-      for (int kb = 0; kb < kbn; kb++) {
-        if (!__all_sync(0xffffffffu, mbar_wait(empty_bar(s), ph ^ 1u))) { ok = false; break; }
-        const uint32_t dst = stages_at + s * p.stage_bytes + (CTAS == 2 ? A_BYTES : 0);
-        if (CTAS == 1 || rank == 0) expect_bytes(full_bar(s), p.tn * BK, lead);     // pair: both blocks' bytes
-        copy_box<CTAS>(dst, &map_x, (kb0 + kb) * 64, row, CTAS == 2 ? map_to_cta(full_bar(s), 0) : full_bar(s), lead);
-        s = s + 1 == p.stages ? 0 : s + 1;
+      for (int kb = 0; kb < kbn; kb += STEP) {
+        if (!__all_sync(0xffffffffu, mbar_wait(empty_bar(s + STEP - 1), ph ^ 1u))) { ok = false; break; }
+        if (CTAS == 1 || rank == 0) expect_bytes(full_bar(s), STEP * p.tn * BK, lead);     // pair of blocks: both blocks' bytes
+#pragma unroll
+        for (int i = 0; i < STEP; i++)
+          copy_box<CTAS>(stages_at + (s + i) * p.stage_bytes + (CTAS == 2 ? A_BYTES : 0), &map_x, (kb0 + kb + i) * 64, row,
+                         CTAS == 2 ? map_to_cta(full_bar(s), 0) : full_bar(s), lead);
+        s = s + STEP == p.stages ? 0 : s + STEP;
         ph ^= s == 0 ? 1u : 0u;
       }
     }
@@ -336,14 +339,17 @@ __global__ void __launch_bounds__(Roles<CTAS>::THREADS, 1)
         if (!__all_sync(0xffffffffu, mbar_wait(tempty_bar(acc), ((tl >> 1) & 1u) ^ 1u))) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * ACC_COLUMNS<CTAS>;
-        for (int kb = 0; kb < kbn; kb++) {
+        for (int kb = 0; kb < kbn; kb += STEP) {
           if (!__all_sync(0xffffffffu, mbar_wait(full_bar(s), ph))) { ok = false; break; }
           tc_fence_after();
-          const uint32_t lo = ((stages_at + s * p.stage_bytes) >> 4) | (1u << 16);
-          if (CTAS == 2) stage_mmas<CTAS>(d_tmem, lo, lo + (A_BYTES >> 4), p.idesc, kb != 0 ? 1u : 0u, lead);
-          else stage_mmas_tmem(d_tmem, tmem_base + TILES_AT + s * STAGE_COLUMNS, lo, p.idesc, kb != 0 ? 1u : 0u, lead);
-          commit<CTAS>(empty_bar(s), lead);
-          s = s + 1 == p.stages ? 0 : s + 1;
+#pragma unroll
+          for (int i = 0; i < STEP; i++) {
+            const uint32_t lo = ((stages_at + (s + i) * p.stage_bytes) >> 4) | (1u << 16);
+            if (CTAS == 2) stage_mmas<CTAS>(d_tmem, lo, lo + (A_BYTES >> 4), p.idesc, kb + i != 0 ? 1u : 0u, lead);
+            else stage_mmas_tmem(d_tmem, tmem_base + TILES_AT + (s + i) * STAGE_COLUMNS, lo, p.idesc, kb + i != 0 ? 1u : 0u, lead);
+          }
+          commit<CTAS>(empty_bar(s + STEP - 1), lead);
+          s = s + STEP == p.stages ? 0 : s + STEP;
           ph ^= s == 0 ? 1u : 0u;
         }
         if (ok) commit<CTAS>(tfull_bar(acc), lead);
@@ -378,7 +384,7 @@ __global__ void __launch_bounds__(Roles<CTAS>::THREADS, 1)
         named_sync(group_barrier<GROUPS>(pair), GROUP_THREADS + 32);
 #pragma unroll
         for (int i = 0; i < 2; i++, s = (s + 1 == p.stages) ? 0 : s + 1)
-          if (lane == 0) arrive_remote(full0 + 8u * s);
+          if (lane == 0 && (i == 0 || STEP == 1)) arrive_remote(full0 + 8u * s);
       }
   } else if (warp >= FIRST_SPREAD) {
     // ---------------- spread the weights ----------------
@@ -645,6 +651,7 @@ apnn_status linear_tile(cudaStream_t s, const LinearParams& l, bool bf16) {
   p.stage_bytes = (plan.ctas == 2 ? A_BYTES : 0) + plan.tn / plan.ctas * BK;
   p.stages = (SMEM_BYTES - 2048 - CHUNKS * l.wbits * PLANE_BYTES) / p.stage_bytes;
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+  if (plan.ctas == 1) p.stages &= ~1;
   if (p.stages < 2 * (plan.ctas == 2 ? Roles<2>::GROUPS : Roles<1>::GROUPS)) return APNN_ERR_UNSUPPORTED;      // not reached: 5 and 8 at least
   const long long tiles = (long long)p.tiles_x * p.tiles_w;
   const int slots = sms / plan.ctas;
