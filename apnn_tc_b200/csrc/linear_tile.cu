@@ -13,8 +13,8 @@
 //
 // What bounds a stage: of the pair's 256 x 256 tile, shared memory, 32 KiB in and out for the weight tile and 256 bytes for each row
 // of X a block holds, at 128 bytes a clock, 512 clk and as long as its MMAs (4096 x 16384 x 4096, 4 bits: 352 us, 1.56 PFLOP/s).  Of a
-// block alone about 0.2 us whatever its width: 240 clk of the integer pipe at 4 bits, and 215 clk for the one warp that waits for a
-// stage, issues its MMAs and commits them (16 x 16384 x 4096, 2 bits: 16 us; with the tiles in shared memory 18.8).
+// block alone 0.15 us (1 bit) to 0.18 (4) whatever its width: the integer pipe, 240 clk at 4 bits, and the one warp that waits for
+// stages, issues their MMAs and commits them (16 x 16384 x 4096, 2 bits: 13 us; with the tiles in shared memory 18.8).
 //
 // Few tiles and a long K: the blocks of a cluster share a tile's K, and each finishes a slice of the tile's rows of X from the others'
 // sums in its shared memory, added in the order of the ranks.
@@ -36,10 +36,10 @@ constexpr int CHUNKS = 2;
 constexpr int EPI_WARPS = 8, FIRST_SPREAD = 2 + EPI_WARPS, GROUP_THREADS = 128;
 // Groups of spreading warps.  A group that has spread a pair of stages waits for the slots of its next pair, 2 GROUPS stages on: with
 // no fewer slots in the ring the use before the one it waits for is over by then, so the parity names one use only.  (128 x 4096 x 4096, 4
-// bits, a block alone: 18.3 us with two groups, 17.6 with three, 18.1 with four.)
+// bits, a block alone: 17.9 us with two groups, 16.7 with three, 16.0 with four; 1 bit 14.5, 14.0, 13.7.)
 template <int CTAS>
 struct Roles {
-  static constexpr int GROUPS = CTAS == 2 ? 2 : 3, SPREAD_WARPS = 4 * GROUPS;
+  static constexpr int GROUPS = CTAS == 2 ? 2 : 4, SPREAD_WARPS = 4 * GROUPS;
   static constexpr int PUBLISH = FIRST_SPREAD + SPREAD_WARPS, PLANES = PUBLISH + 1, THREADS = 32 * (PLANES + 1);
 };
 constexpr int COLUMNS = 16;                     // of an accumulator that an epilogue warp takes at a time
@@ -558,8 +558,8 @@ struct Plan {
 
 // The plan of the shortest estimated time.  A wave of tiles takes its stages or its epilogue, whichever is longer, and the last
 // epilogue shows; a split adds the exchange.  The figures (us) are fitted to 24 shapes on every plan (16 to 4096 rows, 1000 to 32003
-// weights, K from 128 to 8192), most within a tenth: e.g. 333 x 2337 x 2296 14.9 on 64-wide tiles, 18.7 on the pair's 256; 128 x 4096 x 4096
-// 17.9 with 128-wide tiles and K in four, 23.5 without.
+// weights, K from 128 to 8192), most within a tenth: e.g. 333 x 2337 x 2296 13.2 on 64-wide tiles, 18.9 on the pair's 256;
+// 32 x 4096 x 4096 10.9 with K in four, 18.0 without.
 Plan pick_plan(int M, int N, int kblocks, int sms) {
   Plan best = {1, 32, 1};
   double least = 1e30;
@@ -571,7 +571,7 @@ Plan pick_plan(int M, int N, int kblocks, int sms) {
         // a cluster finds its blocks within one group of SMs: the driver knows how many fit
         const int slots = split > 1 ? cluster_capacity(reinterpret_cast<const void*>(linear_tile_kernel<4, true, 1>), Roles<1>::THREADS, SMEM_BYTES, split) : sms / ctas;
         if (slots < 1) continue;
-        const double stage = ctas == 1 ? (tn <= 64 ? 0.2 : 0.215) : (tn == 64 ? 0.265 : tn == 128 ? 0.285 : 0.375);
+        const double stage = ctas == 1 ? (tn <= 64 ? 0.185 : 0.2) : (tn == 64 ? 0.265 : tn == 128 ? 0.285 : 0.355);
         const double epilogue = (ctas == 1 ? 0.8 : 1.4) + 0.012 * tn;
         const double stages = stage * (double)((kblocks / 2 + split - 1) / split * 2);
         const double exchange = split > 1 ? 1.5 + 0.1 * (tn / split) + 0.015 * tn : 0.0;
