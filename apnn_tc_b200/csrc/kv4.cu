@@ -66,6 +66,8 @@ constexpr int ROW_WARPS = 8;
 // Warps that fit a multiprocessor with the registers that the launch bounds leave.
 constexpr int APPEND_RESIDENT = 32, READ_RESIDENT = 48;
 
+constexpr float FIFTEENTH = 1.0f / 15.0f;
+
 // max that keeps NaN, so that one NaN among a row's elements shows in its step
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
@@ -75,12 +77,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // Where the rows t0 .. t0 + R - 1 of the batch lie, lane i holding row t0 + i; R <= 32.
 struct Places {
-  int count;               // rows before the last sequence's end
+  int count;               // rows before the last sequence's end and the tensors'
   int pos;
   uint8_t* page;           // null where there is none
 };
 __device__ __forceinline__ Places places_of(const Kv4View& cache, const Kv4Batch& batch, int t0, int R, int lane) {
-  Places out = {min(R, __ldg(batch.cu_q + batch.sequences) - t0), 0, nullptr};
+  Places out = {min(R, min(__ldg(batch.cu_q + batch.sequences), batch.rows) - t0), 0, nullptr};
   if (out.count <= 0) return out;
   int b = sequence_of(batch.cu_q, batch.sequences, t0, lane);
   const int t = t0 + min(lane, out.count - 1);
@@ -106,7 +108,7 @@ __device__ __forceinline__ Places places_of(const Kv4View& cache, const Kv4Batch
 // sequence, position and page is a chain of four dependent loads, paid once for all of them (lane i looks for row i) and not
 // for each (measured with a row a block: 42 us for 9325 rows of 3 * 16 heads of 64, all of it that chain).  Inputs are loaded
 // one row ahead, the first while the chain runs.  At that size 215 instructions for each 32 * 8 elements bound it: they issue in
-// 65% of the cycles.  Packed arithmetic saved a tenth of them and cost the registers that keep 32 warps resident (35 us).
+// 65% of the cycles.  Packed arithmetic saved a tenth of them and cost the registers that keep 32 warps resident (35 us against 33).
 template <bool BF16, int D>
 __global__ void __launch_bounds__(ROW_WARPS * 32, APPEND_RESIDENT / ROW_WARPS) kv4_append_kernel(const AppendParams p, const int R) {
   constexpr int LANES = D / 8;
@@ -235,7 +237,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, APPEND_RESIDENT / ROW_WARPS) k
     }
     if (live && page != nullptr) {
       // an infinity among the elements is lo or hi, a NaN is hi: either way the step is not finite
-      float step = round16<BF16>(__fsub_rn(__fdiv_rn(hi, 15.0f), __fdiv_rn(lo, 15.0f)));
+      float step = round16<BF16>(__fsub_rn(__fmul_rn(hi, FIFTEENTH), __fmul_rn(lo, FIFTEENTH)));
       float low = round16<BF16>(lo);
       if (step < 1.17549435e-38f) step = 0.0f;
       uint32_t word = 0;
@@ -307,7 +309,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, READ_RESIDENT / ROW_WARPS) kv4
 template <typename... Params, typename... Args>
 apnn_status launch_rows(const char* what, void (*kernel)(Params...), int rows, int pieces, int resident, void* stream, Args... args) {
   // rows of a block: what one wave of resident blocks leaves to each, up to the lanes that look them up (9325 rows of 3 * 16
-  // heads of 64, append and read: a row a block 42 + 20 us, 8 rows 34 + 11, this rule 33 + 11; from a cold L2 41 + 19)
+  // heads of 64, append and read: a row a block 42 + 20 us, 8 rows 34 + 11, this rule 31 + 11; from a cold L2 40 + 19)
   const int passes = (pieces + ROW_WARPS - 1) / ROW_WARPS, warps = (pieces + passes - 1) / passes;
   const int wave = device_sm_count() * (resident / warps);
   const int R = std::min((rows + wave - 1) / wave, 32);

@@ -318,8 +318,11 @@ def kv4_attention(cache: KVCache4, batch: KVBatch, q: torch.Tensor, *, scale: Op
         if lse.dtype is not torch.float32 or tuple(lse.shape) != (rows, q_heads) or not lse.is_contiguous():
             raise ValueError(f"lse must be a contiguous float32 [{rows}, {q_heads}]")
         lse_ptr = _on(index, "lse", lse)
-    if window and not causal:
-        raise ValueError("a window needs causal")
+    if window:
+        if not causal:
+            raise ValueError("a window needs causal")
+        if window >= 1 << 31:
+            raise ValueError("window must be below 2^31")
     q_ptr = _on(index, "q", q)
     if workspace is not None:
         if not workspace.is_contiguous():

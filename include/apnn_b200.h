@@ -455,7 +455,8 @@ typedef struct apnn_kv4_batch {
  *   y = x * (1 / sqrt(mean(x^2) + eps)) * weight          (with a norm weight; else y = x)
  *   (a, b) -> (a c - b s, b c + a s)                      over `rotary_dim` leading elements, pairs (i, i + rotary_dim/2) or
  *                                                         adjacent ones; c and s from rotary[position]
- *   lowest = min y, step = max y / 15 - min y / 15, both rounded to the cache's type (a step below 2^-126 counts as 0),
+ *   lowest = min y, step = max y * c - min y * c with the float32 c nearest to 1/15, both rounded to the cache's type (a step below
+ *   2^-126 counts as 0),
  *   level = clamp(rint((y - lowest) * (1 / step)), 0, 15), 0 where step is 0
  * Values are quantised as they are.  A row with a value, step or lowest that is not finite is held as NaN, as is a row
  * whose position lies behind the rotary table.  q (may be null) is only normed and rotated, into q_out (may be q itself). */

@@ -59,7 +59,8 @@ def quantise(x: np.ndarray, dtype):
     x = x.astype(np.float32)
     with np.errstate(all="ignore"):
         lo, hi = x.min(-1, keepdims=True), x.max(-1, keepdims=True)
-        step = hi / np.float32(15) - lo / np.float32(15)
+        c = np.float32(1) / np.float32(15)
+        step = hi * c - lo * c
         step, low = (torch.from_numpy(np.ascontiguousarray(a)).to(dtype).float().numpy() for a in (step, lo))
         step = np.where(step < np.float32(2.0 ** -126), np.float32(0), step)
         bad = ~(np.isfinite(x).all(-1, keepdims=True) & np.isfinite(step) & np.isfinite(low))

@@ -296,6 +296,29 @@ def test_append_rows_that_share_a_block(cuda_device, Hq, heads, D, most, B, norm
     check_append(s, Hq, norm, rot, False, rows=most + 12)
 
 
+@pytest.mark.parametrize("T,rows", [(20, 7), (9000, 7001), (9000, 8999), (60000, 59995)])
+def test_append_and_read_no_further_than_their_tensors(cuda_device, T, rows):
+    """Tensors of fewer rows than the batch's sequences: the cache and everything behind the tensors' rows stay as they were."""
+    s = Setup(T, [T], [T], 1, 64, 1024, BF)
+    k, v, q = (s.randn(rows + 40, n, 64).cuda() for n in (1, 1, 2))
+    before = s.data.clone()
+    q_out = torch.full_like(q, 3.0)
+    s.ap.kv4_append(s.cache, s.batch, k[:rows], v[:rows], q=q[:rows], q_out=q_out[:rows])
+    assert torch.equal(q_out[:rows], q[:rows]) and bool((q_out[rows:] == 3.0).all())
+    outs = [torch.full((rows + 40, 1, 64), 3.0, dtype=BF, device="cuda") for _ in range(2)]
+    s.ap.kv4_read(s.cache, s.batch, k_out=outs[0][:rows], v_out=outs[1][:rows])
+    for out in outs:
+        assert bool((out[rows:] == 3.0).all())
+    held = s.plain()
+    old = ref.Cache(before, s.page, s.D, s.dtype)
+    where, at = s.table[0, np.arange(rows, T) // s.page], np.arange(rows, T) % s.page
+    assert np.array_equal(held.levels[where, :, :, at], old.levels[where, :, :, at])
+    assert np.array_equal(held.params[where, :, :, at], old.params[where, :, :, at])
+    for i, out in enumerate(outs):
+        want = torch.from_numpy(held.values()[s.table[0, np.arange(rows) // s.page], :, i, np.arange(rows) % s.page].astype(np.float32)).to(BF)
+        assert torch.equal(out[:rows].cpu(), want)
+
+
 def test_append_bad_pages_and_positions(cuda_device):
     """Page numbers outside the cache, lengths shorter than the rows, lengths behind the table: those rows are not written."""
     s = Setup(4, [6, 9, 4], [40, 5, 60], 2, 64, 16, BF, wide=3)
