@@ -74,7 +74,8 @@ struct Flow {
   static constexpr bool Q_IN_REGS = NQ * WK <= 4;
   static constexpr int Q_BYTES = Q_IN_REGS ? 0 : 2 * WK * NQ * 32 * 8;
   static constexpr int SMEM = FLOW_WARPS * PER_WARP + Q_BYTES + ROWS * 8 + 128;
-  static constexpr int BLOCKS = NQ == 1 ? (D == 256 ? 2 : 4) : NQ == 2 ? (D == 256 ? 2 : 3) : 2;   // per SM
+  // per SM (one row, D = 128: one sequence of 65536 keys 24.3 us at 2, 24.5 at 3, 26.0 at 4; 64 ragged ones 67, 60, 60)
+  static constexpr int BLOCKS = NQ <= 2 && D != 256 ? 3 : 2;
   static constexpr int SLOT = ROWS * (D + 2);            // floats of a partial result
 };
 
@@ -672,10 +673,9 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) kv4_attention_join_kernel(con
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependency_wait();
   const int bh = blockIdx.x, b = bh / p.cache.heads, h = bh - b * p.cache.heads;
+  const int2 pc = __ldcg(fp.pieces + bh);      // on its way with the span's loads; what it holds without rows is not looked at
   const Span s = span_of<FLOW_TILE>(p, b);
-  if (s.n <= 0) return;
-  const int2 pc = __ldcg(fp.pieces + bh);
-  if (pc.y == 0) return;
+  if (s.n <= 0 || pc.y == 0) return;
   for (int r = blockIdx.y; r < s.n * p.group; r += gridDim.y) {
     float M = -INFINITY, L = 0.0f;
     float4 v[V];
