@@ -48,9 +48,9 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t* r) {
 //   sum_j p_j v_jd = 2^(R - 6) (sum_j w_j n_jd - 8 sum_j w_j) + sum_j p_j (low_j + 8 step_j)
 // takes the same rounded w in both sums, so the rounding meets levels centred at 8, not 0..15 (half the error of fp16
 // results).  Value words of two keys are put side by side by PRMT to give pairs along the keys.
-// HBM is the floor, (D + 8) bytes per key and head; the steady state runs at 1.36 times that, bound by instruction issue (585
-// for 32 keys of a warp), and some 17 us go to the start, the meeting of the warps and the joining kernel (64 sequences of up to
-// 16384 keys, 212 MB: 66 us, 3.2 TB/s; one of 65536, 71 MB: 28 us).
+// HBM is the floor, (D + 8) bytes per key and head; the steady state is bound by instruction issue (some 600 for 32 keys of a
+// warp, 56% of the cycles, the integer pipe at 51%), and about 10 us go to the start, the meeting of the warps and the joining
+// kernel (64 sequences of up to 16384 keys, 212 MB: 60 us, 3.5 TB/s; one of 65536, 71 MB: 24.5 us).
 constexpr int FLOW_WARPS = 4;
 constexpr int FLOW_KEYS = 32;                       // per warp and tile
 constexpr int FLOW_TILE = FLOW_WARPS * FLOW_KEYS;   // 128
