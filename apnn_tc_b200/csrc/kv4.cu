@@ -107,8 +107,8 @@ __device__ __forceinline__ Places places_of(const Kv4View& cache, const Kv4Batch
 // or all values, so a query is not quantised and a value neither normed nor turned.  A block takes `R` rows: finding a row's
 // sequence, position and page is a chain of four dependent loads, paid once for all of them (lane i looks for row i) and not
 // for each (measured with a row a block: 42 us for 9325 rows of 3 * 16 heads of 64, all of it that chain).  Inputs are loaded
-// one row ahead, the first while the chain runs.  At that size 215 instructions for each 32 * 8 elements bound it: they issue in
-// 65% of the cycles.  Packed arithmetic saved a tenth of them and cost the registers that keep 32 warps resident (35 us against 33).
+// one row ahead, the first while the chain runs.  At that size 200 instructions for each 32 * 8 elements bound it: they issue in
+// 69% of the cycles.  Packed arithmetic saved a tenth of them and cost the registers that keep 32 warps resident (35 us against 33).
 template <bool BF16, int D>
 __global__ void __launch_bounds__(ROW_WARPS * 32, APPEND_RESIDENT / ROW_WARPS) kv4_append_kernel(const AppendParams p, const int R) {
   constexpr int LANES = D / 8;

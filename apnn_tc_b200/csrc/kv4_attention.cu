@@ -49,7 +49,7 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t* r) {
 // takes the same rounded w in both sums, so the rounding meets levels centred at 8, not 0..15 (half the error of fp16
 // results).  Value words of two keys are put side by side by PRMT to give pairs along the keys.
 // HBM is the floor, (D + 8) bytes per key and head; the steady state is bound by instruction issue (some 600 for 32 keys of a
-// warp, 56% of the cycles, the integer pipe at 51%), and about 10 us go to the start, the meeting of the warps and the joining
+// warp, half of the cycles, the integer pipe at 46%), and about 10 us go to the start, the meeting of the warps and the joining
 // kernel (64 sequences of up to 16384 keys, 212 MB: 60 us, 3.5 TB/s; one of 65536, 71 MB: 24.5 us).
 constexpr int FLOW_WARPS = 4;
 constexpr int FLOW_KEYS = 32;                       // per warp and tile
