@@ -264,48 +264,52 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
     long long at = locate(0), at1 = locate(1);
     fetch(0, 0, at);
     fetch(1, 0, at);
-    for (int j = 0; j < tiles && ok; j++) {
+    // After a wait that ran out a warp announces nothing any more, but keeps meeting the other three at the barrier below, so that
+    // all of them reach the end.
+    for (int j = 0; j < tiles; j++) {
       const int s = j % P::DEPTH;
       const uint32_t ph = (uint32_t)(j / P::DEPTH) & 1u;
       const uint32_t slot_at = base + P::PAR_AT + (uint32_t)(j % SLOTS) * P::SLOT + (uint32_t)(key >> 1) * 16u + (uint32_t)(key & 1) * 4u;
       const long long at2 = locate(j + 2);
-      if (!__all_sync(0xffffffffu, mbar_wait(k_empty(s), ph ^ 1u))) { ok = false; break; }
-      store(0, base + P::K_AT + s * P::OPERAND);
-      {
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(k_empty(s), ph ^ 1u));
+      if (ok) {
+        store(0, base + P::K_AT + s * P::OPERAND);
         const float2 f = unpack2<BF16>(par[0]);
         sts32(slot_at, __float_as_uint(f.x));
         sts32(slot_at + 8, __float_as_uint(fmaf(8.0f, f.x, f.y)));      // the value of level 8
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(k_full(s));
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(k_full(s));
       fetch(0, j + 1, at1);
-      if (!__all_sync(0xffffffffu, mbar_wait(v_empty(s), ph ^ 1u))) { ok = false; break; }
-      store(1, base + P::V_AT + s * P::OPERAND);
-      {
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(v_empty(s), ph ^ 1u));
+      const float2 f = unpack2<BF16>(par[1]);
+      const uint32_t head_at = base + P::PAR_AT + (uint32_t)(j % SLOTS) * P::SLOT + 2048u;
+      if (ok) {
+        store(1, base + P::V_AT + s * P::OPERAND);
         const bool live = at >= 0;
-        const float2 f = unpack2<BF16>(par[1]);
         sts32(slot_at + 1024 + 8, __float_as_uint(fmaf(8.0f, f.x, f.y)));
         const uint32_t bits = __float_as_uint(fabsf(f.x));
         const uint32_t lives = __ballot_sync(0xffffffffu, live);
         const uint32_t most = __reduce_max_sync(0xffffffffu, live && bits < 0x7f800000u && (tile0 + j) * TILE + key >= key_begin ? bits : 0u);
-        // 2^R is above every value step met so far, within fp32's range: the largest of the four warps' keys
-        const uint32_t head_at = base + P::PAR_AT + (uint32_t)(j % SLOTS) * P::SLOT + 2048u;
         if (lane == 0) {
           sts32(head_at + warp * 4, lives);
           sts32(head_at + 16 + warp * 4, most);
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (ok) {
+        // 2^R is above every value step met so far, within fp32's range: the largest of the four warps' keys
         const uint32_t all = max(max(lds(head_at + 16), lds(head_at + 20)), max(lds(head_at + 24), lds(head_at + 28)));
         R = max(R, min((int)(all >> 23) - 126, 127));
         if (key == 0) sts32(head_at + 32, (uint32_t)R);
         sts32(slot_at + 1024, __float_as_uint(f.x * power2(6 - R)));
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(v_full(s));
-        mbar_arrive(par_full(j % SLOTS));
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(v_full(s));
+          mbar_arrive(par_full(j % SLOTS));
+        }
       }
       fetch(1, j + 1, at1);
       at = at1;
