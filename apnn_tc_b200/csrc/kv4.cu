@@ -174,10 +174,11 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, APPEND_RESIDENT / ROW_WARPS) k
       }
       const uint16_t* weight = p.norm[kind_now];
       if (weight != nullptr) {
-        // squares of 16-bit floats are exact in fp32; their sum is held in fp64, so its order does not show in the levels
+        // Squares are taken in fp64, where those of 16-bit floats are exact (in fp32 those of bf16 leave its range from 2^64 on and
+        // lose bits below 2^-63); so is their sum, so that its order does not show in the levels
         double sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) sum += (double)__fmul_rn(y[i], y[i]);
+        for (int i = 0; i < 8; i++) sum = fma((double)y[i], (double)y[i], sum);
 #pragma unroll
         for (int d = 1; d < LANES; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         const float scale = __fdiv_rn(1.0f, __fsqrt_rn((float)(sum / D + p.eps)));

@@ -459,7 +459,7 @@ typedef struct apnn_kv4_batch {
  *   2^-126 counts as 0),
  *   level = clamp(rint((y - lowest) * (1 / step)), 0, 15), 0 where step is 0
  * Values are quantised as they are.  A row with a value, step or lowest that is not finite is held as NaN, as is a row
- * whose position lies behind the rotary table.  q (may be null) is only normed and rotated, into q_out (may be q itself). */
+ * whose position lies behind the rotary table.  A head whose mean of squares is beyond fp32 norms to 0.  q (may be null) is only normed and rotated, into q_out (may be q itself). */
 typedef struct apnn_kv4_append_args {
   uint32_t struct_size;
   int32_t rows;           /* rows of q, k, v: none beyond is touched */
