@@ -47,10 +47,14 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t* r) {
 // reference point); they are rounded once, and
 //   sum_j p_j v_jd = 2^(R - 6) (sum_j w_j n_jd - 8 sum_j w_j) + sum_j p_j (low_j + 8 step_j)
 // takes the same rounded w in both sums, so the rounding meets levels centred at 8, not 0..15 (half the error of fp16
-// results).  Value words of two keys are put side by side by PRMT to give pairs along the keys.
+// results).  Where the steps of a segment lie more than 2^STEP_SPAN apart, the rest of it goes with a reference point of each row for the
+// values, apart from that of the softmax: w_j = 2^(s_j - m + log2 step_j - a) with a at most 14 below the largest exponent.
+// Value words of two keys are put side by side by PRMT to give pairs along the keys.
 // HBM is the floor, (D + 8) bytes per key and head; the steady state is bound by instruction issue (some 600 for 32 keys of a
 // warp, half of the cycles, the integer pipe at 46%), and about 10 us go to the start, the meeting of the warps and the joining
-// kernel (64 sequences of up to 16384 keys, 212 MB: 60 us, 3.5 TB/s; one of 65536, 71 MB: 24.5 us).
+// kernel (64 sequences of up to 16384 keys, 212 MB: 60 us, 3.5 TB/s; one of 65536, 71 MB: 25 us in a row on the device, 27 with the
+// host's call).  Looking after the steps' range costs one comparison a tile; 64 sequences of 4096 keys whose steps lie far apart take
+// 93 us, others 77.
 constexpr int FLOW_WARPS = 4;
 constexpr int FLOW_KEYS = 32;                       // per warp and tile
 constexpr int FLOW_TILE = FLOW_WARPS * FLOW_KEYS;   // 128
@@ -74,7 +78,7 @@ struct Flow {
   static constexpr bool Q_IN_REGS = NQ * WK <= 4;
   static constexpr int Q_BYTES = Q_IN_REGS ? 0 : 2 * WK * NQ * 32 * 8;
   static constexpr int SMEM = FLOW_WARPS * PER_WARP + Q_BYTES + ROWS * 8 + 128;
-  // per SM (one row, D = 128: one sequence of 65536 keys 24.3 us at 2, 24.5 at 3, 26.0 at 4; 64 ragged ones 67, 60, 60)
+  // per SM (one row, D = 128, on the device: one sequence of 65536 keys 24.3 us at 2, 24.5 at 3, 26.0 at 4; 64 ragged ones 67, 60, 60)
   static constexpr int BLOCKS = NQ <= 2 && D != 256 ? 3 : 2;
   static constexpr int SLOT = ROWS * (D + 2);            // floats of a partial result
 };
@@ -374,10 +378,15 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
     };
     int R = -112;
     uint32_t step_bits = 0;     // the fp32 bits of 2^R, 0 before the first key: larger steps raise R
+    uint32_t under = 0xffffffffu;      // the bits of a power of two no step but 0 was below, less 1; all ones before the first
     float lift = __uint_as_float((uint32_t)(127 + 6 + 112) << 23);
+    float apart[2 * NQ];        // steps far apart: the values' reference points less the softmax's, log2
 
-    auto attend = [&](auto tag, int key, uint32_t at, uint32_t live) {
+    // False, with nothing done, where the steps turn out to lie too far apart for one power of two
+
+    auto attend = [&](auto tag, auto far_tag, int key, uint32_t at, uint32_t live) -> bool {
       constexpr bool WHOLE = decltype(tag)::value;      // every row sees every key: no mask is looked at
+      constexpr bool FAR = decltype(far_tag)::value;
       // ---- scores of two tiles of 16 keys
       float sc[2][NQ][4];
 #pragma unroll
@@ -454,20 +463,29 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
           top[2 * q] = fmaxf(top[2 * q], x[0]);
           top[2 * q + 1] = fmaxf(top[2 * q + 1], x[1]);
         }
-      // exponent of the largest value step of these keys (a step that is not finite shows in its weight instead)
-      uint32_t bits = __float_as_uint(fabsf(unpack2<BF16>(lds32(at + F::VP_AT + lane * 4)).x));
-      if (bits >= 0x7f800000u || (!WHOLE && (key + lane >= s.end || key + lane < s.begin || !((live >> ((lane >> fp.run_shift) * 4)) & 1u)))) bits = 0;
+      // exponents of the largest and the smallest value step of these keys (a step that is not finite shows in its weight instead)
+      uint32_t bits = 0;
+      if (!FAR) {
+        bits = __float_as_uint(fabsf(unpack2<BF16>(lds32(at + F::VP_AT + lane * 4)).x));
+        if (bits >= 0x7f800000u || (!WHOLE && (key + lane >= s.end || key + lane < s.begin || !((live >> ((lane >> fp.run_shift) * 4)) & 1u)))) bits = 0;
+      }
       // The reference point m follows the running maximum only where that has risen by more than 2^8: weights then stay below
       // 2^8 of it, and most tiles after a segment's first neither exchange maxima nor touch the sums.
-      bool moved = bits > step_bits;
+      bool moved = !FAR && (bits > step_bits || bits - 1u < under);
 #pragma unroll
       for (int c = 0; c < 2 * NQ; c++) moved |= top[c] > rise_at[c];
       if (__any_sync(0xffffffffu, moved)) {
-        const int rise = max(R, min((int)(__reduce_max_sync(0xffffffffu, bits) >> 23) - 126, 127));
-        const float shrink = __uint_as_float((uint32_t)max(127 + R - rise, 0) << 23);      // 2^(R - rise)
-        R = rise;
-        step_bits = (uint32_t)(127 + R) << 23;
-        lift = __uint_as_float((uint32_t)(127 + 6 - R) << 23);
+        float shrink = 1.0f;      // 2^(R - rise)
+        if (!FAR) {
+          const int rise = max(R, min((int)(__reduce_max_sync(0xffffffffu, bits) >> 23) - 126, 127));
+          const uint32_t least = min(under, __reduce_min_sync(0xffffffffu, bits - 1u));
+          if (steps_far_apart(rise, least)) return false;
+          if (least != 0xffffffffu) under = max((least + 1u) & 0x7f800000u, 1u) - 1u;
+          shrink = __uint_as_float((uint32_t)max(127 + R - rise, 0) << 23);
+          R = rise;
+          step_bits = (uint32_t)(127 + R) << 23;
+          lift = __uint_as_float((uint32_t)(127 + 6 - R) << 23);
+        }
         float kept[2 * NQ];
 #pragma unroll
         for (int c = 0; c < 2 * NQ; c++) {
@@ -479,12 +497,16 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
           rise_at[c] = top[c] + 8.0f;
           const float k = keep * shrink;
           kept[c] = keep;
+          if (FAR) {
+            if (m != top[c]) apart[c] += m - top[c];      // the values' own point stays; -inf where no key was met
+          } else {
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
+            for (int e = 0; e < 2; e++) {
 #pragma unroll
-            for (int w = 0; w < F::WV; w++)
+              for (int w = 0; w < F::WV; w++)
 #pragma unroll
-              for (int j = 0; j < 4; j++) o[w][j][c >> 1][(c & 1) + 2 * e] *= k;
+                for (int j = 0; j < 4; j++) o[w][j][c >> 1][(c & 1) + 2 * e] *= k;
+            }
           }
         }
 #pragma unroll
@@ -492,6 +514,38 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
           l[q] = mul2(l[q], pair(kept[2 * q], kept[2 * q + 1]));
           vsum[q] = mul2(vsum[q], pair(kept[2 * q], kept[2 * q + 1]));
           below[q] = pair(top[2 * q] == -INFINITY ? 0.0f : -top[2 * q], top[2 * q + 1] == -INFINITY ? 0.0f : -top[2 * q + 1]);
+        }
+      }
+      float lg[4];      // log2 of the value steps, to 2^-22 of themselves or of 1: far below an fp16 rounding of the weights
+      if (FAR) {
+        float most[2 * NQ];
+#pragma unroll
+        for (int c = 0; c < 2 * NQ; c++) most[c] = -INFINITY;
+        bool over = false;
+#pragma unroll
+        for (int r = 0; r < 4; r++) lg[r] = __log2f(fabsf(vp[r].x));
+#pragma unroll
+        for (int c = 0; c < 2 * NQ; c++) {
+          const float2 f = unpair(below[c >> 1]);
+#pragma unroll
+          for (int r = 0; r < 4; r++) most[c] = fmaxf(most[c], sc[r >> 1][c >> 1][2 * (r & 1) + (c & 1)] + (c & 1 ? f.y : f.x) + lg[r]);      // NaN counts as none
+          over |= most[c] > apart[c] + 14.0f;
+        }
+        if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+          for (int c = 0; c < 2 * NQ; c++) {
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) most[c] = fmaxf(most[c], __shfl_xor_sync(0xffffffffu, most[c], d));
+            const float up = fmaxf(apart[c], most[c] - 6.0f), k = up == apart[c] ? 1.0f : ex2(apart[c] - up);
+            apart[c] = up;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+#pragma unroll
+              for (int w = 0; w < F::WV; w++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[w][j][c >> 1][(c & 1) + 2 * e] *= k;
+            }
+          }
         }
       }
       // ---- weights, and their products with the values.  Levels are centred at 8 tile by tile: sums of what is all positive
@@ -512,7 +566,13 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
           const float2 z = unpair(add2(pair(x[0], x[1]), below[q]));
           const Pair e = pair(ex2(z.x), ex2(z.y));
           l[q] = add2(l[q], e);
-          float2 w = unpair(mul2(e, pair(step, step)));
+          float2 w;
+          if (FAR) {
+            w.x = copysignf(ex2(z.x + (lg[r] - (apart[2 * q] == -INFINITY ? 0.0f : apart[2 * q]))), vp[r].x);
+            w.y = copysignf(ex2(z.y + (lg[r] - (apart[2 * q + 1] == -INFINITY ? 0.0f : apart[2 * q + 1]))), vp[r].x);
+          } else {
+            w = unpair(mul2(e, pair(step, step)));
+          }
           if (WHOLE) {
             vsum[q] = fma2(e, pair(mid, mid), vsum[q]);
           } else {      // a masked place may hold NaN
@@ -563,24 +623,36 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
             o[w][j][q][3] = b.y;
           }
       }
+      return true;
     };
 
-    for (int i = 0; i < nt; i++) {
-      const uint8_t* next = source();
-      asm volatile("cp.async.wait_group %0;" ::"n"(FLOW_STAGES - 2) : "memory");
-      __syncwarp();
-      const uint32_t live = live_of[0];
-      const int key = key0 + i * FLOW_TILE;
-      if (key < s.end && key + FLOW_KEYS > s.begin) {       // warp-uniform
-        const uint32_t at = ring + (i % FLOW_STAGES) * F::STAGE;
-        if (live == all_live && key >= last_begin && key + FLOW_KEYS <= first_end) attend(std::true_type(), key, at, live);
-        else attend(std::false_type(), key, at, live);
-      }
-      __syncwarp();
+    int i = 0;
+    auto walk = [&](auto far_tag) {      // from tile i on, to the end or to a tile whose steps lie too far apart
+      for (; i < nt; i++) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(FLOW_STAGES - 2) : "memory");
+        __syncwarp();
+        const uint32_t live = live_of[0];
+        const int key = key0 + i * FLOW_TILE;
+        if (key < s.end && key + FLOW_KEYS > s.begin) {       // warp-uniform
+          const uint32_t at = ring + (i % FLOW_STAGES) * F::STAGE;
+          bool done;
+          if (!decltype(far_tag)::value && live == all_live && key >= last_begin && key + FLOW_KEYS <= first_end) done = attend(std::true_type(), std::false_type(), key, at, live);
+          else done = attend(std::false_type(), far_tag, key, at, live);
+          if (!done) return;
+        }
+        __syncwarp();
 #pragma unroll
-      for (int k = 0; k < FLOW_STAGES - 2; k++) live_of[k] = live_of[k + 1];
-      live_of[FLOW_STAGES - 2] = issue(i + FLOW_STAGES - 1, src);
-      src = next;
+        for (int k = 0; k < FLOW_STAGES - 2; k++) live_of[k] = live_of[k + 1];
+        live_of[FLOW_STAGES - 2] = issue(i + FLOW_STAGES - 1, src);
+        src = source();
+      }
+    };
+    walk(std::false_type());
+    const bool far = i < nt;      // of this warp
+    if (far) {
+#pragma unroll
+      for (int c = 0; c < 2 * NQ; c++) apart[c] = rise_at[c] == -INFINITY ? -INFINITY : (float)(R - 6);
+      walk(std::true_type());
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
@@ -588,11 +660,13 @@ __global__ void __launch_bounds__(32 * FLOW_WARPS, Flow<D, NQ>::BLOCKS) kv4_atte
     // ---- the four warps' results meet in shared memory
     {
       float* mine = reinterpret_cast<float*>(my_smem);
-      const float unit = __uint_as_float((uint32_t)(127 + 24 - 6) << 23);
-      const float lower = __uint_as_float((uint32_t)(127 + R) << 23);       // R >= -112
+      constexpr float LEVEL = 16777216.0f;      // the levels are multiples of 2^-24
 #pragma unroll
       for (int c = 0; c < 2 * NQ; c++) {
         const int r = (c >> 1) * 8 + 2 * t + (c & 1);
+        // the values' reference point in two factors: 2^(R - 6), R >= -112
+        const float root = ex2(0.5f * apart[c]);
+        const float unit = LEVEL * (far ? root : 0.015625f), lower = far ? root : __uint_as_float((uint32_t)(127 + R) << 23);
         const float2 l2 = unpair(l[c >> 1]), v2 = unpair(vsum[c >> 1]);
         float lc = c & 1 ? l2.y : l2.x, vc = c & 1 ? v2.y : v2.x;
 #pragma unroll

@@ -28,6 +28,16 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Weights of the values carry the values' steps and are rounded to fp16, so what the largest step leaves of a smaller one counts.  Up
+// to this many powers of two between the steps met, all rows of a block share one power of two for them: a row that sees only the
+// smallest steps then keeps fp16's eleven bits down to weights of 2^-10 of its reference point.  Steps further apart (a row that is
+// masked or all but weightless may hold any) take a path on which each row has its own.
+constexpr int STEP_SPAN = 10;
+// Whether steps lie too far apart: 2^top is above the largest, `under` the fp32 bits of the smallest (not 0), less 1; all ones: none.
+__device__ __forceinline__ bool steps_far_apart(int top, uint32_t under) {
+  return under != 0xffffffffu && top + 126 - (int)((under + 1u) >> 23) > STEP_SPAN;
+}
+
 // Two fp32 in one instruction.
 struct Pair { unsigned long long v; };
 __device__ __forceinline__ Pair pair(float x, float y) {

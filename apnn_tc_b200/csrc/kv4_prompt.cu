@@ -11,7 +11,8 @@
 //   warp 12      issues the MMAs, as a whole warp with uniform operands
 // The scores' scale and offset belong to the key: s = scale (step_j (q . n_j) + low_j sum q), three packed operations for
 // two scores, their parameters broadcast from shared memory.  Weights as on the flow kernel (kv4_attention.cu): they carry the value's step,
-// relative to a reference point that follows the running maximum in steps of 2^8, so O is rescaled in TMEM only when it moves.
+// relative to a reference point that follows the running maximum in steps of 2^8, so O is rescaled in TMEM only when it moves.  From
+// the first tile on whose steps lie too far from those before, weights are taken against a second reference point of each row.
 // Registers: 96 / 184 / 184 / 48 for the four warpgroups out of the 128 each was launched with (setmaxnreg; a thread keeps 128 scores).
 // Bounds per 128 x 128 tile and 128 elements: 1024 clk of MMAs, 1024 of exponentials, about 950 issue slots of softmax and 200 of
 // spreading (one K / V tile serves both row tiles).  Measured: 8192 tokens, 32 heads on 8, causal, 881 us, 624 TFLOP/s, 0.37 of the
@@ -40,7 +41,9 @@ struct Prompt {
   static constexpr int ROWS = TILE * QT;
   static constexpr int OPERAND = D / 64 * 16384;          // 128 rows of D fp16, in 64-element columns of 16 KiB
   static constexpr int K_AT = QT * OPERAND, V_AT = K_AT + DEPTH * OPERAND, PAR_AT = V_AT + DEPTH * OPERAND;
-  static constexpr int SLOT = 2 * 64 * 16 + 64;           // pairs of keys: (step, step, mid, mid) of the keys, of the values; live bits and exponents
+  // pairs of keys: (step, step, mid, mid) of the keys, of the values; then live bits (4 words), the largest steps (4), R, whether steps
+  // lie far apart, and the smallest steps (4, at 48)
+  static constexpr int SLOT = 2 * 64 * 16 + 64;
   static constexpr int BAR_AT = PAR_AT + SLOTS * SLOT;
   static constexpr int SMEM = BAR_AT + 256 + 1024;
   static constexpr int O_COLUMN = QT * TILE;              // S of the row tiles first
@@ -261,6 +264,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
     };
     bool ok = true;
     int R = -112;
+    uint32_t under = 0xffffffffu;      // as steps_far_apart takes it
     long long at = locate(0), at1 = locate(1);
     fetch(0, 0, at);
     fetch(1, 0, at);
@@ -291,10 +295,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
         sts32(slot_at + 1024 + 8, __float_as_uint(fmaf(8.0f, f.x, f.y)));
         const uint32_t bits = __float_as_uint(fabsf(f.x));
         const uint32_t lives = __ballot_sync(0xffffffffu, live);
-        const uint32_t most = __reduce_max_sync(0xffffffffu, live && bits < 0x7f800000u && (tile0 + j) * TILE + key >= key_begin ? bits : 0u);
+        const uint32_t counted = live && bits < 0x7f800000u && (tile0 + j) * TILE + key >= key_begin ? bits : 0u;
+        const uint32_t most = __reduce_max_sync(0xffffffffu, counted), least = __reduce_min_sync(0xffffffffu, counted - 1u);
         if (lane == 0) {
           sts32(head_at + warp * 4, lives);
           sts32(head_at + 16 + warp * 4, most);
+          sts32(head_at + 48 + warp * 4, least);
         }
       }
       asm volatile("bar.sync 1, 128;" ::: "memory");
@@ -302,8 +308,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
         // 2^R is above every value step met so far, within fp32's range: the largest of the four warps' keys
         const uint32_t all = max(max(lds(head_at + 16), lds(head_at + 20)), max(lds(head_at + 24), lds(head_at + 28)));
         R = max(R, min((int)(all >> 23) - 126, 127));
-        if (key == 0) sts32(head_at + 32, (uint32_t)R);
-        sts32(slot_at + 1024, __float_as_uint(f.x * power2(6 - R)));
+        under = min(under, min(min(lds(head_at + 48), lds(head_at + 52)), min(lds(head_at + 56), lds(head_at + 60))));
+        const bool far = steps_far_apart(R, under);
+        if (far) under = 0u;      // and from here on: R is -112 at least
+        if (key == 0) {
+          sts32(head_at + 32, (uint32_t)R);
+          sts32(head_at + 36, far ? 1u : 0u);
+        }
+        uint32_t held = __float_as_uint(f.x * power2(6 - R));
+        if (far) held = (__float_as_uint(__log2f(fabsf(f.x))) & ~1u) | (f.x < 0.0f ? 1u : 0u);      // log2, the sign in its lowest bit (2^-23 of an exponent)
+        sts32(slot_at + 1024, held);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
@@ -370,12 +384,27 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
         float below = 0.0f, rise_at = -INFINITY;                    // minus the reference point (0: none yet), and 8 above it
         int R = -112;      // the values' steps come times 2^(6 - R)
         bool ok = true;
-        for (int j = 0; j < tiles && ok; j++) {
+        int j = 0;
+        auto rescale = [&](float k) {      // O of the row, behind the product that added to it last
+          ok = __all_sync(0xffffffffu, mbar_wait(o_done(qt), (uint32_t)(j - 1) & 1u));
+          if (!ok) return;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_at + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * k);
+            tmem_st32(o_at + c, o);
+          }
+        };
+        for (; j < tiles && ok; j++) {
           const uint32_t slot = base + P::PAR_AT + (uint32_t)(j % SLOTS) * P::SLOT;
           const PairPair* pars = reinterpret_cast<const PairPair*>(smem_raw + (slot - raw));      // keys, then values
           const int key = (tile0 + j) * TILE;
           ok = __all_sync(0xffffffffu, mbar_wait(par_full(j % SLOTS), (uint32_t)(j / SLOTS) & 1u) && mbar_wait(s_full(qt), (uint32_t)j & 1u));
-          if (!ok) break;
+          if (!ok || lds(slot + 2084) != 0u) break;
           tc_fence_after();
           float sc[TILE];
           tmem_ld32(s_at, *reinterpret_cast<uint32_t(*)[32]>(&sc[0]));
@@ -427,19 +456,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
               vsum[c] = mul2(vsum[c], pair(keep, keep));
             }
             if (j > 0) {
-              ok = __all_sync(0xffffffffu, mbar_wait(o_done(qt), (uint32_t)(j - 1) & 1u));
+              rescale(keep * shrink);
               if (!ok) break;
-              tc_fence_after();
-              const float k = keep * shrink;
-#pragma unroll 1
-              for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
-                tmem_ld32(o_at + c, o);
-                tmem_ld_wait();
-#pragma unroll
-                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * k);
-                tmem_st32(o_at + c, o);
-              }
             }
           }
           const Pair below2 = pair(below, below);
@@ -477,6 +495,93 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
           __syncwarp();
           if (lane == 0) mbar_arrive(w_full(qt));
         }
+        // ---- the tiles from the first on whose steps lie far apart and come as their logarithms.  Two passes over the scores in TMEM, 32
+        // columns at a time: weights of 32 columns take 16, which were read by then (4096 tokens, 32 heads on 8, D = 128: 390 us against
+        // 240; with the scores in registers and the ordinary tiles' loop shared 434 and 280).
+        const bool far = ok && j < tiles;
+        float apart = far && rise_at != -INFINITY ? (float)(R - 6) : -INFINITY;      // the values' reference point less the softmax's
+        for (; j < tiles && ok; j++) {
+          const uint32_t slot = base + P::PAR_AT + (uint32_t)(j % SLOTS) * P::SLOT;
+          const PairPair* pars = reinterpret_cast<const PairPair*>(smem_raw + (slot - raw));
+          const int key = (tile0 + j) * TILE;
+          ok = __all_sync(0xffffffffu, mbar_wait(par_full(j % SLOTS), (uint32_t)(j / SLOTS) & 1u) && mbar_wait(s_full(qt), (uint32_t)j & 1u));
+          if (!ok) break;
+          tc_fence_after();
+          auto scores = [&](int c, float (&sc)[32]) -> uint32_t {      // of 32 keys, and which of them the row sees
+            const uint32_t seen = lds(slot + 2048 + 4 * c) & bit_range(begin - key - 32 * c, end - key - 32 * c);
+            __syncwarp();
+            tmem_ld32(s_at + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&sc[0]));
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const Pair step = pars[16 * c + e / 2].step, mid = pars[16 * c + e / 2].mid;
+              const float2 v = unpair(fma2(mul2(pair(sc[e], sc[e + 1]), step), qf2, mul2(mid, ql2)));
+              sc[e] = (seen >> e) & 1u ? v.x : -INFINITY;
+              sc[e + 1] = (seen >> (e + 1)) & 1u ? v.y : -INFINITY;
+            }
+            return seen;
+          };
+          float top = -INFINITY, most = -INFINITY;      // of the scores, and of them and the steps; NaN counts as none
+#pragma unroll 1
+          for (int c = 0; c < 4; c++) {
+            float sc[32];
+            scores(c, sc);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 z = unpair(add2(pair(sc[e], sc[e + 1]), pars[64 + 16 * c + e / 2].step));
+              top = fmaxf(top, fmaxf(sc[e], sc[e + 1]));
+              most = fmaxf(most, fmaxf(z.x, z.y));
+            }
+          }
+          if (__any_sync(0xffffffffu, top > rise_at)) {
+            const float m = rise_at == -INFINITY ? -INFINITY : -below;
+            top = fmaxf(top, m);
+            const float keep = m == top ? 1.0f : ex2(m - top);
+            if (m != top) apart += m - top;      // the values' own point stays; -inf where no key was met
+            below = top == -INFINITY ? 0.0f : -top;
+            rise_at = top + 8.0f;
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+              l[c] = mul2(l[c], pair(keep, keep));
+              vsum[c] = mul2(vsum[c], pair(keep, keep));
+            }
+          }
+          most += below;
+          if (__any_sync(0xffffffffu, most > apart + 14.0f)) {
+            const float up = fmaxf(apart, most - 6.0f), k = up == apart ? 1.0f : ex2(apart - up);
+            apart = up;
+            if (j > 0) {
+              rescale(k);
+              if (!ok) break;
+            }
+          }
+          const float from = apart == -INFINITY ? 0.0f : -apart;
+#pragma unroll 1
+          for (int c = 0; c < 4; c++) {
+            float sc[32];
+            const uint32_t seen = scores(c, sc);
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const Pair step = pars[64 + 16 * c + e / 2].step;
+              const float2 mid = unpair(pars[64 + 16 * c + e / 2].mid), lg = unpair(step);
+              const Pair z = add2(pair(sc[e], sc[e + 1]), pair(below, below));
+              const float2 z2 = unpair(z), x = unpair(add2(z, add2(step, pair(from, from))));
+              const Pair ex = pair(ex2(z2.x), ex2(z2.y));
+              const bool on0 = (seen >> e) & 1u, on1 = (seen >> (e + 1)) & 1u;      // a masked place may hold NaN
+              l[0] = add2(l[0], ex);
+              vsum[0] = fma2(ex, pair(on0 ? mid.x : 0.0f, on1 ? mid.y : 0.0f), vsum[0]);
+              const float f0 = __uint_as_float(__float_as_uint(ex2(x.x)) | (__float_as_uint(lg.x) << 31));
+              const float f1 = __uint_as_float(__float_as_uint(ex2(x.y)) | (__float_as_uint(lg.y) << 31));
+              w[e / 2] = pack2<false>(on0 ? f0 : 0.0f, on1 ? f1 : 0.0f);
+            }
+            tmem_st16(s_at + 16 * c, w);
+          }
+          tmem_st_done();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(w_full(qt));
+        }
         // ---- the row's output
         float total, mids;
         {
@@ -491,7 +596,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const PromptPara
         if (!ok && lane == 0) give_up(2);
         if (ok) {
           const float m = rise_at == -INFINITY ? -INFINITY : -below;
-          const float unit = power2(-6), lower = power2(R);
+          // the values' reference point in two factors: 2^(R - 6)
+          const float root = ex2(0.5f * apart), unit = far ? root : power2(-6), lower = far ? root : power2(R);
           const bool none = total == 0.0f;      // no key seen
           const float inv = none ? 0.0f : 1.0f / total;
           float* part_row = pp.split > 1 ? pp.parts + ((((long long)bh * pp.blocks_q + qb) * pp.split + part) * P::ROWS + qt * TILE + r) * (D + 4) : nullptr;

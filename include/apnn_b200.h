@@ -487,8 +487,11 @@ apnn_status apnn_kv4_read(void *stream, const apnn_kv4_cache *cache, const apnn_
 /* Attention of the batch's rows over the cache.  Query head h reads key head h / (q_heads / heads).  A row at position p
  * sees the keys j < kv_len (causal: j <= p; with a window also j > p - window); masked places are never multiplied, whatever they hold.
  *   Out = softmax(scale * q k^T) v;   lse = ln sum exp(scale * q k^T);   a row that sees no key: Out 0, lse -infinity.
- * Products of levels are exact, softmax statistics and sums are held in 32 bits, the weights of the values in fp16
- * relative to the row's maximum; one rounding at the store.  Results do not depend on timing (no atomics on values).
+ * Products of levels are exact, softmax statistics and sums are held in 32 bits, the weights of the values (times the values'
+ * steps) in fp16 relative to the row's largest; one rounding at the store.  Results do not depend on timing (no atomics on
+ * values).  Value rows may have any steps; where those that a call meets lie more than 2^10 apart, it takes a quarter longer for
+ * single tokens and up to two thirds for prompts.  Values are summed at up to 2^8 times their weight before the division, so in a
+ * bf16 cache values times 2^8 times the number of keys have to stay below 2^128.
  * At most 2^30 positions in a table row and 2^31 tiles of 128 of them over all sequences and heads (else APNN_ERR_UNSUPPORTED).
  * workspace: apnn_kv4_attention_workspace_bytes of device memory, 16-byte aligned, for one call at a time. */
 typedef struct apnn_kv4_attention_args {
