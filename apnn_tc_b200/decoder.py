@@ -7,7 +7,8 @@
 * ``kv4_read`` -- rows back out of the cache; ``kv4_attention`` -- attention over it.
 
 The reference has no counterpart (it runs convolutional networks).  Every call goes through the C ABI on the current stream of
-the tensors' device; nothing here computes on the CPU, and nothing synchronises except ``kv4_attention_check``.
+the tensors' device; nothing here computes on the CPU, and nothing synchronises except ``kv4_attention_check``.  The operators
+serve: there is no backward pass, and a tensor that requires a gradient is refused outside ``torch.no_grad()``.
 """
 from __future__ import annotations
 
@@ -38,6 +39,11 @@ def _launch(index: int, what: str, fn, *args) -> None:
         _cabi.check(status, what)
 
 
+def _refuse_gradient(what: str) -> None:
+    if torch.is_grad_enabled():
+        raise ValueError(f"{what} has no backward pass and was given a tensor that requires a gradient; call it under torch.no_grad()")
+
+
 def _on(index: int, name: str, t: torch.Tensor) -> int:
     """The address of a tensor that has to lie on device ``index``."""
     if t.get_device() != index:
@@ -57,6 +63,9 @@ def linear_planes(x: torch.Tensor, planes: torch.Tensor, scale: torch.Tensor, *,
     multiple of 1/2 in 0..15.  activation: "none" | "relu" | "silu" | "gelu" | "gelu_tanh".  residual and out: [M, N] of x's type,
     or float32 (``out_dtype``), unit element stride; residual may be out.  M may be 0.
     """
+    if (x.requires_grad or scale.requires_grad or (bias is not None and bias.requires_grad)
+            or (residual is not None and residual.requires_grad) or (out is not None and out.requires_grad)):
+        _refuse_gradient("linear_planes")
     if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor (there is no CPU path)")
     if x.dim() != 2 or planes.dim() != 3:
@@ -225,6 +234,10 @@ def kv4_append(cache: KVCache4, batch: KVBatch, k: torch.Tensor, v: torch.Tensor
     k, v: [rows, heads, D]; q: [rows, q_heads, D] or None; views of one fused projection are taken as they are.  q_norm,
     k_norm: [D] weights in the cache's type.  rotary: float32 [positions, rotary_dim], rotary_dim/2 cosines and as many sines.
     """
+    if (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad) or (q_out is not None and q_out.requires_grad)
+            or (q_norm is not None and q_norm.requires_grad) or (k_norm is not None and k_norm.requires_grad)
+            or (rotary is not None and rotary.requires_grad)):
+        _refuse_gradient("kv4_append")
     index = _same(cache, batch)
     rows, heads, k_stride = _rows("k", k, cache)
     v_rows, v_heads, v_stride = _rows("v", v, cache)
@@ -301,6 +314,8 @@ def kv4_attention(cache: KVCache4, batch: KVBatch, q: torch.Tensor, *, scale: Op
     positions back a row sees, itself included (0: all); needs causal.  lse: True, or a float32 [rows, q_heads] to write.
     workspace: ``kv4_attention_workspace_bytes`` bytes (uint8), used by one call at a time; allocated here if None.
     """
+    if q.requires_grad or (out is not None and out.requires_grad):
+        _refuse_gradient("kv4_attention")
     index = _same(cache, batch)
     rows, q_heads, q_stride = _rows("q", q, cache)
     if out is None:
