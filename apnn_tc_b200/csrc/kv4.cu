@@ -12,6 +12,7 @@ apnn_status kv4_view(const apnn_kv4_cache* c, Kv4View* v) {
   if (c->type != APNN_TYPE_BF16 && c->type != APNN_TYPE_FP16) return APNN_ERR_INVALID_ARG;
   if (c->pages <= 0 || c->heads <= 0) return APNN_ERR_INVALID_ARG;
   if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return APNN_ERR_UNSUPPORTED;
+  if (c->heads > MOST_HEADS) return APNN_ERR_UNSUPPORTED;
   if (c->page_size < 8 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)) != 0) return APNN_ERR_UNSUPPORTED;
   v->head_bytes = (long long)c->page_size * (c->head_dim + 8);
   if ((reinterpret_cast<uintptr_t>(c->data) & 15u) != 0 || c->page_stride % 16 != 0) return APNN_ERR_ALIGNMENT;
@@ -346,7 +347,7 @@ apnn_status apnn_kv4_append(void* stream, const apnn_kv4_cache* cache, const apn
   const int D = cache->head_dim;
   if ((a->q != nullptr) != (a->q_out != nullptr) || (a->q && a->q_heads <= 0)) return APNN_ERR_INVALID_ARG;
   if (a->rotary_dim < 0 || a->rotary_dim > D || (a->interleaved != 0 && a->interleaved != 1)) return APNN_ERR_INVALID_ARG;
-  if (a->rotary_dim % 16 != 0) return APNN_ERR_UNSUPPORTED;
+  if (a->rotary_dim % 16 != 0 || (a->q && a->q_heads > MOST_HEADS)) return APNN_ERR_UNSUPPORTED;
   if (a->rotary_dim > 0 && (!a->rotary || a->rotary_rows <= 0)) return APNN_ERR_INVALID_ARG;
   if (!(a->eps >= 0.0) || !(a->eps < 1e30)) return APNN_ERR_INVALID_ARG;
   const long long row = (long long)cache->heads * D;

@@ -23,6 +23,8 @@ struct Kv4Batch {
   int sequences, table_width, max_q, rows;
 };
 
+constexpr int MOST_HEADS = 1 << 20;      // of keys, of queries: what a row's pieces are counted in
+
 // Checks shared by the entry points; fill the kernels' views.
 apnn_status kv4_view(const apnn_kv4_cache* c, Kv4View* v);
 apnn_status kv4_batch(const apnn_kv4_batch* b, int rows, Kv4Batch* out);

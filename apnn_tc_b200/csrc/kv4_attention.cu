@@ -881,7 +881,7 @@ size_t apnn_kv4_attention_workspace_bytes(const apnn_kv4_cache* cache, const apn
   Kv4View view = {};
   Kv4Batch geo = {};
   if (kv4_view(cache, &view) != APNN_OK || kv4_batch(batch, 1, &geo) != APNN_OK || q_heads <= 0 || q_heads % cache->heads != 0 ||
-      too_long(cache, batch))
+      q_heads > MOST_HEADS || too_long(cache, batch))
     return 0;
   const int group = q_heads / cache->heads;
   if ((long long)batch->max_q * group > largest_rows(cache->head_dim)) return kv4_prompt_workspace_bytes(cache, batch, group);
@@ -896,7 +896,7 @@ apnn_status apnn_kv4_attention(void* stream, const apnn_kv4_cache* cache, const 
   if (st == APNN_OK) st = kv4_batch(batch, a->rows, &p.batch);
   if (st != APNN_OK) return st;
   if (a->q_heads <= 0 || a->q_heads % cache->heads != 0) return APNN_ERR_INVALID_ARG;
-  if (too_long(cache, batch)) return APNN_ERR_UNSUPPORTED;
+  if (too_long(cache, batch) || a->q_heads > MOST_HEADS) return APNN_ERR_UNSUPPORTED;
   if ((a->causal != 0 && a->causal != 1) || a->window < 0 || (a->window > 0 && !a->causal)) return APNN_ERR_INVALID_ARG;
   if (!std::isfinite(a->scale)) return APNN_ERR_INVALID_ARG;
   const long long row = (long long)a->q_heads * cache->head_dim;

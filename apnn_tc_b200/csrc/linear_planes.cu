@@ -212,7 +212,9 @@ extern "C" apnn_status apnn_linear_planes(void* stream, int wbits, const void* W
   if (d->activation < APNN_ACT_NONE || d->activation > APNN_ACT_GELU_TANH) return APNN_ERR_INVALID_ARG;
   if (!(d->zero >= 0.0f && d->zero <= 15.0f) || d->zero * 2.0f != std::floor(d->zero * 2.0f)) return APNN_ERR_INVALID_ARG;
   if (d->ldx < K || d->ldo < N || (d->residual && d->ldr < N)) return APNN_ERR_INVALID_ARG;
-  if (wbits < 1 || wbits > 4 || (long long)N * wbits > 0x7fffffffll) return APNN_ERR_UNSUPPORTED;      // rows of all planes are counted in 32 bits
+  if (wbits < 1 || wbits > 4) return APNN_ERR_UNSUPPORTED;
+  // rows of X, rows of all planes and elements of K are counted in 32 bits, up to the ends of the last tile (256 rows) and block (512 of K)
+  if (M > 0x7fffffff - 256 || (long long)N * wbits > 0x7fffffff - 256 || K > 0x7fffffff - 512) return APNN_ERR_UNSUPPORTED;
   const uintptr_t element = d->out_type == APNN_TYPE_FP32 ? 3u : 1u;
   if (((reinterpret_cast<uintptr_t>(W) | reinterpret_cast<uintptr_t>(X)) & 15u) != 0 || d->ldx % 8 != 0 ||
       ((reinterpret_cast<uintptr_t>(Out) | reinterpret_cast<uintptr_t>(d->residual)) & element) != 0 ||

@@ -354,4 +354,6 @@ def kv4_attention(cache: KVCache4, batch: KVBatch, q: torch.Tensor, *, scale: Op
 
 def kv4_attention_check(workspace: torch.Tensor) -> None:
     """Synchronise and raise if the attention that last used ``workspace`` gave up on a wait."""
+    if not workspace.is_cuda:
+        raise ValueError("workspace must be a CUDA tensor")
     _launch(workspace.get_device(), "apnn_kv4_attention_check", _cabi.lib().apnn_kv4_attention_check, workspace.data_ptr())

@@ -401,7 +401,8 @@ enum {
  * zero: a multiple of 1/2 in 0..15, so that level - zero is exact in either type (1/2 with one plane: weights of
  * -scale/2 and +scale/2; (2^wbits - 1)/2: symmetric levels).  bias and residual may be null; residual may be Out itself
  * (same stride).  Values of X that are not finite make their row NaN or infinite and touch no other row.
- * Rules: W, X 16-byte aligned, ldx a multiple of 8; Out and residual aligned to their element; M, N, K >= 1 (ragged edges handled).
+ * Rules: W, X 16-byte aligned, ldx a multiple of 8; Out and residual aligned to their element; M, N, K >= 1 (ragged edges handled),
+ * M and N * wbits up to 2^31 - 257, K up to 2^31 - 513 (else APNN_ERR_UNSUPPORTED).
  * status_flag: null, or 4 bytes of device memory, written 0 at launch and non-zero if a bounded wait expires. */
 typedef struct apnn_linear_desc {
   uint32_t struct_size;
@@ -422,7 +423,7 @@ apnn_status apnn_linear_planes(void *stream, int wbits, const void *W, const voi
  *   key levels [page_size][D/2] (two per byte, the even element in the low half), value levels [page_size][D/2],
  *   (step, lowest) of every key row [page_size][2], (step, lowest) of every value row [page_size][2], in `type`,
  * page_size * (D + 8) bytes, heads one after the other, pages page_stride bytes apart (a multiple of 16).  An element
- * stands for step * level + lowest.  D is 64, 128 or 256, page_size a power of two from 8 to 1024. */
+ * stands for step * level + lowest.  D is 64, 128 or 256, page_size a power of two from 8 to 1024, at most 2^20 heads (of queries, too). */
 typedef struct apnn_kv4_cache {
   uint32_t struct_size;
   int32_t type;          /* APNN_TYPE_BF16 or APNN_TYPE_FP16: of the row parameters, and of q, k, v and out */
@@ -492,7 +493,8 @@ apnn_status apnn_kv4_read(void *stream, const apnn_kv4_cache *cache, const apnn_
  * values).  Value rows may have any steps; where those that a call meets lie more than 2^10 apart, it takes a quarter longer for
  * single tokens and up to two thirds for prompts.  Values are summed at up to 2^8 times their weight before the division, so in a
  * bf16 cache values times 2^8 times the number of keys have to stay below 2^128.
- * At most 2^30 positions in a table row and 2^31 tiles of 128 of them over all sequences and heads (else APNN_ERR_UNSUPPORTED).
+ * At most 2^30 positions in a table row, 2^31 tiles of 128 of them over all sequences and heads, and 65535 * 256 rows of a sequence and key
+ * head (max_q times q_heads / heads; half of it at D = 256), else APNN_ERR_UNSUPPORTED.
  * workspace: apnn_kv4_attention_workspace_bytes of device memory, 16-byte aligned, for one call at a time. */
 typedef struct apnn_kv4_attention_args {
   uint32_t struct_size;
