@@ -30,7 +30,7 @@ EXPORTS = (
     "apnn_conv2d_workspace_bytes", "apnn_conv2d_check", "apnn_conv2d_i8", "apnn_bit_compress", "apnn_quantize_pack", "apnn_quantize_im2col", "apnn_create",
     "apnn_destroy", "apnn_gemm_host", "apnn_conv2d_host", "apnn_probe_peak", "apnn_quantize_im2col_i8", "apnn_quantize_window_rows_i8", "apnn_quantize_blocks_i8", "apnn_maxpool2x2_i8", "apnn_requantize_i32",
     "apnn_conv2d_fp4", "apnn_linear_fp4", "apnn_gemm_planes", "apnn_conv2d_i8_to_fp4", "apnn_maxpool2x2_rows",
-    "apnn_linear_planes", "apnn_kv4_append", "apnn_kv4_read", "apnn_kv4_attention", "apnn_kv4_attention_workspace_bytes",
+    "apnn_linear_planes", "apnn_linear_planes_plan", "apnn_kv4_append", "apnn_kv4_read", "apnn_kv4_attention", "apnn_kv4_attention_workspace_bytes",
     "apnn_kv4_attention_check",
 )
 
@@ -174,6 +174,7 @@ def lib() -> ctypes.CDLL:
     L.apnn_gemm_host.argtypes = [vp, i, i, i, vp, vp, vp, i, i, i, ep]
     L.apnn_conv2d_host.argtypes = [vp, i, i, vp, vp, vp, i, i, i, i, i, i, i, ep]
     L.apnn_linear_planes.argtypes = [vp, i, vp, vp, vp, i, i, i, vp, vp]
+    L.apnn_linear_planes_plan.argtypes = [i, i, i, vp, vp, vp]
     L.apnn_kv4_append.argtypes = [vp, vp, vp, vp]
     L.apnn_kv4_read.argtypes = [vp, vp, vp, vp, vp, i]
     L.apnn_kv4_attention_workspace_bytes.restype = sz

@@ -50,7 +50,11 @@ __device__ __forceinline__ void store_element(const LinearParams& p, long long m
   }
 }
 
-// More than a few rows (linear_tile.cu).
+// More than a few rows (linear_tile.cu): blocks that share a tile (1 or 2), rows of X in it, blocks of a cluster that share its K.
+struct LinearPlan {
+  int ctas, tn, split;
+};
+LinearPlan linear_tile_plan(int M, int N, int kwords);
 apnn_status linear_tile(cudaStream_t s, const LinearParams& p, bool bf16);
 
 }  // namespace apnn

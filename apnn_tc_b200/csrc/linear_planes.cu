@@ -198,10 +198,48 @@ void (*few_rows_kernel(int wbits))(LinearParams) {
   return wbits == 1 ? linear_few_rows_kernel<1, BF16> : wbits == 2 ? linear_few_rows_kernel<2, BF16> : wbits == 3 ? linear_few_rows_kernel<3, BF16> : linear_few_rows_kernel<4, BF16>;
 }
 
+long long few_x_bytes(int M, int kwords, int split) {
+  const int blocks = (kwords + 15) / 16;
+  return (long long)M * ((blocks + split - 1) / split) * 1024;
+}
+
+// Blocks that share K on the kernel of few rows, 0 where it does not take the call.  The split whose waves (two blocks to an SM) of
+// 512-element steps are fewest; beginning and ending a block counts as two steps.  A split is taken as soon as X fits.
+int few_rows_split(int M, int N, int kwords) {
+  if (M > FEW_ROWS) return 0;
+  const int tiles = (N + FEW_TILE - 1) / FEW_TILE, blocks = (kwords + 15) / 16, slots = 2 * device_sm_count();
+  int split = 0;
+  long long best = -1;
+  for (int s = 1; s <= FEW_SPLIT && s <= blocks; s *= 2) {
+    const long long steps = ((long long)tiles * s + slots - 1) / slots * ((blocks + s - 1) / s + 2);
+    if (few_x_bytes(M, kwords, s) <= FEW_X_BYTES && (best < 0 || steps < best)) {
+      best = steps;
+      split = s;
+    }
+  }
+  return split;
+}
+
+// What the kernels' counts in 32 bits hold: rows of X, rows of all planes and elements of K, up to the ends of the last tile (256 rows)
+// and block (512 of K)
+bool sizes_held(int M, long long rows, int K) { return M <= 0x7fffffff - 256 && rows <= 0x7fffffff - 256 && K <= 0x7fffffff - 512; }
+
 }  // namespace
 }  // namespace apnn
 
 using namespace apnn;
+
+extern "C" apnn_status apnn_linear_planes_plan(int M, int N, int K, int* blocks, int* rows, int* split) {
+  if (M <= 0 || N <= 0 || K <= 0 || !blocks || !rows || !split) return APNN_ERR_INVALID_ARG;
+  if (!sizes_held(M, N, K)) return APNN_ERR_UNSUPPORTED;
+  const int kwords = (K + 127) / 128 * 4;
+  LinearPlan plan = {0, FEW_ROWS, few_rows_split(M, N, kwords)};
+  if (plan.split == 0) plan = linear_tile_plan(M, N, kwords);
+  *blocks = plan.ctas;
+  *rows = plan.tn;
+  *split = plan.split;
+  return APNN_OK;
+}
 
 extern "C" apnn_status apnn_linear_planes(void* stream, int wbits, const void* W, const void* X, void* Out, int M, int N, int K,
                                           const apnn_linear_desc* d, int* status_flag) {
@@ -213,8 +251,7 @@ extern "C" apnn_status apnn_linear_planes(void* stream, int wbits, const void* W
   if (!(d->zero >= 0.0f && d->zero <= 15.0f) || d->zero * 2.0f != std::floor(d->zero * 2.0f)) return APNN_ERR_INVALID_ARG;
   if (d->ldx < K || d->ldo < N || (d->residual && d->ldr < N)) return APNN_ERR_INVALID_ARG;
   if (wbits < 1 || wbits > 4) return APNN_ERR_UNSUPPORTED;
-  // rows of X, rows of all planes and elements of K are counted in 32 bits, up to the ends of the last tile (256 rows) and block (512 of K)
-  if (M > 0x7fffffff - 256 || (long long)N * wbits > 0x7fffffff - 256 || K > 0x7fffffff - 512) return APNN_ERR_UNSUPPORTED;
+  if (!sizes_held(M, (long long)N * wbits, K)) return APNN_ERR_UNSUPPORTED;
   const uintptr_t element = d->out_type == APNN_TYPE_FP32 ? 3u : 1u;
   if (((reinterpret_cast<uintptr_t>(W) | reinterpret_cast<uintptr_t>(X)) & 15u) != 0 || d->ldx % 8 != 0 ||
       ((reinterpret_cast<uintptr_t>(Out) | reinterpret_cast<uintptr_t>(d->residual)) & element) != 0 ||
@@ -240,43 +277,28 @@ extern "C" apnn_status apnn_linear_planes(void* stream, int wbits, const void* W
   p.out_f32 = d->out_type == APNN_TYPE_FP32;
   p.zero = d->zero;
   p.status_flag = status_flag;
-  if (M <= FEW_ROWS) {
+  p.split = few_rows_split(M, N, p.kwords);
+  if (p.split > 0) {
     cudaLaunchConfig_t cfg = {};
-    // The split whose waves (two blocks to an SM) of 512-element steps are fewest; beginning and ending a block counts as two
-    // steps.  A split is taken as soon as X fits.
-    const int tiles = (N + FEW_TILE - 1) / FEW_TILE, blocks = (p.kwords + 15) / 16, slots = 2 * device_sm_count();
-    auto x_bytes = [&](int s) { return (long long)M * ((blocks + s - 1) / s) * 1024; };
-    int split = 1;
-    long long best = -1;
-    for (int s = 1; s <= FEW_SPLIT && s <= blocks; s *= 2) {
-      const long long steps = ((long long)tiles * s + slots - 1) / slots * ((blocks + s - 1) / s + 2);
-      if (x_bytes(s) <= FEW_X_BYTES && (best < 0 || steps < best)) {
-        best = steps;
-        split = s;
-      }
+    void (*const kernel)(LinearParams) = d->x_type == APNN_TYPE_BF16 ? few_rows_kernel<true>(wbits) : few_rows_kernel<false>(wbits);
+    cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(kernel), FEW_X_BYTES);
+    if (e != cudaSuccess) return cuda_fail(e, "linear_few_rows_kernel shared memory");
+    cfg.gridDim = dim3((unsigned)((N + FEW_TILE - 1) / FEW_TILE * p.split), 1, 1);
+    cfg.blockDim = dim3(32 * FEW_WARPS, 1, 1);
+    cfg.dynamicSmemBytes = (size_t)few_x_bytes(M, p.kwords, p.split);
+    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[2];
+    cfg.numAttrs = pdl_attribute(attr);
+    if (p.split > 1) {
+      attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+      attr[cfg.numAttrs].val.clusterDim.x = (unsigned)p.split;
+      attr[cfg.numAttrs].val.clusterDim.y = 1;
+      attr[cfg.numAttrs].val.clusterDim.z = 1;
+      cfg.numAttrs++;
     }
-    if (x_bytes(split) <= FEW_X_BYTES) {
-      p.split = split;
-      void (*const kernel)(LinearParams) = d->x_type == APNN_TYPE_BF16 ? few_rows_kernel<true>(wbits) : few_rows_kernel<false>(wbits);
-      cudaError_t e = ensure_max_smem(reinterpret_cast<const void*>(kernel), FEW_X_BYTES);
-      if (e != cudaSuccess) return cuda_fail(e, "linear_few_rows_kernel shared memory");
-      cfg.gridDim = dim3((unsigned)(tiles * split), 1, 1);
-      cfg.blockDim = dim3(32 * FEW_WARPS, 1, 1);
-      cfg.dynamicSmemBytes = (size_t)x_bytes(split);
-      cfg.stream = reinterpret_cast<cudaStream_t>(stream);
-      cudaLaunchAttribute attr[2];
-      cfg.numAttrs = pdl_attribute(attr);
-      if (split > 1) {
-        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attr[cfg.numAttrs].val.clusterDim.x = (unsigned)split;
-        attr[cfg.numAttrs].val.clusterDim.y = 1;
-        attr[cfg.numAttrs].val.clusterDim.z = 1;
-        cfg.numAttrs++;
-      }
-      cfg.attrs = attr;
-      e = cudaLaunchKernelEx(&cfg, kernel, p);
-      return e == cudaSuccess ? APNN_OK : cuda_fail(e, "linear_few_rows_kernel");
-    }
+    cfg.attrs = attr;
+    e = cudaLaunchKernelEx(&cfg, kernel, p);
+    return e == cudaSuccess ? APNN_OK : cuda_fail(e, "linear_few_rows_kernel");
   }
   return linear_tile(reinterpret_cast<cudaStream_t>(stream), p, d->x_type == APNN_TYPE_BF16);
 }

@@ -552,16 +552,12 @@ __global__ void __launch_bounds__(Roles<CTAS>::THREADS, 1)
   }
 }
 
-struct Plan {
-  int ctas, tn, split;
-};
-
 // The plan of the shortest estimated time.  A wave of tiles takes its stages or its epilogue, whichever is longer, and the last
 // epilogue shows; a split adds the exchange.  The figures (us) are fitted to 24 shapes on every plan (16 to 4096 rows, 1000 to 32003
 // weights, K from 128 to 8192), most within a tenth: e.g. 333 x 2337 x 2296 13.2 on 64-wide tiles, 18.9 on the pair's 256;
 // 32 x 4096 x 4096 10.9 with K in four, 18.0 without.
-Plan pick_plan(int M, int N, int kblocks, int sms) {
-  Plan best = {1, 32, 1};
+LinearPlan pick_plan(int M, int N, int kblocks, int sms) {
+  LinearPlan best = {1, 32, 1};
   double least = 1e30;
   for (int ctas = 1; ctas <= 2; ctas++)
     for (int tn = ctas == 2 ? 64 : 32; tn <= 128 * ctas; tn *= 2)
@@ -621,13 +617,15 @@ apnn_status launch_bits(cudaStream_t s, const CUtensorMap& map, const CUtensorMa
 
 }  // namespace
 
+LinearPlan linear_tile_plan(int M, int N, int kwords) { return pick_plan(M, N, kwords / 2, device_sm_count()); }
+
 apnn_status linear_tile(cudaStream_t s, const LinearParams& l, bool bf16) {
   TileParams p = {};
   p.l = l;
   p.kblocks = l.kwords / 2;
   p.wide = !l.out_f32 && l.ldo % 2 == 0 && (reinterpret_cast<uintptr_t>(l.out) & 3u) == 0;
   const int sms = device_sm_count();
-  const Plan plan = pick_plan(l.M, l.N, p.kblocks, sms);
+  const LinearPlan plan = linear_tile_plan(l.M, l.N, l.kwords);
   p.tn = plan.tn;
   p.split = plan.split;
   p.tiles_x = (l.M + plan.tn - 1) / plan.tn;

@@ -419,6 +419,10 @@ typedef struct apnn_linear_desc {
 apnn_status apnn_linear_planes(void *stream, int wbits, const void *W, const void *X, void *Out, int M, int N, int K,
                                const apnn_linear_desc *desc, int *status_flag);
 
+/* Which kernel a product of these sizes takes on the current device: the blocks that share a tile of weight rows (2: a pair of
+ * 128 rows each; 1: a block alone; 0: the kernel of up to 8 rows), the rows of X in a tile, and the blocks that share its K. */
+apnn_status apnn_linear_planes_plan(int M, int N, int K, int *blocks, int *rows, int *split);
+
 /* A cache of keys and values in 4 bits, in pages.  A page holds `page_size` positions of every head; for each head
  *   key levels [page_size][D/2] (two per byte, the even element in the low half), value levels [page_size][D/2],
  *   (step, lowest) of every key row [page_size][2], (step, lowest) of every value row [page_size][2], in `type`,
