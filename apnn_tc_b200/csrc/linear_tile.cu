@@ -1,7 +1,7 @@
 // Matrix product over weight planes for more than a few rows of X, on tcgen05.
 //
 // The weights are the M operand of tcgen05.mma kind::f16 (128 of them to a block, 256 to a pair of blocks with cta_group::2), rows of X
-// the N operand (tiles of 32 to 256), so a thread of the epilogue owns one weight row: its scale and bias stay in registers and a warp
+// the N operand (tiles of 32 to 128, a pair's 256), so a thread of the epilogue owns one weight row: its scale and bias stay in registers and a warp
 // stores 32 neighbouring columns of one row of the output.  X comes by TMA (128-byte swizzle, zeros beyond its edges), and so do the
 // planes, 512 elements of K of every row at a time into a ring of two (loads of 8 bytes from 128 rows took as many L1
 // cycles as a stage's MMAs: 0.74 against 0.43 ms at 4096 x 16384 x 4096, 4 bits).  The weights never exist as 16-bit floats in
@@ -560,14 +560,14 @@ LinearPlan pick_plan(int M, int N, int kblocks, int sms) {
   LinearPlan best = {1, 32, 1};
   double least = 1e30;
   for (int ctas = 1; ctas <= 2; ctas++)
-    for (int tn = ctas == 2 ? 64 : 32; tn <= 128 * ctas; tn *= 2)
+    for (int tn = ctas == 2 ? 256 : 32; tn <= 128 * ctas; tn *= 2)      // a pair: its full width alone, narrower ones were never shortest
       for (int split = 1; split <= (ctas == 2 ? 1 : MAX_SPLIT) && 2 * split <= kblocks; split *= 2) {
         if (tn / split < 4) continue;
         const long long tiles = (long long)((M + tn - 1) / tn) * ((N + ROWS * ctas - 1) / (ROWS * ctas));
         // a cluster finds its blocks within one group of SMs: the driver knows how many fit
         const int slots = split > 1 ? cluster_capacity(reinterpret_cast<const void*>(linear_tile_kernel<4, true, 1>), Roles<1>::THREADS, SMEM_BYTES, split) : sms / ctas;
         if (slots < 1) continue;
-        const double stage = ctas == 1 ? (tn <= 64 ? 0.185 : 0.2) : (tn == 64 ? 0.265 : tn == 128 ? 0.285 : 0.355);
+        const double stage = ctas == 1 ? (tn <= 64 ? 0.185 : 0.2) : 0.355;
         const double epilogue = (ctas == 1 ? 0.8 : 1.4) + 0.012 * tn;
         const double stages = stage * (double)((kblocks / 2 + split - 1) / split * 2);
         const double exchange = split > 1 ? 1.5 + 0.1 * (tn / split) + 0.015 * tn : 0.0;
