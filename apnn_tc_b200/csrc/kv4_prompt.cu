@@ -15,9 +15,9 @@
 // the first tile on whose steps lie too far from those before, weights are taken against a second reference point of each row.
 // Registers: 96 / 184 / 184 / 48 for the four warpgroups out of the 128 each was launched with (setmaxnreg; a thread keeps 128 scores).
 // Bounds per 128 x 128 tile and 128 elements: 1024 clk of MMAs, 1024 of exponentials, about 950 issue slots of softmax and 200 of
-// spreading (one K / V tile serves both row tiles).  Measured: 8192 tokens, 32 heads on 8, causal, 881 us, 624 TFLOP/s, 0.37 of the
-// tensor cores' rate; a row tile's turn takes some 3200 clk, nearly all of it the one softmax warp a row tile has on a scheduler,
-// whose loads, packed products, exponentials and roundings wait on one another (instructions issue in 35% of the cycles).  Sixteen
+// spreading (one K / V tile serves both row tiles).  Measured: 8192 tokens, 32 heads on 8, causal, 850 us, 647 TFLOP/s, 0.38 of the
+// tensor cores' rate; a row tile's turn takes some 3100 clk, nearly all of it the one softmax warp a row tile has on a scheduler,
+// whose loads, packed products, exponentials and roundings wait on one another (instructions issue in 44% of the cycles).  Sixteen
 // softmax warps had too few registers for a row of scores and took 1.22 ms; scalar products in place of packed ones 1.02 ms.
 // Few units and many keys: the keys are split over blocks and kv4_prompt_join_kernel adds the parts in order.
 #include <type_traits>

@@ -400,7 +400,8 @@ enum {
  * rows ldx elements apart, Out and residual with rows ldo and ldr apart.  Sums in 32 bits, one rounding at the store.
  * zero: a multiple of 1/2 in 0..15, so that level - zero is exact in either type (1/2 with one plane: weights of
  * -scale/2 and +scale/2; (2^wbits - 1)/2: symmetric levels).  bias and residual may be null; residual may be Out itself
- * (same stride).  Values of X that are not finite make their row NaN or infinite and touch no other row.
+ * (same stride).  silu is held to (|v| + 4) 2^-23 of itself, gelu_tanh to (9 |sqrt(2/pi) (v + 0.044715 v^3)| + 4) 2^-23 of
+ * itself, gelu to |v| 2^-22; fp32 sums are a tensor core's, which truncates.  Values of X that are not finite make their row NaN or infinite and touch no other row.
  * Rules: W, X 16-byte aligned, ldx a multiple of 8; Out and residual aligned to their element; M, N, K >= 1 (ragged edges handled),
  * M and N * wbits up to 2^31 - 257, K up to 2^31 - 513 (else APNN_ERR_UNSUPPORTED).
  * status_flag: null, or 4 bytes of device memory, written 0 at launch and non-zero if a bounded wait expires. */
